@@ -11,6 +11,7 @@ overlap_worker.py:104-127).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -67,6 +68,15 @@ class DecodeCall(ctypes.Structure):
     ]  # fmt: skip
 
 
+class ScoreMods(ctypes.Structure):
+    """``bsgl_score_mods`` of include/bsgl_attn.h."""
+
+    _fields_ = [
+        ("logit_cap", _f32), ("slopes", _vp), ("visible_from", _vp), ("visible_to", _vp),
+        ("token_weights", _vp), ("token_weights_out", _vp), ("weights_row_stride", _i64),
+    ]  # fmt: skip
+
+
 # out .. out_cache_loc: the ten 8-byte fields a caller rewrites on every call, as one packed write
 DECODE_CALL_HEAD = struct.Struct("=10q")
 assert DecodeCall.out.offset == 0 and DecodeCall.out_cache_loc.offset == 72 and DecodeCall.k_slab.offset == 80
@@ -98,6 +108,8 @@ SIGNATURES = {
         + [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp]
         + [_i32, _i32, _i32, _i32, _f32, _i32, _i32, _i32, _i32, _vp],
     ),
+    "bsgl_decode_scored_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
+    "bsgl_paged_decode_scored": (ctypes.c_int, [ctypes.POINTER(DecodeCall), ctypes.POINTER(ScoreMods)]),
     "bsgl_prefill_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "bsgl_paged_prefill": (
         ctypes.c_int,
@@ -224,6 +236,39 @@ def _rows3(x: torch.Tensor):
     else:
         raise ValueError(f"expected a 2-D or 3-D tensor, got shape {tuple(sh)}")
     return x, sh, st
+
+
+def _on_device(device: torch.device):
+    """The tensors' device made current for the launch (a launch goes to the current device, whatever
+    stream it names)."""
+    return contextlib.nullcontext() if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _check_out(out: torch.Tensor, rows: int, width: int, dtype: torch.dtype) -> None:
+    if tuple(out.shape) != (rows, width) or out.dtype != dtype or (rows > 0 and out.stride(1) != 1) or not out.is_cuda:
+        raise ValueError(f"out must be {dtype} [{rows}, {width}] with unit column stride on the GPU, got {out.dtype} {tuple(out.shape)}")
+
+
+def _check_slabs(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor, dim: int) -> None:
+    if k_slab.dtype != q.dtype or v_slab.dtype != q.dtype:
+        raise ValueError(f"q is {q.dtype} but the KV slabs are {k_slab.dtype}")
+    if k_slab.dim() != 3 or k_slab.shape != v_slab.shape or k_slab.shape[2] != dim:
+        raise ValueError(f"KV slabs must be [slots, kv heads, {dim}], got {tuple(k_slab.shape)} and {tuple(v_slab.shape)}")
+    if k_slab.stride() != v_slab.stride() or k_slab.stride(2) != 1 or k_slab.stride(1) != dim:
+        raise ValueError("K and V slabs must share a row stride and have dense rows")
+
+
+def _check_table(req_to_token: torch.Tensor) -> None:
+    if req_to_token.dim() != 2 or req_to_token.dtype != torch.int32 or req_to_token.stride(1) != 1:
+        raise ValueError("req_to_token must be a 2-D int32 tensor with unit column stride")
+
+
+def _index_rows(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    """A dense int64 vector of ``n`` entries on the GPU."""
+    if tuple(t.shape) != (n,):
+        raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
+    t = t if t.dtype == torch.int64 else t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def kv_scatter(k_slab, v_slab, loc, k_new, v_new) -> None:
@@ -413,6 +458,162 @@ def paged_decode(
         _plan[1] if _plan is not None else _stream_ptr(q.device),
     )  # fmt: skip
     _check(rc, "bsgl_paged_decode")
+    return out
+
+
+# ---- scored attention ---------------------------------------------------------------------------
+
+
+def _score_mods(rows: int, n_q_heads: int, device, logit_cap, slopes, visible_from, visible_to):
+    """A ``ScoreMods`` with its checks; the tensors it points into are returned beside it (the caller
+    keeps them until the call has been made)."""
+    m = ScoreMods()
+    cap = float(logit_cap or 0.0)
+    if not (0.0 <= cap < math.inf):
+        raise ValueError(f"logit_cap {logit_cap} is negative or not finite")
+    m.logit_cap = cap
+    keep = []
+    if slopes is not None:
+        _need_gpu(slopes)
+        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (n_q_heads,):
+            raise ValueError(f"slopes must be float32 of shape ({n_q_heads},), got {slopes.dtype} {tuple(slopes.shape)}")
+        slopes = slopes if slopes.is_contiguous() else slopes.contiguous()
+        keep.append(slopes)
+        m.slopes = slopes.data_ptr()
+    for name, t in (("visible_from", visible_from), ("visible_to", visible_to)):
+        if t is None:
+            continue
+        _need_gpu(t)
+        if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (rows,):
+            raise ValueError(f"{name} must be int32 of shape ({rows},), got {t.dtype} {tuple(t.shape)}")
+        if t.dtype == torch.int64:  # (positions fit 32 bits; what does not stays outside the sequence either way)
+            t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+        t = t if t.is_contiguous() else t.contiguous()
+        keep.append(t)
+        setattr(m, name, t.data_ptr())
+    for t in keep:
+        if t.device != device:
+            raise ValueError(f"score tensors must be on q's device {device}, got {t.device}")
+    return m, keep
+
+
+def decode_scored_workspace_bytes(
+    batch: int, n_q_heads: int, head_dim: int, n_splits: int, table_cols: int, with_weights: bool, out_is_f32: bool = False
+) -> int:
+    return lib.bsgl_decode_scored_workspace_bytes(batch, n_q_heads, head_dim, n_splits, int(out_is_f32), table_cols, int(with_weights))
+
+
+def paged_decode_scored(
+    q: torch.Tensor,
+    k_slab: torch.Tensor,
+    v_slab: torch.Tensor,
+    req_to_token: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scale: Optional[float] = None,
+    logit_cap: float = 0.0,
+    slopes: Optional[torch.Tensor] = None,
+    visible_from: Optional[torch.Tensor] = None,
+    visible_to: Optional[torch.Tensor] = None,
+    token_weights: Optional[torch.Tensor] = None,
+    token_weights_out: Optional[torch.Tensor] = None,
+    n_splits: Optional[int] = None,
+    variant: int = DECODE_AUTO,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+    out_dtype: Optional[torch.dtype] = None,
+    k_new: Optional[torch.Tensor] = None,
+    v_new: Optional[torch.Tensor] = None,
+    out_cache_loc: Optional[torch.Tensor] = None,
+    fuse_kv_write: bool = False,
+    max_seq_len: int = 0,
+) -> torch.Tensor:
+    """``paged_decode`` with scored attention (``bsgl_paged_decode_scored``); returns [B, Hq * D].
+
+    ``s = scale q.k``, then ``logit_cap * tanh(s / logit_cap)`` (0: no cap), then
+    ``- slopes[head] * distance`` (float32 [Hq]), over the positions ``[visible_from, visible_to)`` of
+    each request (int32 [B], clamped to the request; default: all of it).  A request that may see
+    nothing gets a zero row.
+
+    ``token_weights`` (float32, [table rows, table columns]): the softmax weight every visible token
+    received, summed over the q heads, is added to it in place -- or, with ``token_weights_out``, the
+    sum goes there (at the visible entries; nothing else of it is touched).  ``workspace`` then holds
+    ``decode_scored_workspace_bytes``; like every decode workspace it must have been created zero-filled.
+    The other arguments are ``paged_decode``'s.
+    """
+    _need_gpu(q, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens)
+    q, q_shape, q_stride = _rows3(q)
+    if len(q_shape) != 3:
+        raise ValueError(f"q must be [batch, heads, dim], got shape {tuple(q_shape)}")
+    batch, hq, dim = q_shape
+    hkv = k_slab.shape[1]
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else q.dtype
+    if out is None:
+        out = torch.empty((batch, hq * dim), dtype=out_dtype, device=q.device)
+    _check_out(out, batch, hq * dim, out_dtype)
+    if batch == 0:
+        return out
+    _check_slabs(q, k_slab, v_slab, dim)
+    _check_table(req_to_token)
+    rows, lens = (_index_rows(t, batch, n) for t, n in ((req_pool_indices, "req_pool_indices"), (seq_lens, "seq_lens")))
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    cols = req_to_token.shape[1]
+    if n_splits is None:
+        n_splits = decode_num_splits(batch, hkv, cols)
+    mods, keep = _score_mods(batch, hq, q.device, logit_cap, slopes, visible_from, visible_to)
+    if token_weights is None and token_weights_out is not None:
+        raise ValueError("token_weights_out without token_weights")
+    if token_weights is not None:
+        if token_weights_out is None:
+            token_weights_out = token_weights
+        for t in (token_weights, token_weights_out):
+            _need_gpu(t)
+            if t.dtype != torch.float32 or t.shape != req_to_token.shape or t.stride(1) != 1 or t.stride(0) < cols:
+                raise ValueError(f"token weights must be float32 of the page table's shape {tuple(req_to_token.shape)} with dense rows")
+        if token_weights.stride(0) != token_weights_out.stride(0):
+            raise ValueError("token_weights and token_weights_out must share a row stride")
+        mods.token_weights, mods.token_weights_out = token_weights.data_ptr(), token_weights_out.data_ptr()
+        mods.weights_row_stride = token_weights.stride(0)
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (batch, hq) or not lse.is_contiguous()):
+        raise ValueError(f"lse must be dense float32 [{batch}, {hq}]")
+    need = decode_scored_workspace_bytes(batch, hq, dim, n_splits, cols, token_weights is not None, out_dtype != q.dtype)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = new_decode_workspace(need, q.device)
+    c = DecodeCall()
+    if k_new is not None or v_new is not None or out_cache_loc is not None:
+        if k_new is None or v_new is None or out_cache_loc is None:
+            raise ValueError("k_new, v_new and out_cache_loc go together")
+        k_new, kn_shape, kn_stride = _rows3(k_new.view(batch, hkv, dim) if k_new.dim() == 2 else k_new)
+        v_new, vn_shape, vn_stride = _rows3(v_new.view(batch, hkv, dim) if v_new.dim() == 2 else v_new)
+        if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
+            raise ValueError("new K/V rows must have q's dtype")
+        if tuple(kn_shape) != (batch, hkv, dim) or tuple(vn_shape) != (batch, hkv, dim):
+            raise ValueError("new K/V rows must be [batch, n_kv_heads, head_dim]")
+        loc = out_cache_loc if out_cache_loc.dtype == torch.int32 else out_cache_loc.to(torch.int32)
+        loc = loc if loc.is_contiguous() else loc.contiguous()
+        if tuple(loc.shape) != (batch,):
+            raise ValueError("out_cache_loc must have one slot per request")
+        c.k_new, c.v_new, c.k_new_row_stride, c.v_new_row_stride = k_new.data_ptr(), v_new.data_ptr(), kn_stride[0], vn_stride[0]
+        c.out_cache_loc = loc.data_ptr()
+        if fuse_kv_write:
+            variant |= DECODE_FUSE_KV_WRITE
+    c.out, c.out_row_stride, c.lse = out.data_ptr(), out.stride(0), lse.data_ptr() if lse is not None else None
+    c.q, c.q_row_stride = q.data_ptr(), q_stride[0]
+    c.k_slab, c.v_slab, c.slab_row_stride, c.n_slots = k_slab.data_ptr(), v_slab.data_ptr(), k_slab.stride(0), k_slab.shape[0]
+    c.req_to_token, c.table_row_stride = req_to_token.data_ptr(), req_to_token.stride(0)
+    c.table_rows, c.table_cols = req_to_token.shape
+    c.req_pool_indices, c.seq_lens = rows.data_ptr(), lens.data_ptr()
+    c.batch, c.n_q_heads, c.n_kv_heads, c.head_dim, c.scale = batch, hq, hkv, dim, scale
+    c.dtype, c.out_dtype, c.n_splits, c.variant = _dtype_code(q), _DTYPE_CODE[out_dtype], n_splits, variant
+    c.max_seq_len = int(max_seq_len)
+    c.workspace = workspace.data_ptr() if need else None
+    c.workspace_bytes = workspace.numel() * workspace.element_size() if need else 0
+    with _on_device(q.device):
+        c.stream = _stream_ptr(q.device)
+        _check(lib.bsgl_paged_decode_scored(ctypes.byref(c), ctypes.byref(mods)), "bsgl_paged_decode_scored")
     return out
 
 

@@ -51,6 +51,23 @@ struct PagedKV {
   int64_t table_cols;
 };
 
+// What happens to a score between q . k and the softmax (scored forms of decode and extend):
+//   s = scale * q . k;  s = cap * tanh(s / cap) when cap > 0;  s -= slopes[head] * |i - j|
+// for query position i and token position j, and the row sees positions [from, to) only.
+struct ScoreMods {
+  float cap;             // 0: none
+  const float* slopes;   // [n_q_heads], NULL: none
+  const int32_t* from;   // [rows], NULL: 0
+  const int32_t* to;     // [rows], NULL: the row's own position + 1
+  // generic extend path: {page-table row, request length, own position, 0} of every extend token (NULL: decode,
+  // whose rows are the requests and whose own position is the last)
+  const int4* rows;
+  // decode: the finished scores in units of log2, [rows, n_q_heads, score_stride], token t of the VISIBLE ones
+  // at column t (NULL: not kept); score_stride is a multiple of 16
+  float* scores;
+  int64_t score_stride;
+};
+
 // One attention "query row": decode has one per request, prefill one per
 // extend token (req / len arrays are then the expanded per-token ones).
 struct DecodeArgs {
@@ -101,6 +118,24 @@ struct DecodeArgs {
   // configuration only): 8 x uint64 per workgroup (in launch order): start, after
   // the prologue, after the streaming loop, end (100 MHz ticks), XCC id, HW id, row, piece
   uint64_t* trace;
+  bool scored;  // the scored forms of the kernels, with these:
+  ScoreMods mods;
+};
+
+// token_weights[req[i], from_i + t] = old + sum over heads of exp2(scores[i, h, t] - lse[i, h] * log2 e)
+struct WeightsArgs {
+  const float* old;   // [table_rows, table_cols] with row_stride; may be `out`
+  float* out;
+  int64_t row_stride;
+  const float* lse;   // [rows, n_q_heads]
+  const int64_t* req_idx;
+  const int64_t* seq_lens;
+  int64_t table_rows;
+  int64_t table_cols;
+  int32_t rows;
+  int32_t n_q_heads;
+  int32_t len_hint;  // no request is longer (0: unknown); shapes the launch only
+  ScoreMods mods;
 };
 
 struct MergeArgs {
@@ -226,6 +261,7 @@ int rmsnorm_max_hidden(int dtype);
 hipError_t launch_rope_kv(const RopeArgs& a, hipStream_t stream);
 
 hipError_t launch_merge(const MergeArgs& a, hipStream_t stream);
+hipError_t launch_token_weights(const WeightsArgs& a, hipStream_t stream);
 hipError_t launch_kv_scatter(const ScatterArgs& a, hipStream_t stream);
 hipError_t launch_prefill_expand(const ExpandArgs& a, hipStream_t stream);
 

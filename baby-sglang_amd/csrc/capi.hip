@@ -383,6 +383,24 @@ int scratch_of_current_device(void** out, bool capturing) {
   return BSGL_OK;
 }
 
+// the description of a scored call into a launch's arguments
+int take_mods(bsgl::DecodeArgs& a, const bsgl_score_mods& m, int32_t n_q_heads) {
+  (void)n_q_heads;
+  if (!(m.logit_cap >= 0.f) || m.logit_cap > 3.0e38f) return fail(BSGL_ERR_BAD_ARG, "logit_cap %g is negative or not finite", (double)m.logit_cap);
+  a.scored = true;
+  a.mods.cap = m.logit_cap;
+  a.mods.slopes = m.slopes;
+  a.mods.from = m.visible_from;
+  a.mods.to = m.visible_to;
+  return BSGL_OK;
+}
+
+// Scored decode with token weights: the log-sum-exps and scores start behind the decode workspace -- and
+// never inside its ticket area, also where this call's own decode needs no workspace at all: one buffer serves
+// calls of different split counts.
+size_t scored_head_bytes(size_t decode_need) { return align_up(decode_need > kCounterBytes ? decode_need : kCounterBytes, 256); }
+int64_t score_row(int64_t table_cols) { return (table_cols + 15) / 16 * 16; }
+
 int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, int64_t q_row_stride,
                  const void* k_new, const void* v_new, int64_t k_new_row_stride, int64_t v_new_row_stride,
                  const int32_t* out_cache_loc,
@@ -391,7 +409,8 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
                  int64_t table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
                  int32_t batch, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
                  int32_t dtype, int32_t out_dtype, int32_t n_splits, int32_t variant,
-                 void* workspace, size_t workspace_bytes, bool static_scratch, int32_t max_seq_len, void* stream) {
+                 void* workspace, size_t workspace_bytes, bool static_scratch, int32_t max_seq_len, void* stream,
+                 const bsgl_score_mods* mods = nullptr) {
   if (batch < 0) return fail(BSGL_ERR_BAD_ARG, "batch < 0");
   if (out_dtype != dtype && out_dtype != BSGL_DTYPE_F32)
     return fail(BSGL_ERR_BAD_ARG, "out_dtype must equal dtype or be f32");
@@ -465,14 +484,66 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
   a.out_dtype = out_dtype;
   a.n_splits = n_splits;
   a.len_hint = max_seq_len > 0 ? max_seq_len : 0;
+  if (mods != nullptr) {
+    if (int rc = take_mods(a, *mods, n_q_heads)) return rc;
+    if (mods->token_weights != nullptr) {
+      const size_t all = bsgl_decode_scored_workspace_bytes(batch, n_q_heads, head_dim, n_splits, f32_out, table_cols, 1);
+      if (workspace == nullptr || workspace_bytes < all || !aligned16(workspace))
+        return fail(BSGL_ERR_WORKSPACE, "scored decode with token weights needs a 16-byte aligned workspace of %zu bytes (got %zu)", all, workspace ? workspace_bytes : (size_t)0);
+      char* tail = (char*)workspace + scored_head_bytes(need);
+      if (a.lse == nullptr) a.lse = (float*)tail;
+      a.mods.scores = (float*)(tail + align_up((size_t)batch * (size_t)n_q_heads * 4, 256));
+      a.mods.score_stride = score_row(table_cols);
+    }
+  }
   const size_t rh = (size_t)batch * (size_t)n_q_heads;
   const size_t cb = kCounterBytes;
   a.ws_o = need ? (float*)((char*)workspace + cb) : nullptr;
   a.ws_lse = need ? (float*)((char*)workspace + cb + align_up((size_t)n_splits * rh * partial_row_width(head_dim) * 4, 256)) : nullptr;
-  return run_decode(a, variant, need ? (uint32_t*)workspace : nullptr, (hipStream_t)stream);
+  bsgl::WeightsArgs w{};
+  if (a.mods.scores != nullptr) {
+    w.old = mods->token_weights;
+    w.out = mods->token_weights_out;
+    w.row_stride = mods->weights_row_stride;
+    w.lse = a.lse;
+    w.req_idx = req_pool_indices;
+    w.seq_lens = seq_lens;
+    w.table_rows = table_rows;
+    w.table_cols = table_cols;
+    w.rows = batch;
+    w.n_q_heads = n_q_heads;
+    w.len_hint = a.len_hint;
+    w.mods = a.mods;
+  }
+  const int rc = run_decode(a, variant, need ? (uint32_t*)workspace : nullptr, (hipStream_t)stream);
+  if (rc != BSGL_OK || w.out == nullptr) return rc;
+  const hipError_t ew = bsgl::launch_token_weights(w, (hipStream_t)stream);
+  if (ew != hipSuccess) return hip_fail("token weight launch", ew);
+  return BSGL_OK;
 }
 
 }  // namespace
+
+size_t bsgl_decode_scored_workspace_bytes(int32_t batch, int32_t n_q_heads, int32_t head_dim, int32_t n_splits,
+                                          int32_t out_is_f32, int64_t table_cols, int32_t with_weights) {
+  const size_t need = bsgl_decode_workspace_bytes(batch, n_q_heads, head_dim, n_splits, out_is_f32);
+  if (!with_weights || batch <= 0 || n_q_heads <= 0 || table_cols <= 0) return need;
+  const size_t rh = (size_t)batch * (size_t)n_q_heads;
+  return scored_head_bytes(need) + align_up(rh * 4, 256) + rh * (size_t)score_row(table_cols) * 4;
+}
+
+int bsgl_paged_decode_scored(const bsgl_decode_call* c, const bsgl_score_mods* mods) {
+  if (c == nullptr || mods == nullptr) return fail(BSGL_ERR_BAD_ARG, "null call descriptor or score description");
+  if ((mods->token_weights == nullptr) != (mods->token_weights_out == nullptr))
+    return fail(BSGL_ERR_BAD_ARG, "token_weights and token_weights_out go together");
+  if (mods->token_weights != nullptr && mods->weights_row_stride < c->table_cols)
+    return fail(BSGL_ERR_BAD_ARG, "token weight row stride shorter than the page table's column count");
+  return decode_entry(c->out, c->out_row_stride, c->lse, c->q, c->q_row_stride, c->k_new, c->v_new, c->k_new_row_stride,
+                      c->v_new_row_stride, c->out_cache_loc, c->k_slab, c->v_slab, c->slab_row_stride, c->n_slots,
+                      c->req_to_token, c->table_row_stride, c->table_rows, c->table_cols, c->req_pool_indices, c->seq_lens,
+                      c->batch, c->n_q_heads, c->n_kv_heads, c->head_dim, c->scale, c->dtype, c->out_dtype, c->n_splits,
+                      c->variant, c->workspace, c->workspace_bytes, false, c->max_seq_len, c->stream, mods);
+}
 
 int bsgl_paged_decode(void* out, int64_t out_row_stride, float* lse, const void* q, int64_t q_row_stride,
                       const void* k_new, const void* v_new, int64_t k_new_row_stride, int64_t v_new_row_stride,

@@ -51,9 +51,16 @@
 // are zero before and after every launch.  (Drawing the ticket early and letting
 // the last drawer wait for a "ready" count was measured and is slower: under
 // load every trip to memory costs about 2.3 us, and the wait adds trips.)
+//
+// Scored form (SCORED, DecodeArgs::mods): the scores go through cap * tanh(s / cap), minus slope[head] * distance,
+// and a row sees the positions [from, to) of its request only.  The interval is cut out before anything else
+// -- a row's length is to - from and its page-table row starts at `from` -- so tokens outside it are never
+// read, whatever they hold.  The finished scores can be kept (mods.scores, 16 bytes per lane and tile) for
+// token_weights.hip.  A build of its own: the plain form's code is what it was.
 #include "bsgl_device.h"
 #include "bsgl_launch.h"
 #include "bsgl_mfma.h"
+#include "bsgl_score.h"
 
 #include <type_traits>
 
@@ -82,7 +89,7 @@ __device__ __forceinline__ int small_div(int x, int d) {
 // ring of its own -- a wave's tile rate is set by its 8 LDS-DMA instructions per tile, so W waves
 // stream a piece W times as fast -- and wave 0 adds up their (m, l, O) in LDS before the piece's
 // result is stored, so the number of parts the split merge sees does not grow.
-template <typename Tag, int HPT, int NSTAGE, bool NT, int W = 1, bool TRACE = false>
+template <typename Tag, int HPT, int NSTAGE, bool NT, int W = 1, bool TRACE = false, bool SCORED = false>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2)))
 void decode_mfma_kernel(DecodeArgs a) {
   using E = Elem<Tag>;
@@ -128,7 +135,9 @@ void decode_mfma_kernel(DecodeArgs a) {
   auto len_of = [&](int i) {
     const int64_t s64 = i < a.rows ? a.seq_lens[i] : 0;
     const int64_t cap = a.kv.table_cols < (1 << 20) ? a.kv.table_cols : (1 << 20);
-    return (int)(s64 < 0 ? 0 : (s64 > cap ? cap : s64));
+    const int s = (int)(s64 < 0 ? 0 : (s64 > cap ? cap : s64));
+    if constexpr (SCORED) return i < a.rows ? visible_range(a.mods, i, s, s).y : 0;
+    return s;
   };
   auto req_of = [&](int i) {
     const int64_t r64 = i < a.rows ? a.req_idx[i] : 0;
@@ -262,6 +271,13 @@ void decode_mfma_kernel(DecodeArgs a) {
   // ---- this row's token range (multiples of the tile so splits start on tiles) ----
   int64_t req;
   int seq;
+  int row_len = 0, row_first = 0;  // (scored form) the request's length, and the first position the row sees
+  if constexpr (SCORED) {
+    // (scalar loads beside the ones below: they leave together)
+    const int64_t s64 = a.seq_lens[row];
+    row_len = (int)(s64 < 0 ? 0 : (s64 > a.kv.table_cols ? a.kv.table_cols : s64));
+    row_first = visible_range(a.mods, row, row_len, row_len).x;
+  }
   if (a.balance_target > 0) {
     req = flat_req;
     seq = flat_seq;
@@ -270,13 +286,14 @@ void decode_mfma_kernel(DecodeArgs a) {
     req = req < 0 ? 0 : (req >= a.kv.table_rows ? a.kv.table_rows - 1 : req);
     const int64_t seq64 = a.seq_lens[row];
     seq = (int)(seq64 < 0 ? 0 : (seq64 > a.kv.table_cols ? a.kv.table_cols : seq64));
+    if constexpr (SCORED) seq = visible_range(a.mods, row, seq, seq).y;
   }
   // the row's pieces are equal among themselves (a piece past the end is empty)
   int chunk = a.balance_target > 0 ? small_div(seq + n_parts - 1, n_parts) : (seq + n_parts - 1) / n_parts;  // (flat grid: seq <= 2^20)
   chunk = (chunk + kTile - 1) / kTile * kTile;
   const int start = split * chunk;
   const int end = (split == n_parts - 1) ? seq : min(seq, start + chunk);
-  const int32_t* table_row = a.kv.table + req * a.kv.table_row_stride;
+  const int32_t* table_row = a.kv.table + req * a.kv.table_row_stride + (SCORED ? row_first : 0);
   const uint32_t max_slot = (uint32_t)(a.kv.n_slots - 1);
   const uint32_t row_units = (uint32_t)(a.kv.slab_row_stride * 2 / 16);
 
@@ -323,6 +340,17 @@ void decode_mfma_kernel(DecodeArgs a) {
       }
   }
   const float scale_log2e = a.scale * kLog2e;
+  ScoreShape shape[HPT];  // (scored form) one q head per lane
+  float* score_dst[HPT];
+  if constexpr (SCORED) {
+#pragma unroll
+    for (int hh = 0; hh < HPT; ++hh) {
+      const int h = (head0 + hh) * G + min(lq, G - 1);
+      shape[hh] = ScoreShape(a.mods, a.scale, h);
+      score_dst[hh] = a.mods.scores == nullptr ? nullptr
+                                               : a.mods.scores + ((int64_t)row * a.n_q_heads + h) * a.mods.score_stride + 4 * lg;
+    }
+  }
 
   // ---- per-lane DMA source: which piece of a token record this lane moves ----------
   const int piece = lane % (REC / 16);             // 16-byte piece inside the record
@@ -453,8 +481,20 @@ void decode_mfma_kernel(DecodeArgs a) {
         float tmax = kNegInf;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          sv[r] = (4 * lg + r < n_valid) ? sc[r] * scale_log2e : kNegInf;
+          if constexpr (SCORED) {
+            const int t = blk + tile * kTile + 4 * lg + r;  // token of the visible ones
+            sv[r] = (4 * lg + r < n_valid) ? shape[hh].fast(sc[r], (float)(row_len - 1 - row_first - t)) : kNegInf;
+          } else {
+            sv[r] = (4 * lg + r < n_valid) ? sc[r] * scale_log2e : kNegInf;
+          }
           tmax = fmaxf(tmax, sv[r]);
+        }
+        if constexpr (SCORED) {
+          // the tile's finished scores, four tokens of a head per lane (a row of the buffer has room for whole
+          // tiles).  The stores count in vmcnt behind the requests of the tile after this one: the waits below
+          // then wait for more than they need, never for less.
+          if (score_dst[hh] != nullptr && lq < G)
+            *(f32x4*)(score_dst[hh] + blk + tile * kTile) = f32x4{sv[0], sv[1], sv[2], sv[3]};
         }
         tmax = quad_group_max(tmax);
         if (__any(tmax > m_run[hh])) {
@@ -749,6 +789,33 @@ void decode_mfma_kernel(DecodeArgs a) {
 
 uint64_t* g_trace = nullptr;
 
+// the waves that share a piece: see launch_tag
+int decode_waves(const DecodeArgs& a) {
+  const int64_t n_pieces = (int64_t)a.rows * a.n_kv_heads * (a.balance_target > 0 ? a.balance_target : a.n_splits);
+  int waves = n_pieces > 512 ? 1 : 4;
+  // (folded kv heads keep a wave busier per tile -- up to 16 q heads -- and gain from a second wave a
+  // little longer: 80 - 96 requests of the 0.5B shapes, 1024 / 2048 / 4095 tokens: -8..-11 % / -2..-6 % / +-1 %)
+  if (a.fold_group > 0 && n_pieces > 512 && n_pieces <= 768) waves = 2;
+  if (a.balance_target > 0 && (a.hint_waves == 1 || a.hint_waves == 2 || a.hint_waves == 4)) waves = a.hint_waves;
+  const int forced = knob(kKnobMfmaWaves);  // tuning override
+  if (forced == 1 || forced == 2 || forced == 4) waves = forced;
+  return waves;
+}
+
+// the scored form: the default ring (two stages, non-temporal requests, one kv head per workgroup) in all
+// three widths; the plain form's rules for the launch
+template <typename Tag>
+hipError_t launch_scored(const DecodeArgs& a, hipStream_t stream) {
+  const int waves = decode_waves(a);
+  const int target = waves > 1 ? max(a.balance_target, a.balance_target_hi) : a.balance_target;
+  dim3 grid(a.rows, a.n_kv_heads, a.n_splits);
+  if (a.balance_target > 0) grid = dim3((unsigned)((int64_t)a.rows * (target + 1) * a.n_kv_heads), 1, 1);
+  if (waves == 1) hipLaunchKernelGGL((decode_mfma_kernel<Tag, 1, 2, true, 1, false, true>), grid, dim3(64), 0, stream, a);
+  else if (waves == 2) hipLaunchKernelGGL((decode_mfma_kernel<Tag, 1, 2, true, 2, false, true>), grid, dim3(128), 0, stream, a);
+  else hipLaunchKernelGGL((decode_mfma_kernel<Tag, 1, 2, true, 4, false, true>), grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
 template <typename Tag, int HPT, int NSTAGE>
 hipError_t launch_inst(const DecodeArgs& a, hipStream_t stream) {
   dim3 grid(a.rows, a.n_kv_heads / HPT, a.n_splits);
@@ -780,16 +847,7 @@ hipError_t launch_tag(const DecodeArgs& a, hipStream_t stream) {
   // else four waves share a piece.  (Two waves for 257 - 512 pieces were the rule before; four are
   // 2 - 8 % faster there: 24 requests x 2048 tokens 16.9 -> 15.6 us, 32 requests 17.9 -> 17.6.  Between
   // 512 and 1024 pieces two waves win at 1024 tokens and lose at 2048 and beyond.)
-  const int64_t n_pieces = (int64_t)a.rows * a.n_kv_heads * (a.balance_target > 0 ? a.balance_target : a.n_splits);
-  int waves = n_pieces > 512 ? 1 : 4;
-  // (folded kv heads keep a wave busier per tile -- up to 16 q heads -- and gain from a second wave a
-  // little longer: 80 - 96 requests of the 0.5B shapes, 1024 / 2048 / 4095 tokens: -8..-11 % / -2..-6 % / +-1 %)
-  if (a.fold_group > 0 && n_pieces > 512 && n_pieces <= 768) waves = 2;
-  if (a.balance_target > 0 && (a.hint_waves == 1 || a.hint_waves == 2 || a.hint_waves == 4)) waves = a.hint_waves;
-  {
-    const int forced = knob(kKnobMfmaWaves);  // tuning override
-    if (forced == 1 || forced == 2 || forced == 4) waves = forced;
-  }
+  const int waves = decode_waves(a);
   if (waves > 1 && knob(kKnobMfmaNT)) {
     dim3 grid(a.rows, a.n_kv_heads, a.n_splits);
     if (a.balance_target > 0) grid = dim3((unsigned)((int64_t)a.rows * (max(a.balance_target, a.balance_target_hi) + 1) * a.n_kv_heads), 1, 1);
@@ -835,7 +893,9 @@ hipError_t launch_decode_mfma(const DecodeArgs& a_in, hipStream_t stream) {
   if (a_in.rows == 0) return hipSuccess;
   DecodeArgs a = a_in;
   a.trace = g_trace;
-  hipError_t e = a.dtype == kBF16 ? launch_tag<bf16_tag>(a, stream) : launch_tag<f16_tag>(a, stream);
+  hipError_t e;
+  if (a.scored) e = a.dtype == kBF16 ? launch_scored<bf16_tag>(a, stream) : launch_scored<f16_tag>(a, stream);
+  else e = a.dtype == kBF16 ? launch_tag<bf16_tag>(a, stream) : launch_tag<f16_tag>(a, stream);
   if (e != hipSuccess || decode_direct_out(a) || a.counters != nullptr) return e;
   MergeArgs mg;
   mg.out = a.out;

@@ -14,8 +14,11 @@
 //   softmax is the online (running max / running sum) form in base 2.
 //   Per-wave states are merged through LDS, per-split states through a second
 //   small kernel (merge_states_kernel).
+// SCORED: the scores of DecodeArgs::mods, as in paged_decode_mfma.hip; with mods.rows a row is an extend
+// token whose own position is not the request's last.
 #include "bsgl_device.h"
 #include "bsgl_launch.h"
+#include "bsgl_score.h"
 
 namespace bsgl {
 
@@ -25,7 +28,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kSlotTile = 1024;  // page-table entries staged in LDS at a time
 
-template <typename Tag, int D, int G, int U>
+template <typename Tag, int D, int G, int U, bool SCORED = false>
 __global__ __launch_bounds__(kThreads) void decode_valu_kernel(DecodeArgs a, int hpw) {
   using E = Elem<Tag>;
   constexpr int VEC = E::VEC;
@@ -50,14 +53,29 @@ __global__ __launch_bounds__(kThreads) void decode_valu_kernel(DecodeArgs a, int
   const int kvh = blockIdx.y * hpw + head_local;
 
   // ---- this row's token range ------------------------------------------------
-  int64_t req = a.req_idx[row];
+  int64_t req, seq64;
+  int pos = 0, first = 0;  // (scored form) the row's own position, and the first one it sees
+  if (SCORED && a.mods.rows != nullptr) {
+    const int4 r4 = a.mods.rows[row];
+    req = r4.x;
+    seq64 = r4.y;
+    pos = r4.z;
+  } else {
+    req = a.req_idx[row];
+    seq64 = a.seq_lens[row];
+  }
   req = req < 0 ? 0 : (req >= a.kv.table_rows ? a.kv.table_rows - 1 : req);
-  int64_t seq64 = a.seq_lens[row];
-  const int seq = (int)(seq64 < 0 ? 0 : (seq64 > a.kv.table_cols ? a.kv.table_cols : seq64));
+  int seq = (int)(seq64 < 0 ? 0 : (seq64 > a.kv.table_cols ? a.kv.table_cols : seq64));
+  if constexpr (SCORED) {
+    if (a.mods.rows == nullptr) pos = seq - 1;
+    const int2 seen = visible_range(a.mods, row, seq, min(seq, pos + 1));
+    first = seen.x;
+    seq = seen.y;
+  }
   const int chunk = (seq + a.n_splits - 1) / a.n_splits;
   const int start = split * chunk;
   const int end = min(seq, start + chunk);
-  const int32_t* table_row = a.kv.table + req * a.kv.table_row_stride;
+  const int32_t* table_row = a.kv.table + req * a.kv.table_row_stride + first;
   const uint32_t max_slot = (uint32_t)(a.kv.n_slots - 1);
 
   // ---- q pieces (packed, as stored) -------------------------------------------
@@ -69,6 +87,11 @@ __global__ __launch_bounds__(kThreads) void decode_valu_kernel(DecodeArgs a, int
       qraw[g] = *(const uint4*)(qrow + ((int64_t)(kvh * G + g) * D + c * VEC) * E::BYTES);
   }
   const float scale_log2e = a.scale * kLog2e;
+  ScoreShape shape[SCORED ? G : 1];
+  if constexpr (SCORED) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) shape[g] = ScoreShape(a.mods, a.scale, kvh * G + g);
+  }
   const int64_t row_bytes = a.kv.slab_row_stride * E::BYTES;
   const int64_t piece_off = ((int64_t)kvh * D + c * VEC) * E::BYTES;
   const char* kbase = (const char*)a.kv.k_slab + piece_off;
@@ -114,7 +137,16 @@ __global__ __launch_bounds__(kThreads) void decode_valu_kernel(DecodeArgs a, int
       for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          float s = group_sum<LPR>(E::dot(qraw[g], kr[u], 0.f)) * scale_log2e;
+          float s = group_sum<LPR>(E::dot(qraw[g], kr[u], 0.f));
+          if constexpr (SCORED) {
+            const int t = blk + base + u * tpi + tok_sub;  // token of the visible ones
+            const float dist = (float)abs(pos - first - t);
+            s = E::BYTES == 4 ? shape[g].precise(s, dist) : shape[g].fast(s, dist);
+            if (a.mods.scores != nullptr && c == 0 && valid[u])
+              a.mods.scores[((int64_t)row * a.n_q_heads + kvh * G + g) * a.mods.score_stride + t] = s;
+          } else {
+            s *= scale_log2e;
+          }
           s = valid[u] ? s : kNegInf;
           p[u][g] = s;
           mt[g] = fmaxf(mt[g], s);
@@ -295,7 +327,8 @@ hipError_t launch_valu_inst(const DecodeArgs& a, hipStream_t stream) {
   while (hpw * 2 <= RPW && a.n_kv_heads % (hpw * 2) == 0) hpw *= 2;
   dim3 grid(a.rows, a.n_kv_heads / hpw, a.n_splits);
   constexpr int U = 4;
-  hipLaunchKernelGGL((decode_valu_kernel<Tag, D, G, U>), grid, dim3(kThreads), 0, stream, a, hpw);
+  if (a.scored) hipLaunchKernelGGL((decode_valu_kernel<Tag, D, G, U, true>), grid, dim3(kThreads), 0, stream, a, hpw);
+  else hipLaunchKernelGGL((decode_valu_kernel<Tag, D, G, U>), grid, dim3(kThreads), 0, stream, a, hpw);
   return hipGetLastError();
 }
 

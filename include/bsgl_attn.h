@@ -251,6 +251,47 @@ int bsgl_paged_decode_static(void* out /*device*/, int64_t out_row_stride,
                              int32_t variant, void* stream);
 
 /*
+ * Scored attention: what happens to a score between q . k and the softmax, in this order.  For the
+ * query at position i of its request, the cached token at position j and q head h
+ *   s = scale * q_h . k_j
+ *   s = logit_cap * tanh(s / logit_cap)        when logit_cap > 0 (0 = none; negative or not finite is refused)
+ *   s = s - slopes[h] * |i - j|                when slopes is given (fp32 [n_q_heads])
+ * and the row attends to j in [visible_from, visible_to) only: int32 per ROW of q (request of a decode
+ * call, extend token of a prefill call), in positions of the request's page-table row, clamped to
+ * [0, seq_len).  Default: from 0 to the row's own position, that one included.  Given, visible_to may lie behind the
+ * row's own position (prefixes read in both directions); document and window masks are a visible_from.
+ * A row whose interval is empty gets zeros (and a log-sum-exp of -inf).  Tokens that no row of a call
+ * may see are not read, whatever they hold.
+ * The reference passes neither a scale nor a mask of its own to its attention (attn_backend.py:94-101,
+ * :141-143): no counterpart there.
+ */
+typedef struct bsgl_score_mods {
+  float logit_cap;
+  const float* slopes;         /* device, [n_q_heads], or NULL */
+  const int32_t* visible_from; /* device, [rows], or NULL */
+  const int32_t* visible_to;   /* device, [rows], or NULL */
+  /* decode only, both or neither: the attention weight every visible token received in this call, summed
+   * over the q heads, is added to a table parallel to the page table --
+   *   token_weights_out[req_pool_indices[i], j] = token_weights[req_pool_indices[i], j] + sum_h softmax(s)[h, j]
+   * (fp32, [table_rows, table_cols] with row stride weights_row_stride; out may be the same table).  Entries of
+   * tokens that are not visible are left as they were.  Requests that name the same row are added up, in
+   * batch order: the result never depends on the launch. */
+  const float* token_weights;
+  float* token_weights_out;
+  int64_t weights_row_stride;
+} bsgl_score_mods;
+
+/*
+ * bsgl_paged_decode (arguments, checks and KV write as there) with scored attention; the row's own
+ * position is seq_lens[i] - 1.  `call->workspace` holds bsgl_decode_scored_workspace_bytes bytes: the decode
+ * workspace of the same n_splits (the same contract for its tickets), followed, when token weights are asked for, by the
+ * log-sum-exps and finished scores [batch, n_q_heads, table_cols] that the second launch reads.
+ */
+size_t bsgl_decode_scored_workspace_bytes(int32_t batch, int32_t n_q_heads, int32_t head_dim, int32_t n_splits,
+                                          int32_t out_is_f32, int64_t table_cols, int32_t with_weights);
+int bsgl_paged_decode_scored(const bsgl_decode_call* call, const bsgl_score_mods* mods);
+
+/*
  * Workspace for bsgl_paged_prefill (host arithmetic).
  */
 size_t bsgl_prefill_workspace_bytes(int32_t batch, int32_t total_q_tokens, int32_t n_q_heads,

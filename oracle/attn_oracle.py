@@ -238,3 +238,47 @@ def merge_states_exact(parts_o: torch.Tensor, parts_lse: torch.Tensor):
     ).unsqueeze(-1)
     merged_lse = torch.where(tot > 0, safe + torch.log(tot), torch.full_like(tot, float("-inf")))
     return out.reshape(out.shape[0], -1), merged_lse
+
+
+# --------------------------------------------------------------------------- scored attention
+def scored_exact(q, k_slab, v_slab, table_rows, seq_lens, row_req, row_pos, scale, cap=0.0, slopes=None, start=None, stop=None):
+    """Scored attention in float64, query row by query row (no counterpart in the reference).
+
+    ``q`` [R, Hq, D]; query row r belongs to request ``row_req[r]`` (whose slots are ``table_rows[req][: seq_lens[req]]``)
+    at position ``row_pos[r]``; it sees ``[start[r], stop[r])`` of it (None: 0 and its own position + 1).
+    Returns ``out`` [R, Hq, D], ``mass`` = sum p |v| of the same shape (what relative errors of the probabilities are
+    weighted with), ``lse`` [R, Hq], ``received``: per row the probability of every position of its request summed over heads,
+    and ``top`` [R, Hq]: the largest sum |q_d k_d| * scale of a visible token (what the error of a score is proportional to)."""
+    n_rows, hq, dim = q.shape
+    hkv = k_slab.shape[1]
+    out = torch.zeros(n_rows, hq, dim, dtype=torch.float64)
+    mass = torch.zeros_like(out)
+    lse = torch.full((n_rows, hq), float("-inf"), dtype=torch.float64)
+    top = torch.zeros(n_rows, hq, dtype=torch.float64)
+    received = []
+    for r in range(n_rows):
+        req, pos = int(row_req[r]), int(row_pos[r])
+        n = int(seq_lens[req])
+        lo = 0 if start is None else int(start[r])
+        hi = pos + 1 if stop is None else int(stop[r])
+        lo = max(0, min(lo, n))
+        hi = max(lo, min(hi, n))
+        got = torch.zeros(n, dtype=torch.float64)
+        if hi > lo:
+            slots = table_rows[req][lo:hi].long()
+            k = k_slab[slots].double().repeat_interleave(hq // hkv, dim=1)  # [n, Hq, D]
+            v = v_slab[slots].double().repeat_interleave(hq // hkv, dim=1)
+            prod = q[r].double()[None] * k
+            s = prod.sum(-1) * scale
+            top[r] = prod.abs().sum(-1).amax(0) * scale
+            if cap > 0:
+                s = cap * torch.tanh(s / cap)
+            if slopes is not None:
+                s = s - slopes.double()[None, :] * (torch.arange(lo, hi, dtype=torch.float64) - pos).abs()[:, None]
+            lse[r] = torch.logsumexp(s, 0)
+            p = torch.exp(s - lse[r])
+            out[r] = (p[:, :, None] * v).sum(0)
+            mass[r] = (p[:, :, None] * v.abs()).sum(0)
+            got[lo:hi] = p.sum(1)
+        received.append(got)
+    return out, mass, lse, received, top
