@@ -77,6 +77,20 @@ class ScoreMods(ctypes.Structure):
     ]  # fmt: skip
 
 
+class LogitCall(ctypes.Structure):
+    """``bsgl_logit_call`` of include/bsgl_attn.h."""
+
+    _fields_ = [
+        ("out", _vp), ("logits", _vp), ("out_row_stride", _i64), ("logits_row_stride", _i64),
+        ("history", _vp), ("history_row_stride", _i64), ("history_n_rows", _i64), ("history_cols", _i64),
+        ("history_rows", _vp), ("history_lens", _vp), ("prompt_lens", _vp),
+        ("repetition", _vp), ("presence", _vp), ("frequency", _vp),
+        ("bias_ids", _vp), ("bias_values", _vp), ("bias_row_stride", _i64),
+        ("token_mask", _vp), ("mask_row_stride", _i64), ("mask_n_rows", _i64), ("mask_rows", _vp),
+        ("n_bias", _i32), ("batch", _i32), ("vocab", _i32), ("dtype", _i32), ("stream", _vp),
+    ]  # fmt: skip
+
+
 # out .. out_cache_loc: the ten 8-byte fields a caller rewrites on every call, as one packed write
 DECODE_CALL_HEAD = struct.Struct("=10q")
 assert DecodeCall.out.offset == 0 and DecodeCall.out_cache_loc.offset == 72 and DecodeCall.k_slab.offset == 80
@@ -110,6 +124,12 @@ SIGNATURES = {
     ),
     "bsgl_decode_scored_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
     "bsgl_paged_decode_scored": (ctypes.c_int, [ctypes.POINTER(DecodeCall), ctypes.POINTER(ScoreMods)]),
+    "bsgl_evict_workspace_bytes": (_sz, [_i32, _i64, _i32]),
+    "bsgl_evict_tokens": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64] + [_i32] * 6 + [_vp, _sz, _vp],
+    ),
+    "bsgl_logit_controls": (ctypes.c_int, [ctypes.POINTER(LogitCall)]),
     "bsgl_prefill_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "bsgl_paged_prefill": (
         ctypes.c_int,
@@ -614,6 +634,193 @@ def paged_decode_scored(
     with _on_device(q.device):
         c.stream = _stream_ptr(q.device)
         _check(lib.bsgl_paged_decode_scored(ctypes.byref(c), ctypes.byref(mods)), "bsgl_paged_decode_scored")
+    return out
+
+
+# ---- eviction by accumulated weight ---------------------------------------------------------------
+
+
+def evict_workspace_bytes(batch: int, table_cols: int, budget: int) -> int:
+    return lib.bsgl_evict_workspace_bytes(batch, table_cols, budget)
+
+
+def evict_tokens(
+    req_to_token: torch.Tensor,
+    token_weights: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    budget: int,
+    recent: int = 0,
+    sinks: int = 0,
+    out_table: Optional[torch.Tensor] = None,
+    out_weights: Optional[torch.Tensor] = None,
+    evicted: Optional[torch.Tensor] = None,
+    new_lens: Optional[torch.Tensor] = None,
+    max_seq_len: int = 0,
+    workspace: Optional[torch.Tensor] = None,
+):
+    """Keep ``budget`` tokens of every longer request -- the first ``sinks``, the last ``recent`` and the
+    heaviest of the others by ``token_weights`` (ties: the earlier) -- and return
+    ``(new_lens [B] int64, evicted [B, width] int32)``: the slots that went, in order, then -1.
+
+    The page-table and weight rows are compacted in place, or into ``out_table`` / ``out_weights`` (same shape
+    and strides).  ``evicted`` may be given with any width; by default it has room for every slot that can go
+    (``max_seq_len``, 0 = the table's width, less the budget)."""
+    _need_gpu(req_to_token, token_weights, req_pool_indices, seq_lens)
+    _check_table(req_to_token)
+    n_rows, cols = req_to_token.shape
+    batch = int(req_pool_indices.shape[0])
+    rows, lens = (_index_rows(t, batch, n) for t, n in ((req_pool_indices, "req_pool_indices"), (seq_lens, "seq_lens")))
+    budget, recent, sinks = int(budget), int(recent), int(sinks)
+    if out_table is None:
+        out_table = req_to_token
+    if out_weights is None:
+        out_weights = token_weights
+    for t in (token_weights, out_weights):
+        _need_gpu(t)
+        if t.dtype != torch.float32 or t.shape != req_to_token.shape or t.stride(1) != 1 or t.stride(0) < cols:
+            raise ValueError(f"token weights must be float32 of the page table's shape {tuple(req_to_token.shape)} with dense rows")
+    if out_table.dtype != torch.int32 or out_table.shape != req_to_token.shape or out_table.stride() != req_to_token.stride() \
+            or out_weights.stride() != token_weights.stride():
+        raise ValueError("out_table and out_weights must have their inputs' types, shapes and strides")
+    if new_lens is None:
+        new_lens = torch.empty(batch, dtype=torch.int64, device=req_to_token.device)
+    elif new_lens.dtype != torch.int64 or tuple(new_lens.shape) != (batch,) or not new_lens.is_contiguous():
+        raise ValueError(f"new_lens must be a dense int64 vector of {batch} entries")
+    if evicted is None:
+        longest = min(int(max_seq_len), cols) if max_seq_len > 0 else cols
+        evicted = torch.empty((batch, max(0, longest - budget)), dtype=torch.int32, device=req_to_token.device)
+    elif evicted.dtype != torch.int32 or evicted.dim() != 2 or evicted.shape[0] != batch or (evicted.shape[1] > 1 and evicted.stride(1) != 1):
+        raise ValueError("evicted must be int32 [batch, width] with dense rows")
+    need = evict_workspace_bytes(batch, cols, budget)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=req_to_token.device)
+    with _on_device(req_to_token.device):
+        rc = lib.bsgl_evict_tokens(
+            out_table.data_ptr(), out_weights.data_ptr(), req_to_token.data_ptr(), req_to_token.stride(0),
+            token_weights.data_ptr(), token_weights.stride(0), n_rows, cols, rows.data_ptr(), lens.data_ptr(),
+            new_lens.data_ptr(), evicted.data_ptr() if evicted.shape[1] else None, max(evicted.stride(0), evicted.shape[1]), evicted.shape[1],
+            batch, budget, recent, sinks, int(max_seq_len),
+            workspace.data_ptr() if need else None, workspace.numel() * workspace.element_size() if need else 0,
+            _stream_ptr(req_to_token.device),
+        )  # fmt: skip
+    _check(rc, "bsgl_evict_tokens")
+    return new_lens, evicted
+
+
+# ---- logit controls -----------------------------------------------------------------------------
+
+
+def _row_floats(x, batch: int, device, name: str):
+    """A per-request float32 vector; a plain number stands for every request."""
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor):
+        return torch.full((batch,), float(x), dtype=torch.float32, device=device)
+    _need_gpu(x)
+    if x.dtype != torch.float32 or tuple(x.shape) != (batch,):
+        raise ValueError(f"{name} must be float32 of shape ({batch},), got {x.dtype} {tuple(x.shape)}")
+    return x if x.is_contiguous() else x.contiguous()
+
+
+def logit_controls(
+    logits: torch.Tensor,
+    history: Optional[torch.Tensor] = None,
+    history_rows: Optional[torch.Tensor] = None,
+    history_lens: Optional[torch.Tensor] = None,
+    prompt_lens: Optional[torch.Tensor] = None,
+    repetition=None,
+    presence=None,
+    frequency=None,
+    bias_ids: Optional[torch.Tensor] = None,
+    bias_values: Optional[torch.Tensor] = None,
+    token_mask: Optional[torch.Tensor] = None,
+    mask_rows: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Penalties, biases and token masks on ``logits`` [batch, vocab] (``bsgl_logit_controls``); returns ``out``
+    (a new tensor unless one is given; ``out=logits`` works in place).
+
+    ``history`` int32 [rows, columns]: token ids, request i's being the first ``history_lens[i]`` of row
+    ``history_rows[i]`` (default i), the first ``prompt_lens[i]`` (default 0) of them its prompt.  ``repetition``
+    applies to every token of the history, ``presence`` and ``frequency`` to those behind the prompt (float32
+    [batch] or one number).  ``bias_ids`` / ``bias_values`` [batch, n] (int32, float32; ids outside the
+    vocabulary are unused places).  ``token_mask`` int32 [rows, ceil(vocab / 32)], bit t % 32 of word t / 32 set =
+    token t allowed; ``mask_rows`` int32 [batch] (default i; negative = no mask)."""
+    _need_gpu(logits)
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [batch, vocab] with unit column stride")
+    batch, vocab = logits.shape
+    dev = logits.device
+    if out is None:
+        out = torch.empty((batch, vocab), dtype=logits.dtype, device=dev)
+    _check_out(out, batch, vocab, logits.dtype)
+    c = LogitCall()
+    c.dtype = _dtype_code(logits)
+    keep = []
+
+    def vector(t, dtype, name):
+        _need_gpu(t)
+        if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (batch,):
+            raise ValueError(f"{name} must be a vector of {batch} integers, got {t.dtype} {tuple(t.shape)}")
+        t = t.to(dtype).contiguous()
+        keep.append(t)
+        return t.data_ptr()
+
+    def table(t, dtype, name):
+        _need_gpu(t)
+        if t.dtype != dtype or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError(f"{name} must be a 2-D {dtype} tensor with dense rows")
+        keep.append(t)
+        return t.data_ptr(), max(t.stride(0), t.shape[1])
+
+    if history is not None:
+        if history_lens is None:
+            raise ValueError("history needs history_lens")
+        c.history, c.history_row_stride = table(history, torch.int32, "history")
+        c.history_n_rows, c.history_cols = history.shape
+        c.history_lens = vector(history_lens, torch.int64, "history_lens")
+        c.history_rows = vector(history_rows, torch.int64, "history_rows") if history_rows is not None else None
+        c.prompt_lens = vector(prompt_lens, torch.int64, "prompt_lens") if prompt_lens is not None else None
+        for name, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+            x = _row_floats(x, batch, dev, name)
+            if x is not None:
+                keep.append(x)
+                setattr(c, name, x.data_ptr())
+    elif any(x is not None for x in (repetition, presence, frequency, history_rows, history_lens, prompt_lens)):
+        raise ValueError("penalties and history rows need a history")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values go together")
+    if bias_ids is not None:
+        if bias_ids.shape != bias_values.shape or bias_ids.dim() != 2 or bias_ids.shape[0] != batch:
+            raise ValueError("bias_ids and bias_values must be [batch, n]")
+        c.bias_ids, c.bias_row_stride = table(bias_ids, torch.int32, "bias_ids")
+        c.bias_values, stride = table(bias_values, torch.float32, "bias_values")
+        if stride != c.bias_row_stride:
+            raise ValueError("bias_ids and bias_values must share a row stride")
+        c.n_bias = bias_ids.shape[1]
+    if token_mask is not None:
+        c.token_mask, c.mask_row_stride = table(token_mask, torch.int32, "token_mask")
+        if token_mask.shape[1] < (vocab + 31) // 32:
+            raise ValueError(f"token_mask rows hold {32 * token_mask.shape[1]} bits, the vocabulary has {vocab} tokens")
+        c.mask_n_rows = token_mask.shape[0]
+        if mask_rows is not None:
+            c.mask_rows = vector(mask_rows, torch.int32, "mask_rows")
+        elif token_mask.shape[0] < batch:
+            raise ValueError("token_mask has fewer rows than the batch")
+    elif mask_rows is not None:
+        raise ValueError("mask_rows without token_mask")
+    for t in keep:
+        if t.device != dev:
+            raise ValueError(f"all tensors must be on the logits' device {dev}, got {t.device}")
+    if batch == 0 or vocab == 0:
+        return out
+    c.out, c.out_row_stride = out.data_ptr(), max(out.stride(0), vocab)
+    c.logits, c.logits_row_stride = logits.data_ptr(), max(logits.stride(0), vocab)
+    c.batch, c.vocab = batch, vocab
+    with _on_device(dev):
+        c.stream = _stream_ptr(dev)
+        _check(lib.bsgl_logit_controls(ctypes.byref(c)), "bsgl_logit_controls")
     return out
 
 

@@ -262,6 +262,58 @@ hipError_t launch_rope_kv(const RopeArgs& a, hipStream_t stream);
 
 hipError_t launch_merge(const MergeArgs& a, hipStream_t stream);
 hipError_t launch_token_weights(const WeightsArgs& a, hipStream_t stream);
+
+struct EvictArgs {
+  int32_t* out_table;  // [table_rows, table_cols], row strides as the inputs'; may be `table` / `weights`
+  float* out_weights;
+  const int32_t* table;
+  const float* weights;
+  int64_t table_row_stride;
+  int64_t weights_row_stride;
+  int64_t table_rows;
+  int64_t table_cols;
+  const int64_t* req_idx;   // [batch]
+  const int64_t* seq_lens;  // [batch]
+  int64_t* new_lens;        // [batch]
+  int32_t* evicted;         // optional [batch, evicted_cols], the rest of a row set to -1
+  int64_t evicted_row_stride;
+  int32_t evicted_cols;
+  int32_t batch;
+  int32_t budget;
+  int32_t recent;
+  int32_t sinks;
+  int32_t longest;  // longest request the host knows of (table_cols if it knows none); shapes the launch only
+};
+hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
+
+struct LogitArgs {
+  void* out;  // may be `logits`
+  const void* logits;
+  int64_t out_row_stride;
+  int64_t logits_row_stride;
+  const int32_t* history;  // optional [history_n_rows, history_cols]
+  int64_t history_row_stride;
+  int64_t history_n_rows;
+  int64_t history_cols;
+  const int64_t* history_rows;  // optional [batch]
+  const int64_t* history_lens;  // [batch]
+  const int64_t* prompt_lens;   // optional [batch]
+  const float* repetition;      // optional [batch] each
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids;  // optional [batch, n_bias]; ids outside the vocabulary are unused places
+  const float* bias_values;
+  int64_t bias_row_stride;
+  const int32_t* token_mask;  // optional [mask_n_rows, ceil(vocab / 32)]
+  int64_t mask_row_stride;
+  int64_t mask_n_rows;
+  const int32_t* mask_rows;  // optional [batch]; outside [0, mask_n_rows): no mask
+  int32_t n_bias;
+  int32_t batch;
+  int32_t vocab;
+  int32_t dtype;
+};
+hipError_t launch_logit_controls(const LogitArgs& a, hipStream_t stream);
 hipError_t launch_kv_scatter(const ScatterArgs& a, hipStream_t stream);
 hipError_t launch_prefill_expand(const ExpandArgs& a, hipStream_t stream);
 

@@ -768,6 +768,105 @@ int bsgl_merge_attn_states(void* out, int64_t out_row_stride, float* lse_out, co
   return BSGL_OK;
 }
 
+size_t bsgl_evict_workspace_bytes(int32_t batch, int64_t table_cols, int32_t budget) {
+  (void)batch; (void)table_cols; (void)budget;
+  return 0;
+}
+
+int bsgl_evict_tokens(int32_t* out_table, float* out_weights, const int32_t* req_to_token, int64_t table_row_stride,
+                      const float* token_weights, int64_t weights_row_stride, int64_t table_rows, int64_t table_cols,
+                      const int64_t* req_pool_indices, const int64_t* seq_lens, int64_t* new_lens, int32_t* evicted,
+                      int64_t evicted_row_stride, int32_t evicted_cols, int32_t batch, int32_t budget, int32_t recent,
+                      int32_t sinks, int32_t max_seq_len, void* workspace, size_t workspace_bytes, void* stream) {
+  (void)workspace; (void)workspace_bytes;
+  if (batch < 0) return fail(BSGL_ERR_BAD_ARG, "batch < 0");
+  if (budget < 1 || recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget)
+    return fail(BSGL_ERR_BAD_ARG, "budget %d must be positive and hold the %d sinks and %d recent tokens", budget, sinks, recent);
+  if (batch == 0) return BSGL_OK;
+  if (!out_table || !out_weights || !req_to_token || !token_weights || !req_pool_indices || !seq_lens || !new_lens)
+    return fail(BSGL_ERR_BAD_ARG, "null device pointer (tables / req_pool_indices / seq_lens / new_lens)");
+  if (table_rows <= 0 || table_cols <= 0 || table_cols > 0x7fffffff) return fail(BSGL_ERR_BAD_ARG, "page-table extents must be positive and below 2^31 columns");
+  if (table_row_stride < table_cols || weights_row_stride < table_cols)
+    return fail(BSGL_ERR_BAD_ARG, "a row stride is shorter than the page table's column count");
+  if (evicted_cols < 0 || (evicted != nullptr && evicted_row_stride < evicted_cols))
+    return fail(BSGL_ERR_BAD_ARG, "evicted row stride shorter than its column count");
+  bsgl::EvictArgs a{};
+  a.out_table = out_table;
+  a.out_weights = out_weights;
+  a.table = req_to_token;
+  a.weights = token_weights;
+  a.table_row_stride = table_row_stride;
+  a.weights_row_stride = weights_row_stride;
+  a.table_rows = table_rows;
+  a.table_cols = table_cols;
+  a.req_idx = req_pool_indices;
+  a.seq_lens = seq_lens;
+  a.new_lens = new_lens;
+  a.evicted = evicted_cols > 0 ? evicted : nullptr;
+  a.evicted_row_stride = evicted_row_stride;
+  a.evicted_cols = evicted_cols;
+  a.batch = batch;
+  a.budget = budget;
+  a.recent = recent;
+  a.sinks = sinks;
+  a.longest = (int32_t)(max_seq_len > 0 && max_seq_len < table_cols ? max_seq_len : table_cols);
+  const hipError_t e = bsgl::launch_evict(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail("evict launch", e);
+  return BSGL_OK;
+}
+
+int bsgl_logit_controls(const bsgl_logit_call* c) {
+  if (c == nullptr) return fail(BSGL_ERR_BAD_ARG, "null call descriptor");
+  if (int rc = check_dtype(c->dtype)) return rc;
+  if (c->batch < 0 || c->vocab < 0 || c->n_bias < 0) return fail(BSGL_ERR_BAD_ARG, "batch, vocab or n_bias < 0");
+  if (c->batch == 0 || c->vocab == 0) return BSGL_OK;
+  if (c->batch > 65535) return fail(BSGL_ERR_UNSUPPORTED, "batch %d above 65535", c->batch);
+  if (c->vocab > (1 << 30)) return fail(BSGL_ERR_UNSUPPORTED, "vocabulary of %d tokens above 2^30", c->vocab);
+  if (!c->out || !c->logits) return fail(BSGL_ERR_BAD_ARG, "null device pointer (out/logits)");
+  if (c->out_row_stride < c->vocab || c->logits_row_stride < c->vocab) return fail(BSGL_ERR_BAD_ARG, "logit row stride shorter than the vocabulary");
+  if (c->history != nullptr) {
+    if (!c->history_lens) return fail(BSGL_ERR_BAD_ARG, "history without history_lens");
+    if (c->history_n_rows <= 0 || c->history_cols < 0 || c->history_cols > 0x7fffffff - 4096 || c->history_row_stride < c->history_cols)
+      return fail(BSGL_ERR_BAD_ARG, "history extents must be positive, its row stride at least its column count");
+    if (c->history_rows == nullptr && c->history_n_rows < c->batch) return fail(BSGL_ERR_BAD_ARG, "history has fewer rows than the batch");
+  } else if (c->repetition || c->presence || c->frequency) {
+    return fail(BSGL_ERR_BAD_ARG, "penalties without a history");
+  }
+  if (c->n_bias > 0 && (!c->bias_ids || !c->bias_values || c->bias_row_stride < c->n_bias))
+    return fail(BSGL_ERR_BAD_ARG, "bias_ids and bias_values go together, with a row stride of at least n_bias");
+  if (c->token_mask != nullptr && (c->mask_n_rows <= 0 || c->mask_row_stride < ((int64_t)c->vocab + 31) / 32))
+    return fail(BSGL_ERR_BAD_ARG, "token mask rows are shorter than the vocabulary's bits");
+  bsgl::LogitArgs a{};
+  a.out = c->out;
+  a.logits = c->logits;
+  a.out_row_stride = c->out_row_stride;
+  a.logits_row_stride = c->logits_row_stride;
+  a.history = c->history;
+  a.history_row_stride = c->history_row_stride;
+  a.history_n_rows = c->history_n_rows;
+  a.history_cols = c->history_cols;
+  a.history_rows = c->history_rows;
+  a.history_lens = c->history_lens;
+  a.prompt_lens = c->prompt_lens;
+  a.repetition = c->repetition;
+  a.presence = c->presence;
+  a.frequency = c->frequency;
+  a.bias_ids = c->n_bias > 0 ? c->bias_ids : nullptr;
+  a.bias_values = c->bias_values;
+  a.bias_row_stride = c->bias_row_stride;
+  a.token_mask = c->token_mask;
+  a.mask_row_stride = c->mask_row_stride;
+  a.mask_n_rows = c->mask_n_rows;
+  a.mask_rows = c->mask_rows;
+  a.n_bias = c->n_bias;
+  a.batch = c->batch;
+  a.vocab = c->vocab;
+  a.dtype = c->dtype;
+  const hipError_t e = bsgl::launch_logit_controls(a, (hipStream_t)c->stream);
+  if (e != hipSuccess) return hip_fail("logit control launch", e);
+  return BSGL_OK;
+}
+
 int bsgl_rmsnorm(void* out, int64_t out_row_stride, void* residual_out, const void* x, int64_t x_row_stride,
                  const void* residual, const void* weight, int32_t rows, int32_t hidden, float eps,
                  int32_t dtype, void* stream) {

@@ -292,6 +292,65 @@ size_t bsgl_decode_scored_workspace_bytes(int32_t batch, int32_t n_q_heads, int3
 int bsgl_paged_decode_scored(const bsgl_decode_call* call, const bsgl_score_mods* mods);
 
 /*
+ * Eviction from the paged cache by accumulated weight (no counterpart in the reference, whose cache gives
+ * up whole requests or prefix-tree leaves only: scheduler.py:322-369, radix_cache.py:209-272).  Request i owns the first
+ * seq_lens[i] entries of page-table row req_pool_indices[i] and of the weight row beside it.  If that is more than
+ * `budget`, exactly `budget` of its tokens stay: the first `sinks`, the last `recent`, and of those between
+ * the ones with the largest weight (of equal weights the earlier; NaN counts as the largest, -0 as 0); sinks + recent <= budget.  The entries that
+ * stay are moved to the front of out_table / out_weights in their order (same strides as the inputs; each may be
+ * its input), new_lens[i] = min(seq_lens[i], budget) receives their number, and evicted (optional, [batch, evicted_cols])
+ * the slots of the others in their order, as many as fit, then -1.  Entries behind new_lens[i], and rows that no request
+ * names, are left as they are.  A row named by several requests is compacted for the first of them; the others get an
+ * empty evicted list.  max_seq_len (0 = unknown) shapes the launch only.  workspace: bsgl_evict_workspace_bytes, may be
+ * NULL when that is 0.
+ */
+size_t bsgl_evict_workspace_bytes(int32_t batch, int64_t table_cols, int32_t budget);
+int bsgl_evict_tokens(int32_t* out_table /*device*/, float* out_weights /*device*/,
+                      const int32_t* req_to_token /*device*/, int64_t table_row_stride,
+                      const float* token_weights /*device*/, int64_t weights_row_stride,
+                      int64_t table_rows, int64_t table_cols,
+                      const int64_t* req_pool_indices /*device, [batch]*/, const int64_t* seq_lens /*device, [batch]*/,
+                      int64_t* new_lens /*device, [batch]*/, int32_t* evicted /*device or NULL*/, int64_t evicted_row_stride,
+                      int32_t evicted_cols, int32_t batch, int32_t budget, int32_t recent, int32_t sinks, int32_t max_seq_len,
+                      void* workspace /*device or NULL*/, size_t workspace_bytes, void* stream);
+
+/*
+ * Penalties, biases and token masks on the logits [batch, vocab] of a step, in this order, in fp32, rounded
+ * once at the end (the reference's counterpart is the repetition penalty alone, sample.py:19-37, one request at a time):
+ *   tokens of the request's history:          x = x > 0 ? x / repetition : x * repetition
+ *   the n times it stands behind the prompt:  x = x - frequency * n - presence   (n > 0)
+ *   sparse biases:                            x = x + sum of the biases of the token, in their order
+ *   token mask:                               x = -inf where bit (t % 32) of word (t / 32) is 0
+ * The history is a table of token ids parallel to the page table: request i's are the first history_lens[i] entries
+ * of row history_rows[i] (NULL: row i), the first prompt_lens[i] (NULL: 0) of them its prompt.  Ids outside the vocabulary are ignored,
+ * in biases too (padding).  mask_rows[i] (NULL: i) outside [0, mask_n_rows) = no mask.  A mask without any bit
+ * leaves a row of -inf.  Everything but logits and out may be NULL; out may be logits.  repetition, presence, frequency: fp32
+ * [batch], repetition > 0.
+ */
+typedef struct bsgl_logit_call {
+  void* out;
+  const void* logits;
+  int64_t out_row_stride, logits_row_stride;
+  const int32_t* history;
+  int64_t history_row_stride, history_n_rows, history_cols;
+  const int64_t* history_rows;
+  const int64_t* history_lens;
+  const int64_t* prompt_lens;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids; /* [batch, n_bias] */
+  const float* bias_values;
+  int64_t bias_row_stride;
+  const int32_t* token_mask; /* [mask_n_rows, ceil(vocab / 32)] */
+  int64_t mask_row_stride, mask_n_rows;
+  const int32_t* mask_rows;
+  int32_t n_bias, batch, vocab, dtype;
+  void* stream;
+} bsgl_logit_call;
+int bsgl_logit_controls(const bsgl_logit_call* call);
+
+/*
  * Workspace for bsgl_paged_prefill (host arithmetic).
  */
 size_t bsgl_prefill_workspace_bytes(int32_t batch, int32_t total_q_tokens, int32_t n_q_heads,

@@ -1,0 +1,95 @@
+"""Refusals and host arithmetic of the scored attention, eviction and logit entry points (CPU only: every one of
+them is answered before anything would be launched)."""
+import ctypes
+
+import pytest
+import torch
+
+from baby_sglang_amd import _hip
+
+lib = _hip.lib
+P = ctypes.c_void_p(256)  # a pointer that a refused call never follows
+
+
+def mods(**kw):
+    m = _hip.ScoreMods()
+    for k, v in kw.items():
+        setattr(m, k, v)
+    return ctypes.byref(m)
+
+
+def decode_call(**kw):
+    c = _hip.DecodeCall()
+    d = dict(out=256, out_row_stride=1536, q=256, q_row_stride=1536, k_slab=256, v_slab=256, slab_row_stride=512, n_slots=9, req_to_token=256,
+             table_row_stride=64, table_rows=2, table_cols=64, req_pool_indices=256, seq_lens=256, batch=2, n_q_heads=12, n_kv_heads=2,
+             head_dim=128, scale=0.1, n_splits=1)
+    d.update(kw)
+    for k, v in d.items():
+        setattr(c, k, v)
+    return ctypes.byref(c)
+
+
+def test_scored_decode_refusals():
+    f = lib.bsgl_paged_decode_scored
+    assert f(None, mods()) == _hip.BSGL_ERR_BAD_ARG and f(decode_call(), None) == _hip.BSGL_ERR_BAD_ARG
+    for cap in (-1.0, float("nan"), float("inf")):
+        assert f(decode_call(), mods(logit_cap=cap)) == _hip.BSGL_ERR_BAD_ARG and b"logit_cap" in lib.bsgl_last_error()
+    assert f(decode_call(), mods(token_weights=256)) == _hip.BSGL_ERR_BAD_ARG
+    assert f(decode_call(), mods(token_weights=256, token_weights_out=256, weights_row_stride=63)) == _hip.BSGL_ERR_BAD_ARG
+    assert f(decode_call(), mods(token_weights=256, token_weights_out=256, weights_row_stride=64)) == _hip.BSGL_ERR_WORKSPACE
+    assert f(decode_call(n_splits=65), mods()) == _hip.BSGL_ERR_BAD_ARG
+    assert f(decode_call(q=None), mods()) == _hip.BSGL_ERR_BAD_ARG
+    assert f(decode_call(dtype=7), mods()) == _hip.BSGL_ERR_UNSUPPORTED
+    assert f(decode_call(batch=0), mods(logit_cap=1.0)) == _hip.BSGL_OK  # nothing to do
+
+
+def test_scored_decode_workspace():
+    plain = _hip.decode_workspace_bytes(4, 12, 128, 8)
+    assert _hip.decode_scored_workspace_bytes(4, 12, 128, 8, 1000, False) == plain
+    with_weights = _hip.decode_scored_workspace_bytes(4, 12, 128, 8, 1000, True)
+    assert with_weights >= plain + 4 * 12 * (1 + 1008) * 4
+    # the ticket area stays free of scores where the decode itself needs no workspace
+    assert _hip.decode_workspace_bytes(4, 12, 128, 1) == 0
+    assert _hip.decode_scored_workspace_bytes(4, 12, 128, 1, 1000, True) >= lib.bsgl_decode_counter_bytes() + 4 * 12 * 1008 * 4
+
+
+def test_evict_refusals():
+    def f(budget=4, recent=1, sinks=1, rows=2, cols=64, ts=64, ws=64, es=8, ec=8, batch=2, table=P):
+        return lib.bsgl_evict_tokens(P, P, table, ts, P, ws, rows, cols, P, P, P, P, es, ec, batch, budget, recent, sinks, 0, None, 0, None)
+
+    for kw in (dict(budget=0), dict(budget=-1), dict(recent=-1), dict(sinks=-1), dict(budget=4, recent=2, sinks=3), dict(recent=2**31 - 1, sinks=2),
+               dict(rows=0), dict(cols=0), dict(cols=2**31, ts=2**31, ws=2**31), dict(ts=63), dict(ws=63), dict(es=7), dict(ec=-1), dict(batch=-1), dict(table=None)):
+        assert f(**kw) == _hip.BSGL_ERR_BAD_ARG, kw
+    assert f(batch=0) == _hip.BSGL_OK
+
+
+def test_logit_refusals():
+    def f(**kw):
+        c = _hip.LogitCall()
+        d = dict(out=256, logits=256, out_row_stride=100, logits_row_stride=100, batch=2, vocab=100, dtype=2)
+        d.update(kw)
+        for k, v in d.items():
+            setattr(c, k, v)
+        return lib.bsgl_logit_controls(ctypes.byref(c))
+
+    hist = dict(history=256, history_row_stride=10, history_n_rows=2, history_cols=10, history_lens=256)
+    for kw in (dict(out=None), dict(logits=None), dict(out_row_stride=99), dict(logits_row_stride=99), dict(batch=-1), dict(vocab=-1), dict(n_bias=-1),
+               dict(n_bias=3), dict(n_bias=3, bias_ids=256, bias_values=256, bias_row_stride=2), dict(repetition=256),
+               dict(hist, history_lens=None), dict(hist, history_n_rows=1), dict(hist, history_n_rows=0), dict(hist, history_row_stride=9),
+               dict(token_mask=256, mask_n_rows=2, mask_row_stride=3), dict(token_mask=256, mask_n_rows=0, mask_row_stride=4)):
+        assert f(**kw) == _hip.BSGL_ERR_BAD_ARG, kw
+    assert f(dtype=5) == _hip.BSGL_ERR_UNSUPPORTED and f(batch=65536) == _hip.BSGL_ERR_UNSUPPORTED
+    assert f(batch=0, out=None) == _hip.BSGL_OK and f(vocab=0, out=None) == _hip.BSGL_OK
+    assert lib.bsgl_logit_controls(None) == _hip.BSGL_ERR_BAD_ARG
+
+
+def test_tensors_off_the_gpu_are_refused():
+    q = torch.zeros(1, 12, 128, dtype=torch.bfloat16)
+    slab = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
+    table, one = torch.zeros(1, 8, dtype=torch.int32), torch.ones(1, dtype=torch.int64)
+    with pytest.raises(RuntimeError):
+        _hip.paged_decode_scored(q, slab, slab, table, one, one)
+    with pytest.raises(RuntimeError):
+        _hip.evict_tokens(table, torch.zeros(1, 8), one, one, 2)
+    with pytest.raises(RuntimeError):
+        _hip.logit_controls(torch.zeros(1, 8))
