@@ -136,6 +136,11 @@ SIGNATURES = {
         [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]
         + [_i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _sz, _vp],
     ),
+    "bsgl_paged_prefill_scored": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]
+        + [_i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _sz, ctypes.POINTER(ScoreMods), _vp],
+    ),
     "bsgl_merge_attn_states": (
         ctypes.c_int,
         [_vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp],
@@ -877,6 +882,66 @@ def paged_prefill(
         _stream_ptr(q.device),
     )  # fmt: skip
     _check(rc, "bsgl_paged_prefill")
+    return out
+
+
+def paged_prefill_scored(
+    q: torch.Tensor,
+    k_slab: torch.Tensor,
+    v_slab: torch.Tensor,
+    req_to_token: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    extended_lens: torch.Tensor,
+    scale: Optional[float] = None,
+    logit_cap: float = 0.0,
+    slopes: Optional[torch.Tensor] = None,
+    visible_from: Optional[torch.Tensor] = None,
+    visible_to: Optional[torch.Tensor] = None,
+    variant: int = DECODE_AUTO,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+    list_ready: bool = False,
+) -> torch.Tensor:
+    """``paged_prefill`` with scored attention (``bsgl_paged_prefill_scored``); returns [T, Hq * D].  Cap, slopes and
+    interval as in ``paged_decode_scored``, the interval (int32 [T]) per row of q in positions of its
+    request; the default sees everything up to the row's own position.  Rows behind the last request's are left as
+    they were."""
+    _need_gpu(q, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens, prefix_lens, extended_lens)
+    q = _rows(q)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [tokens, heads, dim], got shape {tuple(q.shape)}")
+    total_q, hq, dim = q.shape
+    hkv = k_slab.shape[1]
+    batch = int(req_pool_indices.shape[0])
+    if out is None:
+        out = torch.empty((total_q, hq * dim), dtype=q.dtype, device=q.device)
+    _check_out(out, total_q, hq * dim, q.dtype)
+    if total_q == 0 or batch == 0:
+        return out
+    _check_slabs(q, k_slab, v_slab, dim)
+    _check_table(req_to_token)
+    names = ("req_pool_indices", "seq_lens", "prefix_lens", "extended_lens")
+    i64 = [_index_rows(t, batch, n) for t, n in zip((req_pool_indices, seq_lens, prefix_lens, extended_lens), names)]
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    mods, keep = _score_mods(total_q, hq, q.device, logit_cap, slopes, visible_from, visible_to)
+    need = prefill_workspace_bytes(batch, total_q, hq, dim)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        if list_ready:
+            raise ValueError("list_ready needs the workspace that holds the list")
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    with _on_device(q.device):
+        rc = lib.bsgl_paged_prefill_scored(
+            out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0),
+            k_slab.data_ptr(), v_slab.data_ptr(), k_slab.stride(0), k_slab.shape[0],
+            req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[0], req_to_token.shape[1],
+            i64[0].data_ptr(), i64[1].data_ptr(), i64[2].data_ptr(), i64[3].data_ptr(),
+            batch, total_q, hq, hkv, dim, scale, _dtype_code(q), variant | (PREFILL_LIST_READY if list_ready else 0),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), ctypes.byref(mods), _stream_ptr(q.device),
+        )  # fmt: skip
+    _check(rc, "bsgl_paged_prefill_scored")
     return out
 
 

@@ -179,6 +179,7 @@ struct ExpandArgs {
   int32_t grp_blocks;  // blocks per group (0 counts as 1)
   int64_t* row_req;  // [total_q_tokens]; may be NULL (then only the running sums are made)
   int64_t* row_len;  // [total_q_tokens]
+  int4* rows4;       // instead of row_req / row_len, for the scored form: {page-table row, request length, own position, 0}
 };
 
 // extend attention over blocks of 16 query positions (matrix-core kernel)
@@ -206,6 +207,7 @@ struct PrefillArgs {
   int32_t head_dim;
   float scale;
   int32_t dtype;
+  ScoreMods mods;  // scored form only; from / to are per row of q
 };
 
 inline bool decode_direct_out(const DecodeArgs& a) { return a.n_splits == 1 && a.out_dtype == a.dtype; }
@@ -323,5 +325,8 @@ hipError_t launch_prefill_mfma(const PrefillArgs& a, hipStream_t stream);
 // launch_prefill_mfma picks it where it applies
 bool prefill_mfma32_supported(const PrefillArgs& a);
 hipError_t launch_prefill_mfma32(const PrefillArgs& a, hipStream_t stream);
+// scored extend attention where prefill_scored_supported says so
+bool prefill_scored_supported(const PrefillArgs& a, const char** why);
+hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream);
 
 }  // namespace bsgl

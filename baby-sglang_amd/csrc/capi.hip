@@ -384,8 +384,7 @@ int scratch_of_current_device(void** out, bool capturing) {
 }
 
 // the description of a scored call into a launch's arguments
-int take_mods(bsgl::DecodeArgs& a, const bsgl_score_mods& m, int32_t n_q_heads) {
-  (void)n_q_heads;
+int take_mods(bsgl::DecodeArgs& a, const bsgl_score_mods& m) {
   if (!(m.logit_cap >= 0.f) || m.logit_cap > 3.0e38f) return fail(BSGL_ERR_BAD_ARG, "logit_cap %g is negative or not finite", (double)m.logit_cap);
   a.scored = true;
   a.mods.cap = m.logit_cap;
@@ -485,7 +484,7 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
   a.n_splits = n_splits;
   a.len_hint = max_seq_len > 0 ? max_seq_len : 0;
   if (mods != nullptr) {
-    if (int rc = take_mods(a, *mods, n_q_heads)) return rc;
+    if (int rc = take_mods(a, *mods)) return rc;
     if (mods->token_weights != nullptr) {
       const size_t all = bsgl_decode_scored_workspace_bytes(batch, n_q_heads, head_dim, n_splits, f32_out, table_cols, 1);
       if (workspace == nullptr || workspace_bytes < all || !aligned16(workspace))
@@ -598,14 +597,14 @@ size_t bsgl_prefill_workspace_bytes(int32_t batch, int32_t total_q_tokens, int32
   return bytes;
 }
 
-int bsgl_paged_prefill(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
-                       const void* k_slab, const void* v_slab, int64_t slab_row_stride, int64_t n_slots,
-                       const int32_t* req_to_token, int64_t table_row_stride, int64_t table_rows,
-                       int64_t table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
-                       const int64_t* prefix_lens, const int64_t* extended_lens, int32_t batch,
-                       int32_t total_q_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                       float scale, int32_t dtype, int32_t variant, void* workspace,
-                       size_t workspace_bytes, void* stream) {
+static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                         const void* k_slab, const void* v_slab, int64_t slab_row_stride, int64_t n_slots,
+                         const int32_t* req_to_token, int64_t table_row_stride, int64_t table_rows,
+                         int64_t table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                         const int64_t* prefix_lens, const int64_t* extended_lens, int32_t batch,
+                         int32_t total_q_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                         float scale, int32_t dtype, int32_t variant, void* workspace,
+                         size_t workspace_bytes, const bsgl_score_mods* mods, void* stream) {
   if (batch < 0 || total_q_tokens < 0) return fail(BSGL_ERR_BAD_ARG, "batch / total_q_tokens < 0");
   if (batch == 0 || total_q_tokens == 0) return BSGL_OK;
   bsgl::DecodeArgs a{};
@@ -618,6 +617,10 @@ int bsgl_paged_prefill(void* out, int64_t out_row_stride, const void* q, int64_t
     return fail(BSGL_ERR_WORKSPACE, "prefill needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
 
   char* ws = (char*)workspace;
+  bsgl::DecodeArgs scored{};
+  if (mods != nullptr) {
+    if (int rc = take_mods(scored, *mods)) return rc;
+  }
   bsgl::ExpandArgs ex{};
   ex.req_pool_indices = req_pool_indices;
   ex.seq_lens = seq_lens;
@@ -655,11 +658,13 @@ int bsgl_paged_prefill(void* out, int64_t out_row_stride, const void* q, int64_t
   // from 64); with one q head per kv head it is the single-wave kernel, worth it below 24.
   const int64_t short_below = n_kv_heads > 0 && n_q_heads / n_kv_heads >= 2 ? 44 : 24;
   pa.blk_rows = (int64_t)total_q_tokens >= short_below * batch ? 64 : 16;
+  // (scored form, one q head per kv head: there is no single-wave kernel, and of a 16-position workgroup three waves would idle)
+  if (mods != nullptr && n_q_heads == n_kv_heads) pa.blk_rows = 64;
   {
     const int forced = bsgl::knob(bsgl::kKnobPrefillBlk);  // tuning override
     if (forced == 16 || forced == 64) pa.blk_rows = forced;
     // (128: two four-wave teams share a K/V stream; only where the 32x32x16 kernel applies)
-    if (forced == 128 && n_kv_heads > 0 && n_q_heads / n_kv_heads >= 2) pa.blk_rows = 128;
+    if (mods == nullptr && forced == 128 && n_kv_heads > 0 && n_q_heads / n_kv_heads >= 2) pa.blk_rows = 128;
   }
   ex.blk_rows = pa.blk_rows;
   // Groups of up to 8 consecutive blocks of a request share an XCD (and with it an L2).  The grid
@@ -687,6 +692,10 @@ int bsgl_paged_prefill(void* out, int64_t out_row_stride, const void* q, int64_t
   pa.head_dim = head_dim;
   pa.scale = scale;
   pa.dtype = dtype;
+  pa.mods = scored.mods;
+  auto supported = [&](const bsgl::PrefillArgs& x, const char** w) {
+    return mods != nullptr ? bsgl::prefill_scored_supported(x, w) : bsgl::prefill_mfma_supported(x, w);
+  };
   const char* why = "";
   const int32_t kind = variant & 0xff;
   if (kind != BSGL_DECODE_AUTO && kind != BSGL_DECODE_VALU && kind != BSGL_DECODE_MFMA)
@@ -697,9 +706,9 @@ int bsgl_paged_prefill(void* out, int64_t out_row_stride, const void* q, int64_t
     folded.fold_group = n_q_heads / 2;
     folded.n_kv_heads = 1;
     folded.head_dim = 128;
-    if (bsgl::prefill_mfma_supported(folded, &why)) pa = folded;
+    if (supported(folded, &why)) pa = folded;
   }
-  const bool mfma_ok = bsgl::prefill_mfma_supported(pa, &why);
+  const bool mfma_ok = supported(pa, &why);
   if (kind == BSGL_DECODE_MFMA && !mfma_ok) return fail(BSGL_ERR_UNSUPPORTED, "matrix-core extend: %s", why);
   if (kind != BSGL_DECODE_VALU && mfma_ok) {
     ex.row_req = nullptr;  // only the running sums are needed
@@ -708,9 +717,16 @@ int bsgl_paged_prefill(void* out, int64_t out_row_stride, const void* q, int64_t
       e = bsgl::launch_prefill_expand(ex, (hipStream_t)stream);
       if (e != hipSuccess) return hip_fail("prefill running-sum launch", e);
     }
-    e = bsgl::launch_prefill_mfma(pa, (hipStream_t)stream);
+    e = mods != nullptr ? bsgl::launch_prefill_scored(pa, (hipStream_t)stream) : bsgl::launch_prefill_mfma(pa, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail("prefill launch", e);
     return BSGL_OK;
+  }
+  if (mods != nullptr) {
+    // (one {row, length, position} per token where the plain form keeps a row and a length: the same bytes)
+    ex.rows4 = (int4*)ex.row_req;
+    a.scored = true;
+    a.mods = scored.mods;
+    a.mods.rows = ex.rows4;
   }
   hipError_t e = bsgl::launch_prefill_expand(ex, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail("prefill expand launch", e);
@@ -737,6 +753,35 @@ int bsgl_paged_prefill(void* out, int64_t out_row_stride, const void* q, int64_t
   a.ws_o = (float*)(ws + cb);
   a.ws_lse = splits > 1 ? (float*)(ws + cb + align_up((size_t)splits * rh * (size_t)head_dim * 4, 256)) : nullptr;
   return run_decode(a, BSGL_DECODE_VALU, nullptr, (hipStream_t)stream);
+}
+
+int bsgl_paged_prefill(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                       const void* k_slab, const void* v_slab, int64_t slab_row_stride, int64_t n_slots,
+                       const int32_t* req_to_token, int64_t table_row_stride, int64_t table_rows,
+                       int64_t table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                       const int64_t* prefix_lens, const int64_t* extended_lens, int32_t batch,
+                       int32_t total_q_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                       float scale, int32_t dtype, int32_t variant, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  return prefill_entry(out, out_row_stride, q, q_row_stride, k_slab, v_slab, slab_row_stride, n_slots, req_to_token,
+                       table_row_stride, table_rows, table_cols, req_pool_indices, seq_lens, prefix_lens, extended_lens, batch,
+                       total_q_tokens, n_q_heads, n_kv_heads, head_dim, scale, dtype, variant, workspace, workspace_bytes, nullptr, stream);
+}
+
+int bsgl_paged_prefill_scored(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                              const void* k_slab, const void* v_slab, int64_t slab_row_stride, int64_t n_slots,
+                              const int32_t* req_to_token, int64_t table_row_stride, int64_t table_rows,
+                              int64_t table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                              const int64_t* prefix_lens, const int64_t* extended_lens, int32_t batch,
+                              int32_t total_q_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                              float scale, int32_t dtype, int32_t variant, void* workspace,
+                              size_t workspace_bytes, const bsgl_score_mods* mods, void* stream) {
+  if (mods == nullptr) return fail(BSGL_ERR_BAD_ARG, "null score description");
+  if (mods->token_weights != nullptr || mods->token_weights_out != nullptr)
+    return fail(BSGL_ERR_UNSUPPORTED, "token weights are accumulated by decode calls only");
+  return prefill_entry(out, out_row_stride, q, q_row_stride, k_slab, v_slab, slab_row_stride, n_slots, req_to_token,
+                       table_row_stride, table_rows, table_cols, req_pool_indices, seq_lens, prefix_lens, extended_lens, batch,
+                       total_q_tokens, n_q_heads, n_kv_heads, head_dim, scale, dtype, variant, workspace, workspace_bytes, mods, stream);
 }
 
 int bsgl_merge_attn_states(void* out, int64_t out_row_stride, float* lse_out, const float* parts_o,

@@ -92,6 +92,17 @@ __global__ __launch_bounds__(256) void prefill_rows_kernel(ExpandArgs a) {
   // search above lands on the LAST request starting at or before t, which is
   // the one that owns the row.
   int64_t len = 0, req = 0;
+  if (a.rows4 != nullptr) {
+    int4 r4 = make_int4(0, 0, 0, 0);
+    if (a.batch > 0 && t < a.cu_ext[a.batch]) {
+      auto i32 = [](int64_t x) { return (int)max((int64_t)0, min(x, (int64_t)0x7fffffff)); };
+      const int64_t full = max((int64_t)0, a.seq_lens[lo]);
+      const int64_t prefix = max((int64_t)0, min(a.prefix_lens[lo], full));
+      r4 = make_int4(i32(a.req_pool_indices[lo]), i32(full), i32(prefix + (t - a.cu_ext[lo])), 0);
+    }
+    a.rows4[t] = r4;
+    return;
+  }
   if (a.batch > 0 && t < a.cu_ext[a.batch]) {
     const int64_t r = t - a.cu_ext[lo];
     req = a.req_pool_indices[lo];
@@ -116,7 +127,7 @@ hipError_t launch_kv_scatter(const ScatterArgs& a, hipStream_t stream) {
 hipError_t launch_prefill_expand(const ExpandArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(prefill_cu_kernel, dim3(1), dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.total_q_tokens == 0 || a.row_req == nullptr) return e;
+  if (e != hipSuccess || a.total_q_tokens == 0 || (a.row_req == nullptr && a.rows4 == nullptr)) return e;
   hipLaunchKernelGGL(prefill_rows_kernel, dim3((a.total_q_tokens + 255) / 256), dim3(256), 0, stream, a);
   return hipGetLastError();
 }

@@ -382,6 +382,27 @@ int bsgl_paged_prefill(void* out /*device*/, int64_t out_row_stride,
                        void* workspace /*device*/, size_t workspace_bytes, void* stream);
 
 /*
+ * bsgl_paged_prefill (arguments, work list, workspace as there) with scored attention: visible_from / visible_to
+ * are per row of q, and a row's own position is prefix_lens[i] + r.  token_weights is not taken
+ * (BSGL_ERR_UNSUPPORTED).
+ */
+int bsgl_paged_prefill_scored(void* out /*device*/, int64_t out_row_stride,
+                              const void* q /*device*/, int64_t q_row_stride,
+                              const void* k_slab /*device*/, const void* v_slab /*device*/,
+                              int64_t slab_row_stride, int64_t n_slots,
+                              const int32_t* req_to_token /*device*/, int64_t table_row_stride,
+                              int64_t table_rows, int64_t table_cols,
+                              const int64_t* req_pool_indices /*device, [batch]*/,
+                              const int64_t* seq_lens /*device, [batch]*/,
+                              const int64_t* prefix_lens /*device, [batch]*/,
+                              const int64_t* extended_lens /*device, [batch]*/,
+                              int32_t batch, int32_t total_q_tokens,
+                              int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                              float scale, int32_t dtype, int32_t variant,
+                              void* workspace /*device*/, size_t workspace_bytes,
+                              const bsgl_score_mods* mods, void* stream);
+
+/*
  * Merge n_parts attention states computed over disjoint token sets:
  *   w_p = exp(lse_p - max_p lse_p);  out = sum_p w_p o_p / sum_p w_p
  * parts_o is [n_parts, rows, n_heads * head_dim] fp32 (already normalised),

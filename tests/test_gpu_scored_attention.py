@@ -317,3 +317,230 @@ def test_decode_refusals(gpu):
     with pytest.raises(RuntimeError):
         _hip.paged_decode_scored(d["q"].cpu(), *args[1:])
     assert math.isfinite(_hip.paged_decode_scored(*args).float().sum().item())
+
+
+# --------------------------------------------------------------------------- extend
+def intervals(kind, lens, ext, seed):
+    """Per extend row: {start, stop} lists of the mask kinds, or None."""
+    r = random.Random(seed)
+    start, stop = [], []
+    for n, e in zip(lens, ext):
+        cuts = sorted(r.randrange(n) for _ in range(3)) if n else []
+        for i in range(n - e, n):
+            a, b = 0, i + 1
+            if kind == "window":
+                a = max(0, i + 1 - max(1, n // 4))
+            elif kind == "prefix":
+                b = max(b, n // 2)
+            elif kind == "document":
+                a = max([0] + [c for c in cuts if c <= i])
+            elif kind == "both":  # a document read in both directions
+                a = max([0] + [c for c in cuts if c <= i])
+                b = min([n] + [c for c in cuts if c > i])
+            elif kind == "empty" and r.random() < 0.3:
+                b = a
+            elif kind == "wild":
+                a, b = r.randint(-5, n + 5), r.randint(-5, n + 5)
+            start.append(a)
+            stop.append(b)
+    return start, stop
+
+
+def extend_case(gpu, heads, dtype, ext, prefix, cap=0.0, slopes=False, kind=None, seed=0, layout="interleaved", extra_rows=0, only=None, poison=None, **kw):
+    from baby_sglang_amd import _hip
+
+    lens = [a + b for a, b in zip(ext, prefix)]
+    c = make(seed, heads, dtype, lens, layout, q_rows=sum(ext) + extra_rows)
+    st = sp = None
+    if kind is not None:
+        st, sp = (torch.tensor(x, dtype=torch.int32) for x in intervals(kind, lens, ext, seed))
+        st, sp = (torch.cat((x, torch.zeros(extra_rows, dtype=torch.int32))) for x in (st, sp))
+    row_req = [i for i, e in enumerate(ext) for _ in range(e)]
+    row_pos = [n - e + j for n, e in zip(lens, ext) for j in range(e)]
+    rows = list(range(sum(ext)))
+    scale = c["dim"] ** -0.5
+    sl = slopes_of(c["hq"]) if slopes else None
+    if poison is not None:
+        poison(c, row_req, row_pos, st, sp)
+    d = to_gpu(c, gpu)
+    out = torch.full((sum(ext) + extra_rows, c["hq"] * c["dim"]), -3.0, dtype=dtype, device=gpu)
+    got = _hip.paged_prefill_scored(
+        d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.tensor(prefix, device=gpu), torch.tensor(ext, device=gpu), scale=scale,
+        logit_cap=cap, slopes=sl.to(gpu) if slopes else None, visible_from=st.to(gpu) if st is not None else None,
+        visible_to=sp.to(gpu) if sp is not None else None, out=out, **kw)
+    torch.cuda.synchronize()
+    assert got is out
+    if extra_rows:
+        assert bool((out[sum(ext):] == -3.0).all())
+    if only is not None and len(rows) > only:
+        rows = sorted(random.Random(seed).sample(rows, only - 2) + [0, len(rows) - 1])
+    pick = lambda x: x[rows] if x is not None else None  # noqa: E731
+    want, mass, lse, _, top = orc.scored_exact(c["q"][rows], c["k"], c["v"], c["table"][c["req"]], lens, [row_req[r] for r in rows], [row_pos[r] for r in rows],
+                                               scale, cap, sl, pick(st), pick(sp))
+    u_p = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 0.0}[dtype]
+    finite = c["v"][c["v"].isfinite()].abs().max().item()
+    # (f16: probabilities stand against a reference up to 2^6 below the maximum, so the subnormal step is not scaled up)
+    check_rows(out[rows], want, mass, lse, top, cap, dtype, dtype, u_p, max(lens), finite, c["dim"])
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads", list(HEADS))
+@pytest.mark.parametrize("ext,prefix", [([3, 1, 0, 17, 40], [0, 5, 9, 33, 600]), ([130, 64, 1, 200], [0, 31, 70, 513])])
+def test_extend_types_and_heads(gpu, heads, dtype, ext, prefix):
+    hq, hkv, _ = HEADS[heads]
+    if hq // hkv > 8 and dtype == torch.float32:
+        pytest.skip("f32 kernels take up to 8 q heads per kv head")
+    extend_case(gpu, heads, dtype, ext, prefix, cap=8.0, slopes=True, only=60)
+
+
+@pytest.mark.parametrize("heads", ["1.5b", "0.5b"])
+@pytest.mark.parametrize("cap,slopes", [(0.0, False), (0.0, True), (3.0, False), (50.0, False), (50.0, True)])
+@pytest.mark.parametrize("kind", [None, "window", "prefix", "document", "both", "empty", "wild"])
+def test_extend_masks_and_shapes(gpu, heads, cap, slopes, kind):
+    extend_case(gpu, heads, torch.bfloat16, [150, 70, 33], [0, 100, 700], cap=cap, slopes=slopes, kind=kind, seed=20, only=70)
+    extend_case(gpu, heads, torch.float16, [9, 20, 33, 1], [0, 100, 40, 700], cap=cap, slopes=slopes, kind=kind, seed=21, only=40)
+
+
+@pytest.mark.parametrize("kind", [None, "document", "wild"])
+def test_extend_f32_masks(gpu, kind):
+    extend_case(gpu, "7b", torch.float32, [50, 20, 3], [0, 33, 300], cap=10.0, slopes=True, kind=kind, seed=22, only=40)
+
+
+@pytest.mark.parametrize("kw", [dict(layout="split"), dict(extra_rows=5), dict(variant=1), dict(variant=2)])
+def test_extend_launch_forms(gpu, kw):
+    extend_case(gpu, "7b", torch.bfloat16, [65, 100, 7], [513, 0, 64], cap=30.0, kind="document", seed=23, only=50, **kw)
+
+
+def test_extend_long(gpu):
+    """Several blocks of page-table entries, many steps; ring and entry staging wrap."""
+    extend_case(gpu, "one", torch.bfloat16, [700, 64], [2100, 1500], cap=20.0, slopes=True, seed=24, only=24)
+    extend_case(gpu, "mha", torch.float16, [1300], [0], kind="window", slopes=True, seed=25, only=24)
+
+
+def test_extend_many_requests(gpu):
+    r = random.Random(3)
+    ext = [r.choice([0, 1, 2, 5, 30, 64, 65, 129]) for _ in range(90)]
+    extend_case(gpu, "1.5b", torch.bfloat16, ext, [r.randint(0, 90) for _ in ext], cap=12.0, kind="document", seed=26, only=80)
+    ext = [r.randint(0, 20) for _ in range(130)]
+    extend_case(gpu, "7b", torch.float16, ext, [r.randint(0, 90) for _ in ext], slopes=True, kind="both", seed=27, only=80)
+
+
+def test_extend_all_rows_empty(gpu):
+    from baby_sglang_amd import _hip
+
+    c = make(28, "1.5b", torch.bfloat16, [70, 20], q_rows=90)
+    d = to_gpu(c, gpu)
+    out = _hip.paged_prefill_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.zeros(2, dtype=torch.int64, device=gpu), d["seq"],
+                                    logit_cap=5.0, visible_to=torch.zeros(90, dtype=torch.int32, device=gpu))
+    assert not bool(out.any())
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.11])
+def test_extend_scale_of_any_sign(gpu, scale):
+    from baby_sglang_amd import _hip
+
+    c = make(29, "1.5b", torch.bfloat16, [100], q_rows=100)
+    d = to_gpu(c, gpu)
+    for cap in (0.0, 6.0):
+        out = _hip.paged_prefill_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.zeros(1, dtype=torch.int64, device=gpu), d["seq"],
+                                        scale=scale, logit_cap=cap)
+        want, mass, lse, _, top = orc.scored_exact(c["q"], c["k"], c["v"], c["table"][c["req"]], [100], [0] * 100, range(100), scale, cap)
+        check_rows(out, want, mass, lse, top.abs(), cap, torch.bfloat16, torch.bfloat16, 2.0**-8, 100, 6.0, 128)
+
+
+@pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("0.5b", torch.float16), ("7b", torch.float32)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf"), "lowest"])
+def test_extend_nothing_leaks_from_hidden_tokens(gpu, heads, dtype, bad):
+    """A document whose keys and values are not finite beside documents that must not see it, in the same blocks;
+    rows that do see it are not looked at."""
+    from baby_sglang_amd import _hip
+
+    val = torch.finfo(dtype).min if bad == "lowest" else bad
+    lens, ext = [200, 90], [200, 90]
+    c = make(30, heads, dtype, lens, q_rows=290)
+    lo, hi = 70, 101  # the bad document of request 0
+    start = [0 if i < lo else lo if i < hi else hi for i in range(200)] + [0] * 90
+    stop = [lo if i < lo else hi if i < hi else 200 for i in range(200)] + [90] * 90
+    st, sp = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in (start, stop))
+    zero = torch.zeros(2, dtype=torch.int64, device=gpu)
+
+    def call(d):
+        return _hip.paged_prefill_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], zero, d["seq"], logit_cap=9.0, slopes=slopes_of(c["hq"]).to(gpu),
+                                         visible_from=st, visible_to=sp)
+
+    clean = call(to_gpu(c, gpu))
+    slots = c["table"][c["req"][0], lo:hi].long()
+    for what in ("k", "v"):
+        d = to_gpu(c, gpu)
+        d[what][slots.to(gpu)] = val
+        out = call(d)
+        rows = [i for i in range(290) if not lo <= i < hi]
+        assert bool(out[rows].isfinite().all())
+        # (rows that were computed again went through another order of sums: held to the definition)
+        want, mass, lse, _, top = orc.scored_exact(c["q"][rows], c["k"], c["v"], c["table"][c["req"]], lens, [0 if i < 200 else 1 for i in rows],
+                                                   [i if i < 200 else i - 200 for i in rows], c["dim"] ** -0.5, 9.0, slopes_of(c["hq"]),
+                                                   torch.tensor(start)[rows], torch.tensor(stop)[rows])
+        u_p = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 0.0}[dtype]
+        check_rows(out[rows], want, mass, lse, top, 9.0, dtype, dtype, u_p, 200, 6.0, c["dim"])
+        if what == "v" and isinstance(bad, float) and bad != bad:
+            assert bool(out[lo:hi].isnan().all())  # ... and who sees NaN gets NaN
+    assert bool(clean.isfinite().all())
+
+
+def test_extend_without_changes_agrees_with_the_plain_extend(gpu):
+    from baby_sglang_amd import _hip
+
+    for heads in ("1.5b", "7b", "0.5b"):
+        c = make(31, heads, torch.bfloat16, [300, 77, 610], q_rows=377)
+        d = to_gpu(c, gpu)
+        args = (d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.tensor([0, 0, 610], device=gpu), torch.tensor([300, 77, 0], device=gpu))
+        a, b = _hip.paged_prefill_scored(*args).float(), _hip.paged_prefill(*args).float()
+        assert bool(((a - b).abs() <= 2.0**-7 * b.abs() + 2.0**-6).all())  # (two roundings of p and of the result, mass <= 2)
+
+
+def test_extend_graph_replays_with_the_list_of_a_batch(gpu):
+    from baby_sglang_amd import _hip
+
+    c = make(32, "1.5b", torch.bfloat16, [200, 90, 333], q_rows=400)
+    d = to_gpu(c, gpu)
+    pre, ext = torch.tensor([0, 13, 210], device=gpu), torch.tensor([200, 77, 123], device=gpu)
+    st = torch.zeros(400, dtype=torch.int32, device=gpu)
+    ws = torch.empty(_hip.prefill_workspace_bytes(3, 400, 12, 128), dtype=torch.uint8, device=gpu)
+    out = torch.zeros(400, 12 * 128, dtype=torch.bfloat16, device=gpu)
+
+    def call(o, w, **kw):
+        return _hip.paged_prefill_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], pre, ext, logit_cap=9.0, visible_from=st, out=o, workspace=w, **kw)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = call(out, ws).clone()
+        assert torch.equal(call(torch.zeros_like(out), ws, list_ready=True), first)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out, ws)
+    for i in range(4):
+        d["q"].copy_(torch.randn_like(d["q"]))
+        st.fill_(i * 20)
+        eager = call(torch.zeros_like(out), None)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager), i
+
+
+def test_extend_refusals(gpu):
+    from baby_sglang_amd import _hip
+
+    d = to_gpu(make(33, "1.5b", torch.bfloat16, [20, 30], q_rows=50), gpu)
+    args = (d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.zeros(2, dtype=torch.int64, device=gpu), d["seq"])
+    for bad in (dict(logit_cap=-1.0), dict(slopes=torch.zeros(11, device=gpu)), dict(visible_from=torch.zeros(2, dtype=torch.int32, device=gpu)),
+                dict(visible_to=torch.zeros(50, device=gpu)), dict(out=torch.zeros(49, 1536, dtype=torch.bfloat16, device=gpu)), dict(list_ready=True)):
+        with pytest.raises(ValueError):
+            _hip.paged_prefill_scored(*args, **bad)
+    with pytest.raises(ValueError):
+        _hip.paged_prefill_scored(*args[:6], args[6][:1], args[7])
+    with pytest.raises(RuntimeError):
+        _hip.paged_prefill_scored(*args[:7], args[7].cpu())

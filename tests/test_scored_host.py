@@ -39,7 +39,7 @@ def test_scored_decode_refusals():
     assert f(decode_call(), mods(token_weights=256, token_weights_out=256, weights_row_stride=64)) == _hip.BSGL_ERR_WORKSPACE
     assert f(decode_call(n_splits=65), mods()) == _hip.BSGL_ERR_BAD_ARG
     assert f(decode_call(q=None), mods()) == _hip.BSGL_ERR_BAD_ARG
-    assert f(decode_call(dtype=7), mods()) == _hip.BSGL_ERR_UNSUPPORTED
+    assert f(decode_call(dtype=7, out_dtype=7), mods()) == _hip.BSGL_ERR_UNSUPPORTED
     assert f(decode_call(batch=0), mods(logit_cap=1.0)) == _hip.BSGL_OK  # nothing to do
 
 
