@@ -11,7 +11,6 @@ overlap_worker.py:104-127).
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import os
@@ -91,6 +90,13 @@ class LogitCall(ctypes.Structure):
     ]  # fmt: skip
 
 
+# the three descriptors as one packed write each (a Structure's fields assigned one by one cost more than
+# everything else these wrappers do); the bytes are passed as they are
+_PACK_DECODE = struct.Struct("=20q4if5i3q")
+_PACK_MODS = struct.Struct("=f4x6q")
+_PACK_LOGITS = struct.Struct("=21q4iq")
+assert (_PACK_DECODE.size, _PACK_MODS.size, _PACK_LOGITS.size) == tuple(ctypes.sizeof(t) for t in (DecodeCall, ScoreMods, LogitCall))
+
 # out .. out_cache_loc: the ten 8-byte fields a caller rewrites on every call, as one packed write
 DECODE_CALL_HEAD = struct.Struct("=10q")
 assert DecodeCall.out.offset == 0 and DecodeCall.out_cache_loc.offset == 72 and DecodeCall.k_slab.offset == 80
@@ -123,13 +129,13 @@ SIGNATURES = {
         + [_i32, _i32, _i32, _i32, _f32, _i32, _i32, _i32, _i32, _vp],
     ),
     "bsgl_decode_scored_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
-    "bsgl_paged_decode_scored": (ctypes.c_int, [ctypes.POINTER(DecodeCall), ctypes.POINTER(ScoreMods)]),
+    "bsgl_paged_decode_scored": (ctypes.c_int, [_vp, _vp]),
     "bsgl_evict_workspace_bytes": (_sz, [_i32, _i64, _i32]),
     "bsgl_evict_tokens": (
         ctypes.c_int,
         [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64] + [_i32] * 6 + [_vp, _sz, _vp],
     ),
-    "bsgl_logit_controls": (ctypes.c_int, [ctypes.POINTER(LogitCall)]),
+    "bsgl_logit_controls": (ctypes.c_int, [_vp]),
     "bsgl_prefill_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "bsgl_paged_prefill": (
         ctypes.c_int,
@@ -139,7 +145,7 @@ SIGNATURES = {
     "bsgl_paged_prefill_scored": (
         ctypes.c_int,
         [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]
-        + [_i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _sz, ctypes.POINTER(ScoreMods), _vp],
+        + [_i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _sz, _vp, _vp],
     ),
     "bsgl_merge_attn_states": (
         ctypes.c_int,
@@ -263,36 +269,63 @@ def _rows3(x: torch.Tensor):
     return x, sh, st
 
 
-def _on_device(device: torch.device):
-    """The tensors' device made current for the launch (a launch goes to the current device, whatever
+try:  # the current device's index without the lazy-initialisation checks around it
+    _current_device = torch._C._cuda_getDevice
+except AttributeError:  # pragma: no cover
+    _current_device = torch.cuda.current_device
+
+
+def _launch(device_index: int, fn, *args) -> int:
+    """``fn(*args, stream)`` with the tensors' device current (a launch goes to the current device, whatever
     stream it names)."""
-    return contextlib.nullcontext() if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    if device_index == _current_device():
+        return fn(*args, current_stream_handle(device_index))
+    with torch.cuda.device(device_index):
+        return fn(*args, current_stream_handle(device_index))
 
 
-def _check_out(out: torch.Tensor, rows: int, width: int, dtype: torch.dtype) -> None:
-    if tuple(out.shape) != (rows, width) or out.dtype != dtype or (rows > 0 and out.stride(1) != 1) or not out.is_cuda:
-        raise ValueError(f"out must be {dtype} [{rows}, {width}] with unit column stride on the GPU, got {out.dtype} {tuple(out.shape)}")
+def _check_out(out: torch.Tensor, rows: int, width: int, dtype: torch.dtype) -> int:
+    """The row stride of a result tensor of the wanted kind."""
+    row, col = out.stride() if out.dim() == 2 else (0, 0)
+    if out.shape != (rows, width) or out.dtype != dtype or (width > 1 and col != 1) or (rows > 1 and row < width) or not out.is_cuda:
+        raise ValueError(f"out must be {dtype} [{rows}, {width}] with dense rows on the GPU, got {out.dtype} {tuple(out.shape)}")
+    return row if rows > 1 else width
 
 
-def _check_slabs(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor, dim: int) -> None:
-    if k_slab.dtype != q.dtype or v_slab.dtype != q.dtype:
-        raise ValueError(f"q is {q.dtype} but the KV slabs are {k_slab.dtype}")
-    if k_slab.dim() != 3 or k_slab.shape != v_slab.shape or k_slab.shape[2] != dim:
-        raise ValueError(f"KV slabs must be [slots, kv heads, {dim}], got {tuple(k_slab.shape)} and {tuple(v_slab.shape)}")
-    if k_slab.stride() != v_slab.stride() or k_slab.stride(2) != 1 or k_slab.stride(1) != dim:
+def _check_slabs(q_dtype: torch.dtype, k_slab: torch.Tensor, v_slab: torch.Tensor, dim: int):
+    """``(slots, kv heads, row stride)`` of a pair of slabs."""
+    shape, stride = k_slab.shape, k_slab.stride()
+    if k_slab.dtype != q_dtype or v_slab.dtype != q_dtype:
+        raise ValueError(f"q is {q_dtype} but the KV slabs are {k_slab.dtype}")
+    if len(shape) != 3 or shape != v_slab.shape or shape[2] != dim:
+        raise ValueError(f"KV slabs must be [slots, kv heads, {dim}], got {tuple(shape)} and {tuple(v_slab.shape)}")
+    if stride != v_slab.stride() or stride[2] != 1 or stride[1] != dim:
         raise ValueError("K and V slabs must share a row stride and have dense rows")
+    return shape[0], shape[1], stride[0]
 
 
-def _check_table(req_to_token: torch.Tensor) -> None:
-    if req_to_token.dim() != 2 or req_to_token.dtype != torch.int32 or req_to_token.stride(1) != 1:
+def _check_table(req_to_token: torch.Tensor):
+    """``(rows, columns, row stride)`` of a page table."""
+    shape, stride = req_to_token.shape, req_to_token.stride()
+    if len(shape) != 2 or req_to_token.dtype != torch.int32 or stride[1] != 1:
         raise ValueError("req_to_token must be a 2-D int32 tensor with unit column stride")
+    return shape[0], shape[1], stride[0]
+
+
+def _check_weights(t: torch.Tensor, table_shape, cols: int) -> int:
+    """The row stride of a table of token weights."""
+    stride = t.stride()
+    if t.dtype != torch.float32 or t.shape != table_shape or stride[1] != 1 or stride[0] < cols or not t.is_cuda:
+        raise ValueError(f"token weights must be float32 of the page table's shape {tuple(table_shape)} with dense rows on the GPU")
+    return stride[0]
 
 
 def _index_rows(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     """A dense int64 vector of ``n`` entries on the GPU."""
-    if tuple(t.shape) != (n,):
-        raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
-    t = t if t.dtype == torch.int64 else t.to(torch.int64)
+    if t.shape != (n,) or not t.is_cuda:
+        raise ValueError(f"{name} must have shape ({n},) on the GPU, got {tuple(t.shape)} on {t.device}")
+    if t.dtype != torch.int64:
+        t = t.to(torch.int64)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -490,36 +523,30 @@ def paged_decode(
 
 
 def _score_mods(rows: int, n_q_heads: int, device, logit_cap, slopes, visible_from, visible_to):
-    """A ``ScoreMods`` with its checks; the tensors it points into are returned beside it (the caller
-    keeps them until the call has been made)."""
-    m = ScoreMods()
-    cap = float(logit_cap or 0.0)
+    """The checked parts of a ``bsgl_score_mods`` as numbers, ``(cap, slopes, from, to)``, and the tensors
+    behind the pointers (the caller keeps them until the call has been made)."""
+    cap = float(logit_cap) if logit_cap else 0.0
     if not (0.0 <= cap < math.inf):
         raise ValueError(f"logit_cap {logit_cap} is negative or not finite")
-    m.logit_cap = cap
     keep = []
+    ptr = [0, 0, 0]
     if slopes is not None:
-        _need_gpu(slopes)
-        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (n_q_heads,):
-            raise ValueError(f"slopes must be float32 of shape ({n_q_heads},), got {slopes.dtype} {tuple(slopes.shape)}")
+        if slopes.dtype != torch.float32 or slopes.shape != (n_q_heads,) or slopes.device != device:
+            raise ValueError(f"slopes must be float32 of shape ({n_q_heads},) on {device}, got {slopes.dtype} {tuple(slopes.shape)} on {slopes.device}")
         slopes = slopes if slopes.is_contiguous() else slopes.contiguous()
         keep.append(slopes)
-        m.slopes = slopes.data_ptr()
-    for name, t in (("visible_from", visible_from), ("visible_to", visible_to)):
+        ptr[0] = slopes.data_ptr()
+    for at, t in ((1, visible_from), (2, visible_to)):
         if t is None:
             continue
-        _need_gpu(t)
-        if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (rows,):
-            raise ValueError(f"{name} must be int32 of shape ({rows},), got {t.dtype} {tuple(t.shape)}")
+        if t.dtype not in (torch.int32, torch.int64) or t.shape != (rows,) or t.device != device:
+            raise ValueError(f"visible_from / visible_to must be int32 of shape ({rows},) on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         if t.dtype == torch.int64:  # (positions fit 32 bits; what does not stays outside the sequence either way)
             t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
         t = t if t.is_contiguous() else t.contiguous()
         keep.append(t)
-        setattr(m, name, t.data_ptr())
-    for t in keep:
-        if t.device != device:
-            raise ValueError(f"score tensors must be on q's device {device}, got {t.device}")
-    return m, keep
+        ptr[at] = t.data_ptr()
+    return (cap, *ptr), keep
 
 
 def decode_scored_workspace_bytes(
@@ -572,73 +599,81 @@ def paged_decode_scored(
     if len(q_shape) != 3:
         raise ValueError(f"q must be [batch, heads, dim], got shape {tuple(q_shape)}")
     batch, hq, dim = q_shape
-    hkv = k_slab.shape[1]
+    device, q_dtype = q.device, q.dtype
+    q_code = _DTYPE_CODE_GET(q_dtype)
+    if q_code is None:
+        raise NotImplementedError(f"dtype {q_dtype} has no HIP attention kernel")
     if out_dtype is None:
-        out_dtype = out.dtype if out is not None else q.dtype
+        out_dtype = out.dtype if out is not None else q_dtype
     if out is None:
-        out = torch.empty((batch, hq * dim), dtype=out_dtype, device=q.device)
-    _check_out(out, batch, hq * dim, out_dtype)
+        out = torch.empty((batch, hq * dim), dtype=out_dtype, device=device)
+    out_stride = _check_out(out, batch, hq * dim, out_dtype)
     if batch == 0:
         return out
-    _check_slabs(q, k_slab, v_slab, dim)
-    _check_table(req_to_token)
-    rows, lens = (_index_rows(t, batch, n) for t, n in ((req_pool_indices, "req_pool_indices"), (seq_lens, "seq_lens")))
+    out_code = _DTYPE_CODE_GET(out_dtype, -1)
+    slots, hkv, slab_stride = _check_slabs(q_dtype, k_slab, v_slab, dim)
+    rows, cols, table_stride = _check_table(req_to_token)
+    req_pool_indices = _index_rows(req_pool_indices, batch, "req_pool_indices")
+    seq_lens = _index_rows(seq_lens, batch, "seq_lens")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    cols = req_to_token.shape[1]
     if n_splits is None:
         n_splits = decode_num_splits(batch, hkv, cols)
-    mods, keep = _score_mods(batch, hq, q.device, logit_cap, slopes, visible_from, visible_to)
-    if token_weights is None and token_weights_out is not None:
-        raise ValueError("token_weights_out without token_weights")
+    mods, keep = _score_mods(batch, hq, device, logit_cap, slopes, visible_from, visible_to)
+    weights = (0, 0, 0)
     if token_weights is not None:
+        w_stride = _check_weights(token_weights, req_to_token.shape, cols)
         if token_weights_out is None:
             token_weights_out = token_weights
-        for t in (token_weights, token_weights_out):
-            _need_gpu(t)
-            if t.dtype != torch.float32 or t.shape != req_to_token.shape or t.stride(1) != 1 or t.stride(0) < cols:
-                raise ValueError(f"token weights must be float32 of the page table's shape {tuple(req_to_token.shape)} with dense rows")
-        if token_weights.stride(0) != token_weights_out.stride(0):
+        elif _check_weights(token_weights_out, req_to_token.shape, cols) != w_stride:
             raise ValueError("token_weights and token_weights_out must share a row stride")
-        mods.token_weights, mods.token_weights_out = token_weights.data_ptr(), token_weights_out.data_ptr()
-        mods.weights_row_stride = token_weights.stride(0)
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (batch, hq) or not lse.is_contiguous()):
-        raise ValueError(f"lse must be dense float32 [{batch}, {hq}]")
-    need = decode_scored_workspace_bytes(batch, hq, dim, n_splits, cols, token_weights is not None, out_dtype != q.dtype)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = new_decode_workspace(need, q.device)
-    c = DecodeCall()
+        weights = (token_weights.data_ptr(), token_weights_out.data_ptr(), w_stride)
+    elif token_weights_out is not None:
+        raise ValueError("token_weights_out without token_weights")
+    lse_ptr = 0
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.shape != (batch, hq) or not lse.is_contiguous():
+            raise ValueError(f"lse must be dense float32 [{batch}, {hq}]")
+        lse_ptr = lse.data_ptr()
+    need = lib.bsgl_decode_scored_workspace_bytes(batch, hq, dim, n_splits, out_dtype != q_dtype, cols, token_weights is not None)
+    ws_ptr = ws_bytes = 0
+    if need:
+        if workspace is not None:
+            ws_bytes = workspace.numel() * workspace.element_size()
+        if ws_bytes < need:
+            workspace = new_decode_workspace(need, device)
+            ws_bytes = need
+        ws_ptr = workspace.data_ptr()
+    new = (0, 0, 0, 0, 0)
     if k_new is not None or v_new is not None or out_cache_loc is not None:
         if k_new is None or v_new is None or out_cache_loc is None:
             raise ValueError("k_new, v_new and out_cache_loc go together")
         k_new, kn_shape, kn_stride = _rows3(k_new.view(batch, hkv, dim) if k_new.dim() == 2 else k_new)
         v_new, vn_shape, vn_stride = _rows3(v_new.view(batch, hkv, dim) if v_new.dim() == 2 else v_new)
-        if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
+        if k_new.dtype != q_dtype or v_new.dtype != q_dtype:
             raise ValueError("new K/V rows must have q's dtype")
-        if tuple(kn_shape) != (batch, hkv, dim) or tuple(vn_shape) != (batch, hkv, dim):
+        if kn_shape != (batch, hkv, dim) or vn_shape != (batch, hkv, dim):
             raise ValueError("new K/V rows must be [batch, n_kv_heads, head_dim]")
         loc = out_cache_loc if out_cache_loc.dtype == torch.int32 else out_cache_loc.to(torch.int32)
         loc = loc if loc.is_contiguous() else loc.contiguous()
-        if tuple(loc.shape) != (batch,):
+        if loc.shape != (batch,):
             raise ValueError("out_cache_loc must have one slot per request")
-        c.k_new, c.v_new, c.k_new_row_stride, c.v_new_row_stride = k_new.data_ptr(), v_new.data_ptr(), kn_stride[0], vn_stride[0]
-        c.out_cache_loc = loc.data_ptr()
+        new = (k_new.data_ptr(), v_new.data_ptr(), kn_stride[0], vn_stride[0], loc.data_ptr())
         if fuse_kv_write:
             variant |= DECODE_FUSE_KV_WRITE
-    c.out, c.out_row_stride, c.lse = out.data_ptr(), out.stride(0), lse.data_ptr() if lse is not None else None
-    c.q, c.q_row_stride = q.data_ptr(), q_stride[0]
-    c.k_slab, c.v_slab, c.slab_row_stride, c.n_slots = k_slab.data_ptr(), v_slab.data_ptr(), k_slab.stride(0), k_slab.shape[0]
-    c.req_to_token, c.table_row_stride = req_to_token.data_ptr(), req_to_token.stride(0)
-    c.table_rows, c.table_cols = req_to_token.shape
-    c.req_pool_indices, c.seq_lens = rows.data_ptr(), lens.data_ptr()
-    c.batch, c.n_q_heads, c.n_kv_heads, c.head_dim, c.scale = batch, hq, hkv, dim, scale
-    c.dtype, c.out_dtype, c.n_splits, c.variant = _dtype_code(q), _DTYPE_CODE[out_dtype], n_splits, variant
-    c.max_seq_len = int(max_seq_len)
-    c.workspace = workspace.data_ptr() if need else None
-    c.workspace_bytes = workspace.numel() * workspace.element_size() if need else 0
-    with _on_device(q.device):
-        c.stream = _stream_ptr(q.device)
-        _check(lib.bsgl_paged_decode_scored(ctypes.byref(c), ctypes.byref(mods)), "bsgl_paged_decode_scored")
+
+    def call(stream):
+        return lib.bsgl_paged_decode_scored(
+            _PACK_DECODE.pack(
+                out.data_ptr(), out_stride, lse_ptr, q.data_ptr(), q_stride[0], *new, k_slab.data_ptr(), v_slab.data_ptr(), slab_stride, slots,
+                req_to_token.data_ptr(), table_stride, rows, cols, req_pool_indices.data_ptr(), seq_lens.data_ptr(),
+                batch, hq, hkv, dim, scale, q_code, out_code, n_splits, variant, int(max_seq_len), ws_ptr, ws_bytes, stream),
+            _PACK_MODS.pack(*mods, *weights),
+        )  # fmt: skip
+
+    rc = _launch(device.index, call)
+    if rc:
+        _check(rc, "bsgl_paged_decode_scored")
     return out
 
 
@@ -672,60 +707,50 @@ def evict_tokens(
     and strides).  ``evicted`` may be given with any width; by default it has room for every slot that can go
     (``max_seq_len``, 0 = the table's width, less the budget)."""
     _need_gpu(req_to_token, token_weights, req_pool_indices, seq_lens)
-    _check_table(req_to_token)
-    n_rows, cols = req_to_token.shape
-    batch = int(req_pool_indices.shape[0])
-    rows, lens = (_index_rows(t, batch, n) for t, n in ((req_pool_indices, "req_pool_indices"), (seq_lens, "seq_lens")))
-    budget, recent, sinks = int(budget), int(recent), int(sinks)
+    n_rows, cols, stride = _check_table(req_to_token)
+    shape, device = req_to_token.shape, req_to_token.device
+    batch = req_pool_indices.shape[0]
+    req_pool_indices = _index_rows(req_pool_indices, batch, "req_pool_indices")
+    seq_lens = _index_rows(seq_lens, batch, "seq_lens")
+    w_stride = _check_weights(token_weights, shape, cols)
     if out_table is None:
         out_table = req_to_token
+    elif out_table.dtype != torch.int32 or out_table.shape != shape or out_table.stride() != req_to_token.stride() or not out_table.is_cuda:
+        raise ValueError("out_table must have the page table's type, shape and strides")
     if out_weights is None:
         out_weights = token_weights
-    for t in (token_weights, out_weights):
-        _need_gpu(t)
-        if t.dtype != torch.float32 or t.shape != req_to_token.shape or t.stride(1) != 1 or t.stride(0) < cols:
-            raise ValueError(f"token weights must be float32 of the page table's shape {tuple(req_to_token.shape)} with dense rows")
-    if out_table.dtype != torch.int32 or out_table.shape != req_to_token.shape or out_table.stride() != req_to_token.stride() \
-            or out_weights.stride() != token_weights.stride():
-        raise ValueError("out_table and out_weights must have their inputs' types, shapes and strides")
+    elif _check_weights(out_weights, shape, cols) != w_stride:
+        raise ValueError("out_weights must have the token weights' strides")
     if new_lens is None:
-        new_lens = torch.empty(batch, dtype=torch.int64, device=req_to_token.device)
-    elif new_lens.dtype != torch.int64 or tuple(new_lens.shape) != (batch,) or not new_lens.is_contiguous():
-        raise ValueError(f"new_lens must be a dense int64 vector of {batch} entries")
+        new_lens = torch.empty(batch, dtype=torch.int64, device=device)
+    elif new_lens.dtype != torch.int64 or new_lens.shape != (batch,) or not new_lens.is_contiguous() or not new_lens.is_cuda:
+        raise ValueError(f"new_lens must be a dense int64 vector of {batch} entries on the GPU")
     if evicted is None:
         longest = min(int(max_seq_len), cols) if max_seq_len > 0 else cols
-        evicted = torch.empty((batch, max(0, longest - budget)), dtype=torch.int32, device=req_to_token.device)
-    elif evicted.dtype != torch.int32 or evicted.dim() != 2 or evicted.shape[0] != batch or (evicted.shape[1] > 1 and evicted.stride(1) != 1):
-        raise ValueError("evicted must be int32 [batch, width] with dense rows")
-    need = evict_workspace_bytes(batch, cols, budget)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=req_to_token.device)
-    with _on_device(req_to_token.device):
-        rc = lib.bsgl_evict_tokens(
-            out_table.data_ptr(), out_weights.data_ptr(), req_to_token.data_ptr(), req_to_token.stride(0),
-            token_weights.data_ptr(), token_weights.stride(0), n_rows, cols, rows.data_ptr(), lens.data_ptr(),
-            new_lens.data_ptr(), evicted.data_ptr() if evicted.shape[1] else None, max(evicted.stride(0), evicted.shape[1]), evicted.shape[1],
-            batch, budget, recent, sinks, int(max_seq_len),
-            workspace.data_ptr() if need else None, workspace.numel() * workspace.element_size() if need else 0,
-            _stream_ptr(req_to_token.device),
-        )  # fmt: skip
-    _check(rc, "bsgl_evict_tokens")
+        evicted = torch.empty((batch, max(0, longest - budget)), dtype=torch.int32, device=device)
+    elif evicted.dtype != torch.int32 or evicted.dim() != 2 or evicted.shape[0] != batch or not evicted.is_cuda \
+            or (evicted.shape[1] > 1 and evicted.stride(1) != 1):
+        raise ValueError("evicted must be int32 [batch, width] with dense rows on the GPU")
+    width = evicted.shape[1]
+    need = lib.bsgl_evict_workspace_bytes(batch, cols, budget)
+    ws_ptr = ws_bytes = 0
+    if need:
+        if workspace is not None:
+            ws_bytes = workspace.numel() * workspace.element_size()
+        if ws_bytes < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            ws_bytes = need
+        ws_ptr = workspace.data_ptr()
+    rc = _launch(
+        device.index, lib.bsgl_evict_tokens, out_table.data_ptr(), out_weights.data_ptr(), req_to_token.data_ptr(), stride,
+        token_weights.data_ptr(), w_stride, n_rows, cols, req_pool_indices.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(),
+        evicted.data_ptr() if width else None, max(evicted.stride(0), width), width, batch, budget, recent, sinks, int(max_seq_len), ws_ptr, ws_bytes)
+    if rc:
+        _check(rc, "bsgl_evict_tokens")
     return new_lens, evicted
 
 
 # ---- logit controls -----------------------------------------------------------------------------
-
-
-def _row_floats(x, batch: int, device, name: str):
-    """A per-request float32 vector; a plain number stands for every request."""
-    if x is None:
-        return None
-    if not isinstance(x, torch.Tensor):
-        return torch.full((batch,), float(x), dtype=torch.float32, device=device)
-    _need_gpu(x)
-    if x.dtype != torch.float32 or tuple(x.shape) != (batch,):
-        raise ValueError(f"{name} must be float32 of shape ({batch},), got {x.dtype} {tuple(x.shape)}")
-    return x if x.is_contiguous() else x.contiguous()
 
 
 def logit_controls(
@@ -753,79 +778,79 @@ def logit_controls(
     vocabulary are unused places).  ``token_mask`` int32 [rows, ceil(vocab / 32)], bit t % 32 of word t / 32 set =
     token t allowed; ``mask_rows`` int32 [batch] (default i; negative = no mask)."""
     _need_gpu(logits)
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("logits must be [batch, vocab] with unit column stride")
-    batch, vocab = logits.shape
-    dev = logits.device
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1) or (shape[0] > 1 and stride[0] < shape[1]):
+        raise ValueError("logits must be [batch, vocab] with dense rows")
+    batch, vocab = shape
+    device = logits.device
+    code = _dtype_code(logits)
     if out is None:
-        out = torch.empty((batch, vocab), dtype=logits.dtype, device=dev)
-    _check_out(out, batch, vocab, logits.dtype)
-    c = LogitCall()
-    c.dtype = _dtype_code(logits)
+        out = torch.empty((batch, vocab), dtype=logits.dtype, device=device)
+    out_stride = _check_out(out, batch, vocab, logits.dtype)
     keep = []
 
-    def vector(t, dtype, name):
-        _need_gpu(t)
-        if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (batch,):
-            raise ValueError(f"{name} must be a vector of {batch} integers, got {t.dtype} {tuple(t.shape)}")
-        t = t.to(dtype).contiguous()
+    def vector(t, dtypes, name):  # the address of a [batch] vector of one of the types, as the first of them
+        if t is None:
+            return 0
+        if t.dtype not in dtypes or t.shape != (batch,) or t.device != device:
+            raise ValueError(f"{name} must be {dtypes[0]} of shape ({batch},) on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.dtype != dtypes[0]:
+            t = t.to(dtypes[0])
+        if not t.is_contiguous():
+            t = t.contiguous()
         keep.append(t)
         return t.data_ptr()
 
-    def table(t, dtype, name):
-        _need_gpu(t)
-        if t.dtype != dtype or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-            raise ValueError(f"{name} must be a 2-D {dtype} tensor with dense rows")
-        keep.append(t)
-        return t.data_ptr(), max(t.stride(0), t.shape[1])
+    def floats(t, name):
+        if t is not None and not isinstance(t, torch.Tensor):
+            t = torch.full((batch,), float(t), dtype=torch.float32, device=device)
+        return vector(t, (torch.float32,), name)
 
+    def table(t, dtype, name):  # (address, row stride, rows, columns) of a 2-D table with dense rows
+        sh, st = t.shape, t.stride()
+        if t.dtype != dtype or len(sh) != 2 or (sh[1] > 1 and st[1] != 1) or (sh[0] > 1 and st[0] < sh[1]) or t.device != device:
+            raise ValueError(f"{name} must be a 2-D {dtype} tensor with dense rows on {device}")
+        return t.data_ptr(), st[0] if sh[0] > 1 else sh[1], sh[0], sh[1]
+
+    long, int_ = (torch.int64, torch.int32), (torch.int32, torch.int64)
+    past = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     if history is not None:
         if history_lens is None:
             raise ValueError("history needs history_lens")
-        c.history, c.history_row_stride = table(history, torch.int32, "history")
-        c.history_n_rows, c.history_cols = history.shape
-        c.history_lens = vector(history_lens, torch.int64, "history_lens")
-        c.history_rows = vector(history_rows, torch.int64, "history_rows") if history_rows is not None else None
-        c.prompt_lens = vector(prompt_lens, torch.int64, "prompt_lens") if prompt_lens is not None else None
-        for name, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-            x = _row_floats(x, batch, dev, name)
-            if x is not None:
-                keep.append(x)
-                setattr(c, name, x.data_ptr())
+        h = table(history, torch.int32, "history")
+        past = (*h, vector(history_rows, long, "history_rows"), vector(history_lens, long, "history_lens"), vector(prompt_lens, long, "prompt_lens"),
+                floats(repetition, "repetition"), floats(presence, "presence"), floats(frequency, "frequency"))
     elif any(x is not None for x in (repetition, presence, frequency, history_rows, history_lens, prompt_lens)):
         raise ValueError("penalties and history rows need a history")
-    if (bias_ids is None) != (bias_values is None):
-        raise ValueError("bias_ids and bias_values go together")
-    if bias_ids is not None:
-        if bias_ids.shape != bias_values.shape or bias_ids.dim() != 2 or bias_ids.shape[0] != batch:
-            raise ValueError("bias_ids and bias_values must be [batch, n]")
-        c.bias_ids, c.bias_row_stride = table(bias_ids, torch.int32, "bias_ids")
-        c.bias_values, stride = table(bias_values, torch.float32, "bias_values")
-        if stride != c.bias_row_stride:
+    bias = (0, 0, 0)
+    n_bias = 0
+    if bias_ids is not None or bias_values is not None:
+        if bias_ids is None or bias_values is None or bias_ids.shape != bias_values.shape or bias_ids.dim() != 2 or bias_ids.shape[0] != batch:
+            raise ValueError("bias_ids and bias_values go together and must be [batch, n]")
+        b, v = table(bias_ids, torch.int32, "bias_ids"), table(bias_values, torch.float32, "bias_values")
+        if b[1] != v[1]:
             raise ValueError("bias_ids and bias_values must share a row stride")
-        c.n_bias = bias_ids.shape[1]
+        bias, n_bias = (b[0], v[0], b[1]), b[3]
+    mask = (0, 0, 0, 0)
     if token_mask is not None:
-        c.token_mask, c.mask_row_stride = table(token_mask, torch.int32, "token_mask")
-        if token_mask.shape[1] < (vocab + 31) // 32:
-            raise ValueError(f"token_mask rows hold {32 * token_mask.shape[1]} bits, the vocabulary has {vocab} tokens")
-        c.mask_n_rows = token_mask.shape[0]
-        if mask_rows is not None:
-            c.mask_rows = vector(mask_rows, torch.int32, "mask_rows")
-        elif token_mask.shape[0] < batch:
+        m = table(token_mask, torch.int32, "token_mask")
+        if m[3] < (vocab + 31) // 32:
+            raise ValueError(f"token_mask rows hold {32 * m[3]} bits, the vocabulary has {vocab} tokens")
+        if mask_rows is None and m[2] < batch:
             raise ValueError("token_mask has fewer rows than the batch")
+        mask = (m[0], m[1], m[2], vector(mask_rows, int_, "mask_rows"))
     elif mask_rows is not None:
         raise ValueError("mask_rows without token_mask")
-    for t in keep:
-        if t.device != dev:
-            raise ValueError(f"all tensors must be on the logits' device {dev}, got {t.device}")
     if batch == 0 or vocab == 0:
         return out
-    c.out, c.out_row_stride = out.data_ptr(), max(out.stride(0), vocab)
-    c.logits, c.logits_row_stride = logits.data_ptr(), max(logits.stride(0), vocab)
-    c.batch, c.vocab = batch, vocab
-    with _on_device(dev):
-        c.stream = _stream_ptr(dev)
-        _check(lib.bsgl_logit_controls(ctypes.byref(c)), "bsgl_logit_controls")
+
+    def call(stream):
+        return lib.bsgl_logit_controls(_PACK_LOGITS.pack(
+            out.data_ptr(), logits.data_ptr(), out_stride, stride[0] if batch > 1 else vocab, *past, *bias, *mask, n_bias, batch, vocab, code, stream))
+
+    rc = _launch(device.index, call)
+    if rc:
+        _check(rc, "bsgl_logit_controls")
     return out
 
 
@@ -909,39 +934,41 @@ def paged_prefill_scored(
     request; the default sees everything up to the row's own position.  Rows behind the last request's are left as
     they were."""
     _need_gpu(q, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens, prefix_lens, extended_lens)
-    q = _rows(q)
-    if q.dim() != 3:
-        raise ValueError(f"q must be [tokens, heads, dim], got shape {tuple(q.shape)}")
-    total_q, hq, dim = q.shape
-    hkv = k_slab.shape[1]
-    batch = int(req_pool_indices.shape[0])
+    q, q_shape, q_stride = _rows3(q)
+    if len(q_shape) != 3:
+        raise ValueError(f"q must be [tokens, heads, dim], got shape {tuple(q_shape)}")
+    total_q, hq, dim = q_shape
+    device = q.device
+    batch = req_pool_indices.shape[0]
     if out is None:
-        out = torch.empty((total_q, hq * dim), dtype=q.dtype, device=q.device)
-    _check_out(out, total_q, hq * dim, q.dtype)
+        out = torch.empty((total_q, hq * dim), dtype=q.dtype, device=device)
+    out_stride = _check_out(out, total_q, hq * dim, q.dtype)
     if total_q == 0 or batch == 0:
         return out
-    _check_slabs(q, k_slab, v_slab, dim)
-    _check_table(req_to_token)
-    names = ("req_pool_indices", "seq_lens", "prefix_lens", "extended_lens")
-    i64 = [_index_rows(t, batch, n) for t, n in zip((req_pool_indices, seq_lens, prefix_lens, extended_lens), names)]
+    slots, hkv, slab_stride = _check_slabs(q.dtype, k_slab, v_slab, dim)
+    rows, cols, table_stride = _check_table(req_to_token)
+    req_pool_indices = _index_rows(req_pool_indices, batch, "req_pool_indices")
+    seq_lens = _index_rows(seq_lens, batch, "seq_lens")
+    prefix_lens = _index_rows(prefix_lens, batch, "prefix_lens")
+    extended_lens = _index_rows(extended_lens, batch, "extended_lens")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    mods, keep = _score_mods(total_q, hq, q.device, logit_cap, slopes, visible_from, visible_to)
-    need = prefill_workspace_bytes(batch, total_q, hq, dim)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
+    mods, keep = _score_mods(total_q, hq, device, logit_cap, slopes, visible_from, visible_to)
+    need = lib.bsgl_prefill_workspace_bytes(batch, total_q, hq, dim)
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    if ws_bytes < need:
         if list_ready:
             raise ValueError("list_ready needs the workspace that holds the list")
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    with _on_device(q.device):
-        rc = lib.bsgl_paged_prefill_scored(
-            out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0),
-            k_slab.data_ptr(), v_slab.data_ptr(), k_slab.stride(0), k_slab.shape[0],
-            req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[0], req_to_token.shape[1],
-            i64[0].data_ptr(), i64[1].data_ptr(), i64[2].data_ptr(), i64[3].data_ptr(),
-            batch, total_q, hq, hkv, dim, scale, _dtype_code(q), variant | (PREFILL_LIST_READY if list_ready else 0),
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(), ctypes.byref(mods), _stream_ptr(q.device),
-        )  # fmt: skip
-    _check(rc, "bsgl_paged_prefill_scored")
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        ws_bytes = need
+    rc = _launch(
+        device.index, lib.bsgl_paged_prefill_scored, out.data_ptr(), out_stride, q.data_ptr(), q_stride[0],
+        k_slab.data_ptr(), v_slab.data_ptr(), slab_stride, slots, req_to_token.data_ptr(), table_stride, rows, cols,
+        req_pool_indices.data_ptr(), seq_lens.data_ptr(), prefix_lens.data_ptr(), extended_lens.data_ptr(),
+        batch, total_q, hq, hkv, dim, scale, _dtype_code(q), variant | (PREFILL_LIST_READY if list_ready else 0),
+        workspace.data_ptr(), ws_bytes, _PACK_MODS.pack(*mods, 0, 0, 0))
+    if rc:
+        _check(rc, "bsgl_paged_prefill_scored")
     return out
 
 
