@@ -87,6 +87,9 @@ struct DecodeArgs {
   int32_t dtype;
   int32_t out_dtype;  // dtype, or kF32 (then results always pass through the merge kernel)
   int32_t n_splits;
+  // scored form, > 0: pieces wanted per request as if n_splits were this (n_splits itself then only bounds how finely
+  // the longest requests may be cut); what the kernels that cut every request alike use
+  int32_t base_splits;
   float* ws_o;    // [n_splits, rows * n_q_heads, head_dim]   (unless direct)
   float* ws_lse;  // [n_splits, rows * n_q_heads]
   uint32_t* counters;  // [rows, head groups] tickets of the in-kernel merge; zero between launches; may be NULL

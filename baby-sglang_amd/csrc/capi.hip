@@ -139,6 +139,7 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   } else if (variant != BSGL_DECODE_VALU) {
     return fail(BSGL_ERR_BAD_ARG, "unknown decode variant %d", variant);
   }
+  if (!use_mfma && a.base_splits > 0) a.n_splits = a.base_splits;  // (every row is cut into n_splits equal pieces there)
   if (!use_mfma && !bsgl::decode_valu_supported(a, &why)) return fail(BSGL_ERR_UNSUPPORTED, "decode: %s", why);
   // KV write of the new tokens: inside the matrix-core kernel when the caller
   // allows it and the rows qualify, otherwise as its own launch first
@@ -166,6 +167,8 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
     }
   }
   // one ticket per (row, kv head): fall back to the merge kernel when they do not fit
+  if (a.base_splits > 0 && ((size_t)a.n_splits * a.rows * a.n_q_heads * a.head_dim * 4 >= (1ull << 31) || a.rows > 1024)) a.n_splits = a.base_splits;
+  const int32_t wanted = a.base_splits > 0 ? a.base_splits : a.n_splits;
   const bool tickets_fit = (size_t)a.rows * (size_t)a.n_kv_heads * 4 <= kCounterBytes &&
                            (size_t)a.n_splits * a.rows * a.n_q_heads * a.head_dim * 4 < (1ull << 31);
   a.counters = (use_mfma && tickets_fit && (a.fold_group > 0 || bsgl::knob(bsgl::kKnobNoFusedMerge) == 0)) ? counters : nullptr;
@@ -177,7 +180,7 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   a.balance_target_hi = 0;
   a.whole_len = 0;
   if (a.counters != nullptr && a.n_splits > 1 && a.rows <= 1024 && a.kv.table_cols <= (1 << 20) && !uniform_splits && bsgl::knob(bsgl::kKnobDecodeBalance) != 0)
-    a.balance_target = (a.n_splits + 1) / 2;
+    a.balance_target = (wanted + 1) / 2;
   if (a.balance_target > 0) {
     // Small batches get many splits, but pieces much shorter than 256 tokens cost more in the merge
     // than they gain (a piece can be shared by up to four waves instead): no more pieces than
@@ -195,7 +198,7 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
     // slower that way at 3000 - 4095 tokens.)
     if (a.rows > 2 && (int64_t)a.rows * a.n_kv_heads <= 16) {
       const int64_t fine = a.kv.table_cols / 256;
-      const int64_t hi = fine < (a.n_splits + 1) / 2 ? fine : (a.n_splits + 1) / 2;
+      const int64_t hi = fine < (wanted + 1) / 2 ? fine : (wanted + 1) / 2;
       if (hi > a.balance_target) a.balance_target_hi = (int32_t)hi;
     }
     // (where a piece is shared by four waves: 256 pieces or fewer, as launch_decode_mfma decides)
@@ -234,7 +237,7 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   // -- and with half as many kv heads to cut, up to n_splits pieces are wanted below that
   if (a.fold_group > 0 && a.balance_target > 0 && a.hint_waves == 0) {
     const int cap = bsgl::knob(bsgl::kKnobFoldPieces);
-    a.balance_target = a.n_splits < cap ? a.n_splits : cap;
+    a.balance_target = wanted < cap ? wanted : cap;
     a.balance_target_hi = 0;
   }
   const hipError_t e = use_mfma ? bsgl::launch_decode_mfma(a, stream) : bsgl::launch_decode_valu(a, stream);
@@ -398,6 +401,12 @@ int take_mods(bsgl::DecodeArgs& a, const bsgl_score_mods& m) {
 // never inside its ticket area, also where this call's own decode needs no workspace at all: one buffer serves
 // calls of different split counts.
 size_t scored_head_bytes(size_t decode_need) { return align_up(decode_need > kCounterBytes ? decode_need : kCounterBytes, 256); }
+// The most pieces a request of a scored call may be cut into.  n_splits is made for requests of one length; visible
+// intervals (documents, windows) make the lengths of a batch differ far more, and the longest request, cut into
+// n_splits pieces, then sets the time of the launch: 96 requests, 4 kv heads, visible lengths 1 - 4095 (mean 730):
+// 46 us with 6 pieces at most, 38 with 24.  Which requests get them is the kernel's rule (pieces of one length); batches of
+// one length are cut as before.
+int32_t scored_splits(int32_t n_splits) { return n_splits <= 1 ? n_splits : n_splits < 16 ? 4 * n_splits : 64; }
 int64_t score_row(int64_t table_cols) { return (table_cols + 15) / 16 * 16; }
 
 int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, int64_t q_row_stride,
@@ -437,6 +446,12 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
   const int f32_out = out_dtype != dtype;
   if (f32_out && (((uintptr_t)out & 15u) || (out_row_stride * 4) % 16))
     return fail(BSGL_ERR_BAD_ARG, "f32 out must be 16-byte aligned with a 16-byte-multiple row stride");
+  const int32_t asked_splits = n_splits;
+  a.base_splits = 0;
+  if (mods != nullptr && (variant & BSGL_DECODE_UNIFORM_SPLITS) == 0) {
+    a.base_splits = n_splits;
+    n_splits = scored_splits(n_splits);
+  }
   const size_t need = bsgl_decode_workspace_bytes(batch, n_q_heads, head_dim, n_splits, f32_out);
   if (static_scratch && need > 0) {
     if (need > kStaticScratchBytes)
@@ -486,7 +501,7 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
   if (mods != nullptr) {
     if (int rc = take_mods(a, *mods)) return rc;
     if (mods->token_weights != nullptr) {
-      const size_t all = bsgl_decode_scored_workspace_bytes(batch, n_q_heads, head_dim, n_splits, f32_out, table_cols, 1);
+      const size_t all = bsgl_decode_scored_workspace_bytes(batch, n_q_heads, head_dim, asked_splits, f32_out, table_cols, 1);
       if (workspace == nullptr || workspace_bytes < all || !aligned16(workspace))
         return fail(BSGL_ERR_WORKSPACE, "scored decode with token weights needs a 16-byte aligned workspace of %zu bytes (got %zu)", all, workspace ? workspace_bytes : (size_t)0);
       char* tail = (char*)workspace + scored_head_bytes(need);
@@ -525,7 +540,7 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
 
 size_t bsgl_decode_scored_workspace_bytes(int32_t batch, int32_t n_q_heads, int32_t head_dim, int32_t n_splits,
                                           int32_t out_is_f32, int64_t table_cols, int32_t with_weights) {
-  const size_t need = bsgl_decode_workspace_bytes(batch, n_q_heads, head_dim, n_splits, out_is_f32);
+  const size_t need = bsgl_decode_workspace_bytes(batch, n_q_heads, head_dim, scored_splits(n_splits), out_is_f32);
   if (!with_weights || batch <= 0 || n_q_heads <= 0 || table_cols <= 0) return need;
   const size_t rh = (size_t)batch * (size_t)n_q_heads;
   return scored_head_bytes(need) + align_up(rh * 4, 256) + rh * (size_t)score_row(table_cols) * 4;

@@ -135,15 +135,24 @@ void decode_mfma_kernel(DecodeArgs a) {
   auto len_of = [&](int i) {
     const int64_t s64 = i < a.rows ? a.seq_lens[i] : 0;
     const int64_t cap = a.kv.table_cols < (1 << 20) ? a.kv.table_cols : (1 << 20);
-    const int s = (int)(s64 < 0 ? 0 : (s64 > cap ? cap : s64));
-    if constexpr (SCORED) return i < a.rows ? visible_range(a.mods, i, s, s).y : 0;
-    return s;
+    return (int)(s64 < 0 ? 0 : (s64 > cap ? cap : s64));
+  };
+  // (scored form) the first visible position of a request, where its length is cut down to the visible ones
+  auto cut_len = [&](int i, int& s) {
+    if constexpr (SCORED) {
+      const int2 seen = visible_range(a.mods, i < a.rows ? i : 0, s, s);
+      s = i < a.rows ? seen.y : 0;
+      return seen.x;
+    } else {
+      return 0;
+    }
   };
   auto req_of = [&](int i) {
     const int64_t r64 = i < a.rows ? a.req_idx[i] : 0;
     return (int)(r64 < 0 ? 0 : (r64 >= a.kv.table_rows ? a.kv.table_rows - 1 : r64));
   };
-  int len0 = 0, req0 = 0;
+  int len0 = 0, req0 = 0, low0 = 0;
+  int row_first = 0;  // (scored form) the first position the row sees
   if (a.balance_target > 0) {
 #ifdef BSGL_CUT_KNOWN_LEN
     // timing experiment (tools/phase_cut.sh, CUTS=KNOWN_LEN=2048; only right for a batch of that one
@@ -154,6 +163,7 @@ void decode_mfma_kernel(DecodeArgs a) {
 #else
     len0 = len_of(lane);
     req0 = req_of(lane);
+    low0 = cut_len(lane, len0);
 #endif
   }
   const int lq = lane & 15;   // q head (column of S^T / row of O) or d column
@@ -212,10 +222,12 @@ void decode_mfma_kernel(DecodeArgs a) {
       n_parts = parts;
       flat_seq = len_first;
       flat_req = __builtin_amdgcn_readlane(req0, row);
+      if constexpr (SCORED) row_first = __builtin_amdgcn_readlane(low0, row);
     } else {
     int tot = 0, longest = 0;
     for (int r0 = 0; r0 < a.rows; r0 += 64) {
-      const int s = r0 == 0 ? len0 : len_of(r0 + lane);
+      int s = r0 == 0 ? len0 : len_of(r0 + lane);
+      if (SCORED && r0 != 0) cut_len(r0 + lane, s);
       tot += __builtin_amdgcn_readlane(wave_inclusive_scan<ScanAdd>(s), 63);
       longest = max(longest, __builtin_amdgcn_readlane(wave_inclusive_scan<ScanMax>(s), 63));
     }
@@ -236,7 +248,9 @@ void decode_mfma_kernel(DecodeArgs a) {
       int base = 0;
       row = -1;
       for (int r0 = 0; r0 < a.rows; r0 += 64) {
-        const int s = r0 == 0 ? len0 : len_of(r0 + lane);
+        int s = r0 == 0 ? len0 : len_of(r0 + lane);
+        int low = low0;
+        if (SCORED && r0 != 0) low = cut_len(r0 + lane, s);
         const int parts = r0 + lane >= a.rows ? 0 : s <= a.whole_len ? 1 : min(a.n_splits, max(1, small_div(s + piece_len - 1, piece_len)));
         const int incl = wave_inclusive_scan<ScanAdd>(parts);
         const int blk_total = __builtin_amdgcn_readlane(incl, 63);
@@ -249,6 +263,7 @@ void decode_mfma_kernel(DecodeArgs a) {
           n_parts = __builtin_amdgcn_readlane(parts, src);
           flat_seq = __builtin_amdgcn_readlane(s, src);
           flat_req = __builtin_amdgcn_readlane(r0 == 0 ? req0 : req_of(r0 + lane), src);
+          if constexpr (SCORED) row_first = __builtin_amdgcn_readlane(low, src);
         }
         base += blk_total;
       }
@@ -271,13 +286,6 @@ void decode_mfma_kernel(DecodeArgs a) {
   // ---- this row's token range (multiples of the tile so splits start on tiles) ----
   int64_t req;
   int seq;
-  int row_len = 0, row_first = 0;  // (scored form) the request's length, and the first position the row sees
-  if constexpr (SCORED) {
-    // (scalar loads beside the ones below: they leave together)
-    const int64_t s64 = a.seq_lens[row];
-    row_len = (int)(s64 < 0 ? 0 : (s64 > a.kv.table_cols ? a.kv.table_cols : s64));
-    row_first = visible_range(a.mods, row, row_len, row_len).x;
-  }
   if (a.balance_target > 0) {
     req = flat_req;
     seq = flat_seq;
@@ -286,7 +294,7 @@ void decode_mfma_kernel(DecodeArgs a) {
     req = req < 0 ? 0 : (req >= a.kv.table_rows ? a.kv.table_rows - 1 : req);
     const int64_t seq64 = a.seq_lens[row];
     seq = (int)(seq64 < 0 ? 0 : (seq64 > a.kv.table_cols ? a.kv.table_cols : seq64));
-    if constexpr (SCORED) seq = visible_range(a.mods, row, seq, seq).y;
+    row_first = cut_len(row, seq);
   }
   // the row's pieces are equal among themselves (a piece past the end is empty)
   int chunk = a.balance_target > 0 ? small_div(seq + n_parts - 1, n_parts) : (seq + n_parts - 1) / n_parts;  // (flat grid: seq <= 2^20)
@@ -342,7 +350,11 @@ void decode_mfma_kernel(DecodeArgs a) {
   const float scale_log2e = a.scale * kLog2e;
   ScoreShape shape[HPT];  // (scored form) one q head per lane
   float* score_dst[HPT];
+  float far = 0.f;  // distance of the first visible token
   if constexpr (SCORED) {
+    // (only the bias needs it, and no address depends on it: it travels beside the first requests)
+    const int64_t s64 = a.seq_lens[row];
+    far = (float)((int)(s64 < 0 ? 0 : (s64 > a.kv.table_cols ? a.kv.table_cols : s64)) - 1 - row_first);
 #pragma unroll
     for (int hh = 0; hh < HPT; ++hh) {
       const int h = (head0 + hh) * G + min(lq, G - 1);
@@ -453,15 +465,21 @@ void decode_mfma_kernel(DecodeArgs a) {
     for (int t = 0; t < NSTAGE - 1; ++t)
       if (wave + t * W < n_tiles) issue_tile(wave + t * W);
 
+    bool stored = false;  // (scored form) the tile before this one left a store behind
     for (int tile = wave; tile < n_tiles; tile += W) {
       const int ahead = (n_tiles - 1 - tile) / W;  // this wave's tiles after this one (capped below)
       if (ahead >= NSTAGE - 1) {
         issue_tile(tile + (NSTAGE - 1) * W);
-        dma_wait<(NSTAGE - 1) * DMA_PER_TILE>();
+        // (a score store of the tile before counts in vmcnt between this tile's requests and the next one's; operations
+        // retire in order, so it may stay out as well)
+        if (SCORED && NSTAGE == 2 && HPT == 1 && stored) dma_wait<DMA_PER_TILE + 1>();
+        else dma_wait<(NSTAGE - 1) * DMA_PER_TILE>();
       } else if (NSTAGE > 3 && ahead == 2) {
         dma_wait<2 * DMA_PER_TILE>();
       } else if (NSTAGE > 2 && ahead == 1) {
         dma_wait<1 * DMA_PER_TILE>();
+      } else if (SCORED && NSTAGE == 2 && HPT == 1 && stored) {
+        dma_wait<1>();
       } else {
         dma_wait<0>();
       }
@@ -483,18 +501,16 @@ void decode_mfma_kernel(DecodeArgs a) {
         for (int r = 0; r < 4; ++r) {
           if constexpr (SCORED) {
             const int t = blk + tile * kTile + 4 * lg + r;  // token of the visible ones
-            sv[r] = (4 * lg + r < n_valid) ? shape[hh].fast(sc[r], (float)(row_len - 1 - row_first - t)) : kNegInf;
+            sv[r] = (4 * lg + r < n_valid) ? shape[hh].fast(sc[r], far - (float)t) : kNegInf;
           } else {
             sv[r] = (4 * lg + r < n_valid) ? sc[r] * scale_log2e : kNegInf;
           }
           tmax = fmaxf(tmax, sv[r]);
         }
         if constexpr (SCORED) {
-          // the tile's finished scores, four tokens of a head per lane (a row of the buffer has room for whole
-          // tiles).  The stores count in vmcnt behind the requests of the tile after this one: the waits below
-          // then wait for more than they need, never for less.
-          if (score_dst[hh] != nullptr && lq < G)
-            *(f32x4*)(score_dst[hh] + blk + tile * kTile) = f32x4{sv[0], sv[1], sv[2], sv[3]};
+          // the tile's finished scores, four tokens of a head per lane (a row of the buffer has room for whole tiles)
+          stored = score_dst[hh] != nullptr;
+          if (stored && lq < G) *(f32x4*)(score_dst[hh] + blk + tile * kTile) = f32x4{sv[0], sv[1], sv[2], sv[3]};
         }
         tmax = quad_group_max(tmax);
         if (__any(tmax > m_run[hh])) {

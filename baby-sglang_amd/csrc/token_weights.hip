@@ -5,8 +5,9 @@
 //
 // The decode kernel leaves its scores behind (4 bytes per head and token, an eighth to a twentieth of the K/V rows it
 // reads); a second pass is needed because a weight is known only once its whole row has been summed up.  Bound
-// by those bytes, mostly from the caches they were just written to.  A thread owns four consecutive tokens and
-// sums the heads in order, so the result does not depend on the launch.
+// by those bytes, mostly from the caches they were just written to.  A workgroup owns 256 consecutive tokens: its
+// four waves take the heads in turn, four tokens per lane, and their sums are added in LDS in wave order, so
+// the result does not depend on the launch.
 //
 // Two requests of a batch may name the same row: the first of them adds up all of its namesakes, in batch
 // order, and the others leave, so that no two workgroups touch the same entry.
@@ -18,10 +19,16 @@ namespace bsgl {
 
 namespace {
 
-constexpr int kTokens = 256;  // tokens per workgroup of 64 lanes: four per lane
+typedef __attribute__((ext_vector_type(4))) float f32x4;
 
-__global__ __launch_bounds__(64) void token_weights_kernel(WeightsArgs a) {
-  const int lane = threadIdx.x;
+constexpr int kTokens = 256;  // tokens per workgroup: four per lane of a wave
+constexpr int kWaves = 4;     // that share the heads
+
+__global__ __launch_bounds__(64 * kWaves) void token_weights_kernel(WeightsArgs a) {
+  __shared__ f32x4 s_sum[kWaves][64];
+  __shared__ int s_same[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.y;
   auto req_of = [&](int i) {
     const int64_t r = a.req_idx[i];
@@ -33,44 +40,60 @@ __global__ __launch_bounds__(64) void token_weights_kernel(WeightsArgs a) {
   };
   const int64_t req = req_of(row);
   // the request's namesakes: one before it owns the row; `later`: there is one behind it
-  bool before = false, later = false;
-  for (int i0 = 0; i0 < a.rows; i0 += 64) {
-    const int i = i0 + lane;
-    const bool same = i < a.rows && i != row && req_of(min(i, a.rows - 1)) == req;
-    before |= __any(same && i < row);
-    later |= __any(same && i > row);
+  int mine = 0;  // bit 0: one before, bit 1: one behind
+  for (int i = tid; i < a.rows; i += 64 * kWaves) {
+    if (i != row && req_of(i) == req) mine |= i < row ? 1 : 2;
   }
-  if (before) return;
+  mine = (__any(mine & 1) ? 1 : 0) | (__any(mine & 2) ? 2 : 0);
   const int seq = len_of(row);
   const int2 seen = visible_range(a.mods, row, seq, seq);
   const float* src = a.mods.scores + (int64_t)row * a.n_q_heads * a.mods.score_stride;
   const float* lse = a.lse + (int64_t)row * a.n_q_heads;
-  if (!later) {
-    // (grid-stride: the grid is made for the longest request the host knows of)
-    for (int64_t t0 = (int64_t)blockIdx.x * kTokens; t0 < seen.y; t0 += (int64_t)gridDim.x * kTokens) {
-      const int t = (int)t0 + 4 * lane;
-      if (t >= seen.y) continue;
-      float w[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int h = 0; h < a.n_q_heads; ++h) {
-        // (a score row has room for whole groups of 16: the last group's tail is never used)
-        const float4 s = *(const float4*)(src + h * a.mods.score_stride + t);
+  // the wave's head sums of the first 256 tokens leave before it is known whose row this is
+  auto head_sums = [&](int64_t t0) {
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    const int t = (int)t0 + 4 * lane;
+    if (t < seen.y) {
+      // (a score row has room for whole groups of 16: the last group's tail is never used)
+#pragma unroll 4
+      for (int h = wave; h < a.n_q_heads; h += kWaves) {
+        const f32x4 s = *(const f32x4*)(src + h * a.mods.score_stride + t);
         const float l = lse[h] * kLog2e;
-        w[0] += fast_exp2(s.x - l);
-        w[1] += fast_exp2(s.y - l);
-        w[2] += fast_exp2(s.z - l);
-        w[3] += fast_exp2(s.w - l);
-      }
-      const int64_t at = req * a.row_stride + seen.x + t;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (t + k < seen.y) a.out[at + k] = a.old[at + k] + w[k];
+        for (int k = 0; k < 4; ++k) w[k] += fast_exp2(s[k] - l);
+      }
+    }
+    return w;
+  };
+  const int64_t t_first = (int64_t)blockIdx.x * kTokens;
+  if (lane == 0) s_same[wave] = mine;
+  f32x4 w = head_sums(t_first);
+  __syncthreads();
+  mine = s_same[0] | s_same[1] | s_same[2] | s_same[3];
+  if (mine & 1) return;
+  if (mine == 0) {
+    // (grid-stride: the grid is made for the longest request the host knows of)
+    for (int64_t t0 = t_first; t0 < seen.y; t0 += (int64_t)gridDim.x * kTokens) {
+      if (t0 != t_first) {
+        w = head_sums(t0);
+        __syncthreads();  // (the sums before these have been read)
+      }
+      s_sum[wave][lane] = w;
+      __syncthreads();
+      const int64_t t = t0 + tid;
+      if (t < seen.y) {
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) sum += ((const float*)s_sum[v])[tid];
+        const int64_t at = req * a.row_stride + seen.x + t;
+        a.out[at] = a.old[at] + sum;
       }
     }
     return;
   }
   // (rare) several requests on one row: column by column, every one of them that sees it
-  for (int64_t c = (int64_t)blockIdx.x * 64 + lane; c < a.table_cols; c += (int64_t)gridDim.x * 64) {
-    float w = 0.f;
+  for (int64_t c = (int64_t)blockIdx.x * kTokens + tid; c < a.table_cols; c += (int64_t)gridDim.x * kTokens) {
+    float sum = 0.f;
     bool any = false;
     for (int i = row; i < a.rows; ++i) {
       if (req_of(i) != req) continue;
@@ -80,10 +103,10 @@ __global__ __launch_bounds__(64) void token_weights_kernel(WeightsArgs a) {
       if (t < 0 || t >= r.y) continue;
       any = true;
       const float* si = a.mods.scores + (int64_t)i * a.n_q_heads * a.mods.score_stride;
-      for (int h = 0; h < a.n_q_heads; ++h) w += fast_exp2(si[h * a.mods.score_stride + t] - a.lse[(int64_t)i * a.n_q_heads + h] * kLog2e);
+      for (int h = 0; h < a.n_q_heads; ++h) sum += fast_exp2(si[h * a.mods.score_stride + t] - a.lse[(int64_t)i * a.n_q_heads + h] * kLog2e);
     }
     const int64_t at = req * a.row_stride + c;
-    if (any) a.out[at] = a.old[at] + w;
+    if (any) a.out[at] = a.old[at] + sum;
   }
 }
 
@@ -94,7 +117,7 @@ hipError_t launch_token_weights(const WeightsArgs& a, hipStream_t stream) {
   const int64_t longest = a.len_hint > 0 && a.len_hint < a.table_cols ? a.len_hint : a.table_cols;
   const int64_t blocks = (longest + kTokens - 1) / kTokens;
   const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)a.rows);
-  hipLaunchKernelGGL(token_weights_kernel, grid, dim3(64), 0, stream, a);
+  hipLaunchKernelGGL(token_weights_kernel, grid, dim3(64 * kWaves), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -283,8 +283,10 @@ typedef struct bsgl_score_mods {
 
 /*
  * bsgl_paged_decode (arguments, checks and KV write as there) with scored attention; the row's own
- * position is seq_lens[i] - 1.  `call->workspace` holds bsgl_decode_scored_workspace_bytes bytes: the decode
- * workspace of the same n_splits (the same contract for its tickets), followed, when token weights are asked for, by the
+ * position is seq_lens[i] - 1.  n_splits counts as for requests of one length: a request that sees far more
+ * than the others may be cut into up to four times as many pieces (64 at most; 1 stays 1, and so does any number with
+ * BSGL_DECODE_UNIFORM_SPLITS).  `call->workspace` holds bsgl_decode_scored_workspace_bytes bytes: the decode
+ * workspace of that many splits (the same contract for its tickets), followed, when token weights are asked for, by the
  * log-sum-exps and finished scores [batch, n_q_heads, table_cols] that the second launch reads.
  */
 size_t bsgl_decode_scored_workspace_bytes(int32_t batch, int32_t n_q_heads, int32_t head_dim, int32_t n_splits,

@@ -44,7 +44,7 @@ def test_scored_decode_refusals():
 
 
 def test_scored_decode_workspace():
-    plain = _hip.decode_workspace_bytes(4, 12, 128, 8)
+    plain = _hip.decode_workspace_bytes(4, 12, 128, 32)  # (up to four times the splits for a long request)
     assert _hip.decode_scored_workspace_bytes(4, 12, 128, 8, 1000, False) == plain
     with_weights = _hip.decode_scored_workspace_bytes(4, 12, 128, 8, 1000, True)
     assert with_weights >= plain + 4 * 12 * (1 + 1008) * 4
