@@ -288,7 +288,12 @@ struct EvictArgs {
   int32_t recent;
   int32_t sinks;
   int32_t longest;  // longest request the host knows of (table_cols if it knows none); shapes the launch only
+  void* workspace;  // of evict_workspace() bytes for table_cols columns
+  // set by launch_evict
+  int32_t slices;
+  int64_t counts_at, staged_at, staged_row;
 };
+size_t evict_workspace(int64_t batch, int64_t longest, int32_t budget, int64_t* counts_at, int64_t* staged_at, int64_t* staged_row);
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 
 struct LogitArgs {

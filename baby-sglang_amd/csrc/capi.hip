@@ -829,8 +829,7 @@ int bsgl_merge_attn_states(void* out, int64_t out_row_stride, float* lse_out, co
 }
 
 size_t bsgl_evict_workspace_bytes(int32_t batch, int64_t table_cols, int32_t budget) {
-  (void)batch; (void)table_cols; (void)budget;
-  return 0;
+  return budget < 1 ? 0 : bsgl::evict_workspace(batch, table_cols, budget, nullptr, nullptr, nullptr);
 }
 
 int bsgl_evict_tokens(int32_t* out_table, float* out_weights, const int32_t* req_to_token, int64_t table_row_stride,
@@ -838,7 +837,6 @@ int bsgl_evict_tokens(int32_t* out_table, float* out_weights, const int32_t* req
                       const int64_t* req_pool_indices, const int64_t* seq_lens, int64_t* new_lens, int32_t* evicted,
                       int64_t evicted_row_stride, int32_t evicted_cols, int32_t batch, int32_t budget, int32_t recent,
                       int32_t sinks, int32_t max_seq_len, void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace; (void)workspace_bytes;
   if (batch < 0) return fail(BSGL_ERR_BAD_ARG, "batch < 0");
   if (budget < 1 || recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget)
     return fail(BSGL_ERR_BAD_ARG, "budget %d must be positive and hold the %d sinks and %d recent tokens", budget, sinks, recent);
@@ -850,6 +848,11 @@ int bsgl_evict_tokens(int32_t* out_table, float* out_weights, const int32_t* req
     return fail(BSGL_ERR_BAD_ARG, "a row stride is shorter than the page table's column count");
   if (evicted_cols < 0 || (evicted != nullptr && evicted_row_stride < evicted_cols))
     return fail(BSGL_ERR_BAD_ARG, "evicted row stride shorter than its column count");
+  if (batch > 65535) return fail(BSGL_ERR_UNSUPPORTED, "batch %d above 65535", batch);
+  const size_t need = bsgl_evict_workspace_bytes(batch, table_cols, budget);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    return fail(BSGL_ERR_WORKSPACE, "eviction from rows of %lld columns needs a 16-byte aligned workspace of %zu bytes (got %zu)",
+                (long long)table_cols, need, workspace ? workspace_bytes : (size_t)0);
   bsgl::EvictArgs a{};
   a.out_table = out_table;
   a.out_weights = out_weights;
@@ -869,6 +872,7 @@ int bsgl_evict_tokens(int32_t* out_table, float* out_weights, const int32_t* req
   a.budget = budget;
   a.recent = recent;
   a.sinks = sinks;
+  a.workspace = workspace;
   a.longest = (int32_t)(max_seq_len > 0 && max_seq_len < table_cols ? max_seq_len : table_cols);
   const hipError_t e = bsgl::launch_evict(a, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail("evict launch", e);
