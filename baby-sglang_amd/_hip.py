@@ -284,11 +284,19 @@ def _launch(device_index: int, fn, *args) -> int:
         return fn(*args, current_stream_handle(device_index))
 
 
+def _same_gpu(index: int, *tensors: torch.Tensor) -> None:
+    """Every tensor on GPU ``index``: the CPU raises as everywhere in this package, another GPU is a bad argument."""
+    for t in tensors:
+        if t.get_device() != index:
+            _need_gpu(t)
+            raise ValueError(f"the tensors of a call must be on one GPU: got {t.device} beside cuda:{index}")
+
+
 def _check_out(out: torch.Tensor, rows: int, width: int, dtype: torch.dtype) -> int:
     """The row stride of a result tensor of the wanted kind."""
     row, col = out.stride() if out.dim() == 2 else (0, 0)
-    if out.shape != (rows, width) or out.dtype != dtype or (width > 1 and col != 1) or (rows > 1 and row < width) or not out.is_cuda:
-        raise ValueError(f"out must be {dtype} [{rows}, {width}] with dense rows on the GPU, got {out.dtype} {tuple(out.shape)}")
+    if out.shape != (rows, width) or out.dtype != dtype or (width > 1 and col != 1) or (rows > 1 and row < width):
+        raise ValueError(f"out must be {dtype} [{rows}, {width}] with dense rows, got {out.dtype} {tuple(out.shape)}")
     return row if rows > 1 else width
 
 
@@ -315,15 +323,15 @@ def _check_table(req_to_token: torch.Tensor):
 def _check_weights(t: torch.Tensor, table_shape, cols: int) -> int:
     """The row stride of a table of token weights."""
     stride = t.stride()
-    if t.dtype != torch.float32 or t.shape != table_shape or stride[1] != 1 or stride[0] < cols or not t.is_cuda:
-        raise ValueError(f"token weights must be float32 of the page table's shape {tuple(table_shape)} with dense rows on the GPU")
+    if t.dtype != torch.float32 or t.shape != table_shape or stride[1] != 1 or stride[0] < cols:
+        raise ValueError(f"token weights must be float32 of the page table's shape {tuple(table_shape)} with dense rows")
     return stride[0]
 
 
 def _index_rows(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     """A dense int64 vector of ``n`` entries on the GPU."""
-    if t.shape != (n,) or not t.is_cuda:
-        raise ValueError(f"{name} must have shape ({n},) on the GPU, got {tuple(t.shape)} on {t.device}")
+    if t.shape != (n,):
+        raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
     if t.dtype != torch.int64:
         t = t.to(torch.int64)
     return t if t.is_contiguous() else t.contiguous()
@@ -522,7 +530,7 @@ def paged_decode(
 # ---- scored attention ---------------------------------------------------------------------------
 
 
-def _score_mods(rows: int, n_q_heads: int, device, logit_cap, slopes, visible_from, visible_to):
+def _score_mods(rows: int, n_q_heads: int, index: int, logit_cap, slopes, visible_from, visible_to):
     """The checked parts of a ``bsgl_score_mods`` as numbers, ``(cap, slopes, from, to)``, and the tensors
     behind the pointers (the caller keeps them until the call has been made)."""
     cap = float(logit_cap) if logit_cap else 0.0
@@ -531,16 +539,18 @@ def _score_mods(rows: int, n_q_heads: int, device, logit_cap, slopes, visible_fr
     keep = []
     ptr = [0, 0, 0]
     if slopes is not None:
-        if slopes.dtype != torch.float32 or slopes.shape != (n_q_heads,) or slopes.device != device:
-            raise ValueError(f"slopes must be float32 of shape ({n_q_heads},) on {device}, got {slopes.dtype} {tuple(slopes.shape)} on {slopes.device}")
+        _same_gpu(index, slopes)
+        if slopes.dtype != torch.float32 or slopes.shape != (n_q_heads,):
+            raise ValueError(f"slopes must be float32 of shape ({n_q_heads},), got {slopes.dtype} {tuple(slopes.shape)}")
         slopes = slopes if slopes.is_contiguous() else slopes.contiguous()
         keep.append(slopes)
         ptr[0] = slopes.data_ptr()
     for at, t in ((1, visible_from), (2, visible_to)):
         if t is None:
             continue
-        if t.dtype not in (torch.int32, torch.int64) or t.shape != (rows,) or t.device != device:
-            raise ValueError(f"visible_from / visible_to must be int32 of shape ({rows},) on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        _same_gpu(index, t)
+        if t.dtype not in (torch.int32, torch.int64) or t.shape != (rows,):
+            raise ValueError(f"visible_from / visible_to must be int32 of shape ({rows},), got {t.dtype} {tuple(t.shape)}")
         if t.dtype == torch.int64:  # (positions fit 32 bits; what does not stays outside the sequence either way)
             t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
         t = t if t.is_contiguous() else t.contiguous()
@@ -594,7 +604,9 @@ def paged_decode_scored(
     ``decode_scored_workspace_bytes``; like every decode workspace it must have been created zero-filled.
     The other arguments are ``paged_decode``'s.
     """
-    _need_gpu(q, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens)
+    index = q.get_device()
+    _need_gpu(q)
+    _same_gpu(index, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens)
     q, q_shape, q_stride = _rows3(q)
     if len(q_shape) != 3:
         raise ValueError(f"q must be [batch, heads, dim], got shape {tuple(q_shape)}")
@@ -607,6 +619,8 @@ def paged_decode_scored(
         out_dtype = out.dtype if out is not None else q_dtype
     if out is None:
         out = torch.empty((batch, hq * dim), dtype=out_dtype, device=device)
+    else:
+        _same_gpu(index, out)
     out_stride = _check_out(out, batch, hq * dim, out_dtype)
     if batch == 0:
         return out
@@ -619,19 +633,23 @@ def paged_decode_scored(
         scale = 1.0 / math.sqrt(dim)
     if n_splits is None:
         n_splits = decode_num_splits(batch, hkv, cols)
-    mods, keep = _score_mods(batch, hq, device, logit_cap, slopes, visible_from, visible_to)
+    mods, keep = _score_mods(batch, hq, index, logit_cap, slopes, visible_from, visible_to)
     weights = (0, 0, 0)
     if token_weights is not None:
+        _same_gpu(index, token_weights)
         w_stride = _check_weights(token_weights, req_to_token.shape, cols)
         if token_weights_out is None:
             token_weights_out = token_weights
-        elif _check_weights(token_weights_out, req_to_token.shape, cols) != w_stride:
+        else:
+            _same_gpu(index, token_weights_out)
+        if _check_weights(token_weights_out, req_to_token.shape, cols) != w_stride:
             raise ValueError("token_weights and token_weights_out must share a row stride")
         weights = (token_weights.data_ptr(), token_weights_out.data_ptr(), w_stride)
     elif token_weights_out is not None:
         raise ValueError("token_weights_out without token_weights")
     lse_ptr = 0
     if lse is not None:
+        _same_gpu(index, lse)
         if lse.dtype != torch.float32 or lse.shape != (batch, hq) or not lse.is_contiguous():
             raise ValueError(f"lse must be dense float32 [{batch}, {hq}]")
         lse_ptr = lse.data_ptr()
@@ -639,6 +657,7 @@ def paged_decode_scored(
     ws_ptr = ws_bytes = 0
     if need:
         if workspace is not None:
+            _same_gpu(index, workspace)
             ws_bytes = workspace.numel() * workspace.element_size()
         if ws_bytes < need:
             workspace = new_decode_workspace(need, device)
@@ -648,6 +667,7 @@ def paged_decode_scored(
     if k_new is not None or v_new is not None or out_cache_loc is not None:
         if k_new is None or v_new is None or out_cache_loc is None:
             raise ValueError("k_new, v_new and out_cache_loc go together")
+        _same_gpu(index, k_new, v_new, out_cache_loc)
         k_new, kn_shape, kn_stride = _rows3(k_new.view(batch, hkv, dim) if k_new.dim() == 2 else k_new)
         v_new, vn_shape, vn_stride = _rows3(v_new.view(batch, hkv, dim) if v_new.dim() == 2 else v_new)
         if k_new.dtype != q_dtype or v_new.dtype != q_dtype:
@@ -671,7 +691,7 @@ def paged_decode_scored(
             _PACK_MODS.pack(*mods, *weights),
         )  # fmt: skip
 
-    rc = _launch(device.index, call)
+    rc = _launch(index, call)
     if rc:
         _check(rc, "bsgl_paged_decode_scored")
     return out
@@ -706,7 +726,12 @@ def evict_tokens(
     The page-table and weight rows are compacted in place, or into ``out_table`` / ``out_weights`` (same shape
     and strides).  ``evicted`` may be given with any width; by default it has room for every slot that can go
     (``max_seq_len``, 0 = the table's width, less the budget)."""
-    _need_gpu(req_to_token, token_weights, req_pool_indices, seq_lens)
+    index = req_to_token.get_device()
+    _need_gpu(req_to_token)
+    _same_gpu(index, token_weights, req_pool_indices, seq_lens)
+    for t in (out_table, out_weights, evicted, new_lens, workspace):
+        if t is not None:
+            _same_gpu(index, t)
     n_rows, cols, stride = _check_table(req_to_token)
     shape, device = req_to_token.shape, req_to_token.device
     batch = req_pool_indices.shape[0]
@@ -715,7 +740,7 @@ def evict_tokens(
     w_stride = _check_weights(token_weights, shape, cols)
     if out_table is None:
         out_table = req_to_token
-    elif out_table.dtype != torch.int32 or out_table.shape != shape or out_table.stride() != req_to_token.stride() or not out_table.is_cuda:
+    elif out_table.dtype != torch.int32 or out_table.shape != shape or out_table.stride() != req_to_token.stride():
         raise ValueError("out_table must have the page table's type, shape and strides")
     if out_weights is None:
         out_weights = token_weights
@@ -723,14 +748,14 @@ def evict_tokens(
         raise ValueError("out_weights must have the token weights' strides")
     if new_lens is None:
         new_lens = torch.empty(batch, dtype=torch.int64, device=device)
-    elif new_lens.dtype != torch.int64 or new_lens.shape != (batch,) or not new_lens.is_contiguous() or not new_lens.is_cuda:
-        raise ValueError(f"new_lens must be a dense int64 vector of {batch} entries on the GPU")
+    elif new_lens.dtype != torch.int64 or new_lens.shape != (batch,) or not new_lens.is_contiguous():
+        raise ValueError(f"new_lens must be a dense int64 vector of {batch} entries")
     if evicted is None:
         longest = min(int(max_seq_len), cols) if max_seq_len > 0 else cols
         evicted = torch.empty((batch, max(0, longest - budget)), dtype=torch.int32, device=device)
-    elif evicted.dtype != torch.int32 or evicted.dim() != 2 or evicted.shape[0] != batch or not evicted.is_cuda \
+    elif evicted.dtype != torch.int32 or evicted.dim() != 2 or evicted.shape[0] != batch \
             or (evicted.shape[1] > 1 and evicted.stride(1) != 1):
-        raise ValueError("evicted must be int32 [batch, width] with dense rows on the GPU")
+        raise ValueError("evicted must be int32 [batch, width] with dense rows")
     width = evicted.shape[1]
     need = lib.bsgl_evict_workspace_bytes(batch, cols, budget)
     ws_ptr = ws_bytes = 0
@@ -742,7 +767,7 @@ def evict_tokens(
             ws_bytes = need
         ws_ptr = workspace.data_ptr()
     rc = _launch(
-        device.index, lib.bsgl_evict_tokens, out_table.data_ptr(), out_weights.data_ptr(), req_to_token.data_ptr(), stride,
+        index, lib.bsgl_evict_tokens, out_table.data_ptr(), out_weights.data_ptr(), req_to_token.data_ptr(), stride,
         token_weights.data_ptr(), w_stride, n_rows, cols, req_pool_indices.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(),
         evicted.data_ptr() if width else None, max(evicted.stride(0), width), width, batch, budget, recent, sinks, int(max_seq_len), ws_ptr, ws_bytes)
     if rc:
@@ -777,6 +802,7 @@ def logit_controls(
     [batch] or one number).  ``bias_ids`` / ``bias_values`` [batch, n] (int32, float32; ids outside the
     vocabulary are unused places).  ``token_mask`` int32 [rows, ceil(vocab / 32)], bit t % 32 of word t / 32 set =
     token t allowed; ``mask_rows`` int32 [batch] (default i; negative = no mask)."""
+    index = logits.get_device()
     _need_gpu(logits)
     shape, stride = logits.shape, logits.stride()
     if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1) or (shape[0] > 1 and stride[0] < shape[1]):
@@ -786,30 +812,36 @@ def logit_controls(
     code = _dtype_code(logits)
     if out is None:
         out = torch.empty((batch, vocab), dtype=logits.dtype, device=device)
+    else:
+        _same_gpu(index, out)
     out_stride = _check_out(out, batch, vocab, logits.dtype)
-    keep = []
+    keep = []  # what was made here and has to outlive the call
+    want = (batch,)
 
     def vector(t, dtypes, name):  # the address of a [batch] vector of one of the types, as the first of them
         if t is None:
             return 0
-        if t.dtype not in dtypes or t.shape != (batch,) or t.device != device:
-            raise ValueError(f"{name} must be {dtypes[0]} of shape ({batch},) on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if t.dtype != dtypes[0]:
-            t = t.to(dtypes[0])
-        if not t.is_contiguous():
-            t = t.contiguous()
-        keep.append(t)
+        if t.get_device() != index:
+            _same_gpu(index, t)
+        if t.dtype != dtypes[0] or t.shape != want or not t.is_contiguous():
+            if t.dtype not in dtypes or t.shape != want:
+                raise ValueError(f"{name} must be {dtypes[0]} of shape ({batch},), got {t.dtype} {tuple(t.shape)}")
+            t = t.to(dtypes[0]).contiguous()
+            keep.append(t)
         return t.data_ptr()
 
     def floats(t, name):
         if t is not None and not isinstance(t, torch.Tensor):
-            t = torch.full((batch,), float(t), dtype=torch.float32, device=device)
+            t = torch.full(want, float(t), dtype=torch.float32, device=device)
+            keep.append(t)
         return vector(t, (torch.float32,), name)
 
     def table(t, dtype, name):  # (address, row stride, rows, columns) of a 2-D table with dense rows
         sh, st = t.shape, t.stride()
-        if t.dtype != dtype or len(sh) != 2 or (sh[1] > 1 and st[1] != 1) or (sh[0] > 1 and st[0] < sh[1]) or t.device != device:
-            raise ValueError(f"{name} must be a 2-D {dtype} tensor with dense rows on {device}")
+        if t.dtype != dtype or len(sh) != 2 or (sh[1] > 1 and st[1] != 1) or (sh[0] > 1 and st[0] < sh[1]):
+            raise ValueError(f"{name} must be a 2-D {dtype} tensor with dense rows")
+        if t.get_device() != index:
+            _same_gpu(index, t)
         return t.data_ptr(), st[0] if sh[0] > 1 else sh[1], sh[0], sh[1]
 
     long, int_ = (torch.int64, torch.int32), (torch.int32, torch.int64)
@@ -848,7 +880,7 @@ def logit_controls(
         return lib.bsgl_logit_controls(_PACK_LOGITS.pack(
             out.data_ptr(), logits.data_ptr(), out_stride, stride[0] if batch > 1 else vocab, *past, *bias, *mask, n_bias, batch, vocab, code, stream))
 
-    rc = _launch(device.index, call)
+    rc = _launch(index, call)
     if rc:
         _check(rc, "bsgl_logit_controls")
     return out
@@ -933,7 +965,9 @@ def paged_prefill_scored(
     interval as in ``paged_decode_scored``, the interval (int32 [T]) per row of q in positions of its
     request; the default sees everything up to the row's own position.  Rows behind the last request's are left as
     they were."""
-    _need_gpu(q, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens, prefix_lens, extended_lens)
+    index = q.get_device()
+    _need_gpu(q)
+    _same_gpu(index, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens, prefix_lens, extended_lens)
     q, q_shape, q_stride = _rows3(q)
     if len(q_shape) != 3:
         raise ValueError(f"q must be [tokens, heads, dim], got shape {tuple(q_shape)}")
@@ -942,6 +976,8 @@ def paged_prefill_scored(
     batch = req_pool_indices.shape[0]
     if out is None:
         out = torch.empty((total_q, hq * dim), dtype=q.dtype, device=device)
+    else:
+        _same_gpu(index, out)
     out_stride = _check_out(out, total_q, hq * dim, q.dtype)
     if total_q == 0 or batch == 0:
         return out
@@ -953,16 +989,19 @@ def paged_prefill_scored(
     extended_lens = _index_rows(extended_lens, batch, "extended_lens")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    mods, keep = _score_mods(total_q, hq, device, logit_cap, slopes, visible_from, visible_to)
+    mods, keep = _score_mods(total_q, hq, index, logit_cap, slopes, visible_from, visible_to)
     need = lib.bsgl_prefill_workspace_bytes(batch, total_q, hq, dim)
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    ws_bytes = 0
+    if workspace is not None:
+        _same_gpu(index, workspace)
+        ws_bytes = workspace.numel() * workspace.element_size()
     if ws_bytes < need:
         if list_ready:
             raise ValueError("list_ready needs the workspace that holds the list")
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
         ws_bytes = need
     rc = _launch(
-        device.index, lib.bsgl_paged_prefill_scored, out.data_ptr(), out_stride, q.data_ptr(), q_stride[0],
+        index, lib.bsgl_paged_prefill_scored, out.data_ptr(), out_stride, q.data_ptr(), q_stride[0],
         k_slab.data_ptr(), v_slab.data_ptr(), slab_stride, slots, req_to_token.data_ptr(), table_stride, rows, cols,
         req_pool_indices.data_ptr(), seq_lens.data_ptr(), prefix_lens.data_ptr(), extended_lens.data_ptr(),
         batch, total_q, hq, hkv, dim, scale, _dtype_code(q), variant | (PREFILL_LIST_READY if list_ready else 0),

@@ -296,6 +296,8 @@ struct EvictArgs {
 size_t evict_workspace(int64_t batch, int64_t longest, int32_t budget, int64_t* counts_at, int64_t* staged_at, int64_t* staged_row);
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 
+constexpr int kLogitMaxBias = 1 << 12;           // biases per request
+constexpr int kLogitMaxHistory = (1 << 18) - 1;  // tokens of a history row that are looked at
 struct LogitArgs {
   void* out;  // may be `logits`
   const void* logits;

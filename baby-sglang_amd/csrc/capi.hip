@@ -890,7 +890,7 @@ int bsgl_logit_controls(const bsgl_logit_call* c) {
   if (c->out_row_stride < c->vocab || c->logits_row_stride < c->vocab) return fail(BSGL_ERR_BAD_ARG, "logit row stride shorter than the vocabulary");
   if (c->history != nullptr) {
     if (!c->history_lens) return fail(BSGL_ERR_BAD_ARG, "history without history_lens");
-    if (c->history_n_rows <= 0 || c->history_cols < 0 || c->history_cols > 0x7fffffff - 4096 || c->history_row_stride < c->history_cols)
+    if (c->history_n_rows <= 0 || c->history_cols < 0 || c->history_row_stride < c->history_cols)
       return fail(BSGL_ERR_BAD_ARG, "history extents must be positive, its row stride at least its column count");
     if (c->history_rows == nullptr && c->history_n_rows < c->batch) return fail(BSGL_ERR_BAD_ARG, "history has fewer rows than the batch");
   } else if (c->repetition || c->presence || c->frequency) {
@@ -898,6 +898,10 @@ int bsgl_logit_controls(const bsgl_logit_call* c) {
   }
   if (c->n_bias > 0 && (!c->bias_ids || !c->bias_values || c->bias_row_stride < c->n_bias))
     return fail(BSGL_ERR_BAD_ARG, "bias_ids and bias_values go together, with a row stride of at least n_bias");
+  if (c->n_bias > bsgl::kLogitMaxBias)
+    return fail(BSGL_ERR_UNSUPPORTED, "%d biases per request, up to %d are taken (a dense bias is an addition)", c->n_bias, bsgl::kLogitMaxBias);
+  if (c->history != nullptr && c->history_cols > bsgl::kLogitMaxHistory)
+    return fail(BSGL_ERR_UNSUPPORTED, "history of %lld columns, up to %d are taken", (long long)c->history_cols, bsgl::kLogitMaxHistory);
   if (c->token_mask != nullptr && (c->mask_n_rows <= 0 || c->mask_row_stride < ((int64_t)c->vocab + 31) / 32))
     return fail(BSGL_ERR_BAD_ARG, "token mask rows are shorter than the vocabulary's bits");
   bsgl::LogitArgs a{};
@@ -922,7 +926,7 @@ int bsgl_logit_controls(const bsgl_logit_call* c) {
   a.mask_row_stride = c->mask_row_stride;
   a.mask_n_rows = c->mask_n_rows;
   a.mask_rows = c->mask_rows;
-  a.n_bias = c->n_bias;
+  a.n_bias = a.bias_ids != nullptr ? c->n_bias : 0;
   a.batch = c->batch;
   a.vocab = c->vocab;
   a.dtype = c->dtype;

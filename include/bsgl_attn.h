@@ -325,7 +325,8 @@ int bsgl_evict_tokens(int32_t* out_table /*device*/, float* out_weights /*device
  *   token mask:                               x = -inf where bit (t % 32) of word (t / 32) is 0
  * The history is a table of token ids parallel to the page table: request i's are the first history_lens[i] entries
  * of row history_rows[i] (NULL: row i), the first prompt_lens[i] (NULL: 0) of them its prompt.  Ids outside the vocabulary are ignored,
- * in biases too (padding).  mask_rows[i] (NULL: i) outside [0, mask_n_rows) = no mask.  A mask without any bit
+ * in biases too (padding); up to 4096 biases and a history of up to
+ * 262143 tokens per request (BSGL_ERR_UNSUPPORTED beyond).  mask_rows[i] (NULL: i) outside [0, mask_n_rows) = no mask.  A mask without any bit
  * leaves a row of -inf.  Everything but logits and out may be NULL; out may be logits.  repetition, presence, frequency: fp32
  * [batch], repetition > 0.
  */

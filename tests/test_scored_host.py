@@ -78,6 +78,8 @@ def test_logit_refusals():
                dict(hist, history_lens=None), dict(hist, history_n_rows=1), dict(hist, history_n_rows=0), dict(hist, history_row_stride=9),
                dict(token_mask=256, mask_n_rows=2, mask_row_stride=3), dict(token_mask=256, mask_n_rows=0, mask_row_stride=4)):
         assert f(**kw) == _hip.BSGL_ERR_BAD_ARG, kw
+    assert f(history=256, history_row_stride=1 << 18, history_n_rows=2, history_cols=1 << 18, history_lens=256) == _hip.BSGL_ERR_UNSUPPORTED
+    assert f(n_bias=4097, bias_ids=256, bias_values=256, bias_row_stride=4097) == _hip.BSGL_ERR_UNSUPPORTED
     assert f(dtype=5) == _hip.BSGL_ERR_UNSUPPORTED and f(batch=65536) == _hip.BSGL_ERR_UNSUPPORTED
     assert f(batch=0, out=None) == _hip.BSGL_OK and f(vocab=0, out=None) == _hip.BSGL_OK
     assert lib.bsgl_logit_controls(None) == _hip.BSGL_ERR_BAD_ARG
