@@ -59,7 +59,8 @@ struct ScoreMods {
   const float* slopes;   // [n_q_heads], NULL: none
   const int32_t* from;   // [rows], NULL: 0
   const int32_t* to;     // [rows], NULL: the row's own position + 1
-  // generic extend path: {page-table row, request length, own position, 0} of every extend token (NULL: decode,
+  // extend tokens as rows of a decode kernel: {page-table row, request length, own position, 1} of every one, all zero for
+  // a row of q that no request owns, which is not written (NULL: decode,
   // whose rows are the requests and whose own position is the last)
   const int4* rows;
   // decode: the finished scores in units of log2, [rows, n_q_heads, score_stride], token t of the VISIBLE ones
@@ -152,6 +153,7 @@ struct MergeArgs {
   int32_t n_heads;
   int32_t head_dim;
   int32_t dtype;
+  const int4* owned = nullptr;  // ScoreMods::rows: rows whose last word is 0 are not written
 };
 
 struct ScatterArgs {
@@ -182,7 +184,9 @@ struct ExpandArgs {
   int32_t grp_blocks;  // blocks per group (0 counts as 1)
   int64_t* row_req;  // [total_q_tokens]; may be NULL (then only the running sums are made)
   int64_t* row_len;  // [total_q_tokens]
-  int4* rows4;       // instead of row_req / row_len, for the scored form: {page-table row, request length, own position, 0}
+  int4* rows4;       // instead of row_req / row_len, for the scored form: {page-table row, request length, own position, 1}
+  uint32_t* clear;   // words to be set to zero on the way (tickets), or NULL; not with row_req
+  int32_t n_clear;
 };
 
 // extend attention over blocks of 16 query positions (matrix-core kernel)

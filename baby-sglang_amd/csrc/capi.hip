@@ -612,6 +612,8 @@ size_t bsgl_prefill_workspace_bytes(int32_t batch, int32_t total_q_tokens, int32
   return bytes;
 }
 
+static constexpr int64_t kFewTokens = 32768;
+
 static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
                          const void* k_slab, const void* v_slab, int64_t slab_row_stride, int64_t n_slots,
                          const int32_t* req_to_token, int64_t table_row_stride, int64_t table_rows,
@@ -725,7 +727,13 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   }
   const bool mfma_ok = supported(pa, &why);
   if (kind == BSGL_DECODE_MFMA && !mfma_ok) return fail(BSGL_ERR_UNSUPPORTED, "matrix-core extend: %s", why);
-  if (kind != BSGL_DECODE_VALU && mfma_ok) {
+  // A few tokens (scored form): as rows of the decode kernel, which cuts every row over the machine.  The extend kernel gives
+  // a request's block one workgroup, 0.65 us per 32 tokens of its prefix whatever the block holds; as rows every token
+  // streams the prefix again, from L2 at some 6 TB/s.  Per token of prefix that is 20 ns against
+  // total_q_tokens * 4 n_kv_heads head_dim / 6e12 s, equal at total_q_tokens * n_kv_heads * head_dim = 32768.
+  // FEW_NOTE
+  const bool few = mods != nullptr && kind == BSGL_DECODE_AUTO && mfma_ok && (int64_t)total_q_tokens * n_kv_heads * head_dim <= kFewTokens;
+  if (kind != BSGL_DECODE_VALU && mfma_ok && !few) {
     ex.row_req = nullptr;  // only the running sums are needed
     hipError_t e = hipSuccess;
     if ((variant & BSGL_PREFILL_LIST_READY) == 0) {  // (else: an earlier call for this batch left them in the workspace)
@@ -742,6 +750,11 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
     a.scored = true;
     a.mods = scored.mods;
     a.mods.rows = ex.rows4;
+    if (few) {
+      // (the decode kernel's tickets, at the head of the workspace's tail)
+      ex.clear = (uint32_t*)ws;
+      ex.n_clear = total_q_tokens * n_kv_heads;
+    }
   }
   hipError_t e = bsgl::launch_prefill_expand(ex, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail("prefill expand launch", e);
@@ -766,7 +779,8 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   const size_t rh = (size_t)total_q_tokens * (size_t)n_q_heads;
   const size_t cb = kCounterBytes;
   a.ws_o = (float*)(ws + cb);
-  a.ws_lse = splits > 1 ? (float*)(ws + cb + align_up((size_t)splits * rh * (size_t)head_dim * 4, 256)) : nullptr;
+  a.ws_lse = splits > 1 ? (float*)(ws + cb + align_up((size_t)splits * rh * partial_row_width(head_dim) * 4, 256)) : nullptr;
+  if (few) return run_decode(a, BSGL_DECODE_AUTO, splits > 1 ? (uint32_t*)ws : nullptr, (hipStream_t)stream);
   return run_decode(a, BSGL_DECODE_VALU, nullptr, (hipStream_t)stream);
 }
 

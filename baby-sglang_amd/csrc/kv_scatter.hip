@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256) void kv_scatter_kernel(ScatterArgs a) {
 // exclusive running sums of extended_lens and of the block groups of each request,
 // ceil(ceil(extended_lens / blk_rows) / grp_blocks)  (negative lengths count as 0, lengths above
 // the number of q rows as that number)
-__global__ void prefill_cu_kernel(ExpandArgs a) {
+__device__ __forceinline__ void running_sums(const ExpandArgs& a) {
   __shared__ int64_t s_ext[256], s_blk[256];
   const int tid = threadIdx.x;
   const int per = (a.batch + 255) / 256;
@@ -79,9 +79,10 @@ __global__ void prefill_cu_kernel(ExpandArgs a) {
   }
 }
 
-__global__ __launch_bounds__(256) void prefill_rows_kernel(ExpandArgs a) {
-  const int t = blockIdx.x * blockDim.x + threadIdx.x;
-  if (t >= a.total_q_tokens) return;
+__global__ void prefill_cu_kernel(ExpandArgs a) { running_sums(a); }
+
+// what the decode kernels have to know about extend token t
+__device__ __forceinline__ void expand_row(const ExpandArgs& a, int t) {
   // last request i with cu_ext[i] <= t
   int lo = 0, hi = a.batch;  // invariant: cu_ext[lo] <= t (cu_ext[0] == 0), answer in [lo, hi)
   while (hi - lo > 1) {
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(256) void prefill_rows_kernel(ExpandArgs a) {
       auto i32 = [](int64_t x) { return (int)max((int64_t)0, min(x, (int64_t)0x7fffffff)); };
       const int64_t full = max((int64_t)0, a.seq_lens[lo]);
       const int64_t prefix = max((int64_t)0, min(a.prefix_lens[lo], full));
-      r4 = make_int4(i32(a.req_pool_indices[lo]), i32(full), i32(prefix + (t - a.cu_ext[lo])), 0);
+      r4 = make_int4(i32(a.req_pool_indices[lo]), i32(full), i32(prefix + (t - a.cu_ext[lo])), 1);
     }
     a.rows4[t] = r4;
     return;
@@ -115,6 +116,21 @@ __global__ __launch_bounds__(256) void prefill_rows_kernel(ExpandArgs a) {
   a.row_len[t] = len;
 }
 
+__global__ __launch_bounds__(256) void prefill_rows_kernel(ExpandArgs a) {
+  const int t = blockIdx.x * blockDim.x + threadIdx.x;
+  if (t >= a.total_q_tokens) return;
+  expand_row(a, t);
+}
+
+// A few extend tokens that run as rows of the decode kernel: sums, rows and zeroed tickets in one workgroup.
+__global__ __launch_bounds__(256) void prefill_few_kernel(ExpandArgs a) {
+  for (int i = threadIdx.x; i < a.n_clear; i += 256) a.clear[i] = 0;
+  running_sums(a);
+  __threadfence_block();
+  __syncthreads();
+  for (int t = threadIdx.x; t < a.total_q_tokens; t += 256) expand_row(a, t);
+}
+
 }  // namespace
 
 hipError_t launch_kv_scatter(const ScatterArgs& a, hipStream_t stream) {
@@ -125,6 +141,10 @@ hipError_t launch_kv_scatter(const ScatterArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_prefill_expand(const ExpandArgs& a, hipStream_t stream) {
+  if (a.clear != nullptr) {
+    hipLaunchKernelGGL(prefill_few_kernel, dim3(1), dim3(256), 0, stream, a);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL(prefill_cu_kernel, dim3(1), dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.total_q_tokens == 0 || (a.row_req == nullptr && a.rows4 == nullptr)) return e;

@@ -132,15 +132,20 @@ void decode_mfma_kernel(DecodeArgs a) {
   int flat_req = -1, flat_seq = 0;  // the row's page-table row and length, when found by the flat search
   // flat grid: lane i's request length and page-table row, requested first so that the
   // lane-only arithmetic below runs while they travel
+  const int32_t* const rows4 = SCORED ? (const int32_t*)a.mods.rows : nullptr;  // (scored form) four words per row, or NULL
   auto len_of = [&](int i) {
-    const int64_t s64 = i < a.rows ? a.seq_lens[i] : 0;
+    int64_t s64 = 0;
+    if (i < a.rows) s64 = SCORED && rows4 != nullptr ? (int64_t)rows4[4 * i + 1] : a.seq_lens[i];
     const int64_t cap = a.kv.table_cols < (1 << 20) ? a.kv.table_cols : (1 << 20);
     return (int)(s64 < 0 ? 0 : (s64 > cap ? cap : s64));
   };
   // (scored form) the first visible position of a request, where its length is cut down to the visible ones
   auto cut_len = [&](int i, int& s) {
     if constexpr (SCORED) {
-      const int2 seen = visible_range(a.mods, i < a.rows ? i : 0, s, s);
+      const int j = i < a.rows ? i : 0;
+      int to = s;
+      if (rows4 != nullptr) to = min(s, rows4[4 * j + 2] + 1);
+      const int2 seen = visible_range(a.mods, j, s, to);
       s = i < a.rows ? seen.y : 0;
       return seen.x;
     } else {
@@ -148,7 +153,8 @@ void decode_mfma_kernel(DecodeArgs a) {
     }
   };
   auto req_of = [&](int i) {
-    const int64_t r64 = i < a.rows ? a.req_idx[i] : 0;
+    int64_t r64 = 0;
+    if (i < a.rows) r64 = SCORED && rows4 != nullptr ? (int64_t)rows4[4 * i] : a.req_idx[i];
     return (int)(r64 < 0 ? 0 : (r64 >= a.kv.table_rows ? a.kv.table_rows - 1 : r64));
   };
   int len0 = 0, req0 = 0, low0 = 0;
@@ -290,9 +296,10 @@ void decode_mfma_kernel(DecodeArgs a) {
     req = flat_req;
     seq = flat_seq;
   } else {
-    req = a.req_idx[row];
+    const bool listed = SCORED && rows4 != nullptr;
+    req = listed ? (int64_t)rows4[4 * row] : a.req_idx[row];
     req = req < 0 ? 0 : (req >= a.kv.table_rows ? a.kv.table_rows - 1 : req);
-    const int64_t seq64 = a.seq_lens[row];
+    const int64_t seq64 = listed ? (int64_t)rows4[4 * row + 1] : a.seq_lens[row];
     seq = (int)(seq64 < 0 ? 0 : (seq64 > a.kv.table_cols ? a.kv.table_cols : seq64));
     row_first = cut_len(row, seq);
   }
@@ -353,8 +360,15 @@ void decode_mfma_kernel(DecodeArgs a) {
   float far = 0.f;  // distance of the first visible token
   if constexpr (SCORED) {
     // (only the bias needs it, and no address depends on it: it travels beside the first requests)
-    const int64_t s64 = a.seq_lens[row];
-    far = (float)((int)(s64 < 0 ? 0 : (s64 > a.kv.table_cols ? a.kv.table_cols : s64)) - 1 - row_first);
+    int pos;
+    if (rows4 != nullptr) {
+      if (rows4[4 * row + 3] == 0) return;  // (all of the row's pieces: no ticket is drawn)
+      pos = rows4[4 * row + 2];
+    } else {
+      const int64_t s64 = a.seq_lens[row];
+      pos = (int)(s64 < 0 ? 0 : (s64 > a.kv.table_cols ? a.kv.table_cols : s64)) - 1;
+    }
+    far = (float)(pos - row_first);
 #pragma unroll
     for (int hh = 0; hh < HPT; ++hh) {
       const int h = (head0 + hh) * G + min(lq, G - 1);
@@ -501,7 +515,7 @@ void decode_mfma_kernel(DecodeArgs a) {
         for (int r = 0; r < 4; ++r) {
           if constexpr (SCORED) {
             const int t = blk + tile * kTile + 4 * lg + r;  // token of the visible ones
-            sv[r] = (4 * lg + r < n_valid) ? shape[hh].fast(sc[r], far - (float)t) : kNegInf;
+            sv[r] = (4 * lg + r < n_valid) ? shape[hh].fast(sc[r], fabsf(far - (float)t)) : kNegInf;
           } else {
             sv[r] = (4 * lg + r < n_valid) ? sc[r] * scale_log2e : kNegInf;
           }
@@ -697,7 +711,9 @@ void decode_mfma_kernel(DecodeArgs a) {
   // The weights: lane (head k of a load, part p) = P2 * k + p holds lse and weight of its (head,
   // part), P2 = 8 lanes per head for up to 8 parts (64 otherwise), so one
   // load instruction fetches 64 / P2 heads' values and the maxima and sums run inside P2 lanes.
-  auto merge_rows = [&](auto pair_c, auto p2_c) {
+  // (inlined whatever the compiler makes of their size: a call would put the whole argument block on the stack, and every wave of
+  // the launch, merging or not, then runs twice as long)
+  auto merge_rows = [&](auto pair_c, auto p2_c) __attribute__((always_inline)) {
     constexpr int PAIR = decltype(pair_c)::value;
     constexpr int P2 = decltype(p2_c)::value;
     constexpr int HPI = 64 / P2;  // heads per lse load
@@ -792,7 +808,7 @@ void decode_mfma_kernel(DecodeArgs a) {
       }
     }
   };
-  auto merge_p2 = [&](auto pair_c) {
+  auto merge_p2 = [&](auto pair_c) __attribute__((always_inline)) {
     // (16 lanes per head for 9 - 16 parts was measured too: slower than one head per load)
     if (n_parts <= 8) merge_rows(pair_c, std::integral_constant<int, 8>{});
     else merge_rows(pair_c, std::integral_constant<int, 64>{});
@@ -924,6 +940,7 @@ hipError_t launch_decode_mfma(const DecodeArgs& a_in, hipStream_t stream) {
   mg.n_heads = a.n_q_heads;
   mg.head_dim = a.head_dim;
   mg.dtype = a.out_dtype;
+  if (a.scored) mg.owned = a.mods.rows;
   return launch_merge(mg, stream);
 }
 

@@ -57,6 +57,7 @@ __global__ __launch_bounds__(kThreads) void decode_valu_kernel(DecodeArgs a, int
   int pos = 0, first = 0;  // (scored form) the row's own position, and the first one it sees
   if (SCORED && a.mods.rows != nullptr) {
     const int4 r4 = a.mods.rows[row];
+    if (r4.w == 0) return;
     req = r4.x;
     seq64 = r4.y;
     pos = r4.z;
@@ -267,6 +268,7 @@ __global__ __launch_bounds__(256) void merge_states_kernel(MergeArgs a) {
   const int64_t n_rh = (int64_t)a.rows * a.n_heads;
   const int64_t rh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (rh >= n_rh) return;
+  if (a.owned != nullptr && a.owned[rh / a.n_heads].w == 0) return;
   const float my_lse = lane < a.n_parts ? a.parts_lse[(int64_t)lane * n_rh + rh] : kNegInf;
   const float mx = group_max<64>(my_lse);
   const float my_w = (my_lse == kNegInf) ? 0.f : fast_exp2((my_lse - mx) * kLog2e);
@@ -403,6 +405,7 @@ hipError_t launch_decode_valu(const DecodeArgs& a, hipStream_t stream) {
   mg.n_heads = a.n_q_heads;
   mg.head_dim = a.head_dim;
   mg.dtype = a.out_dtype;
+  if (a.scored) mg.owned = a.mods.rows;
   return launch_merge(mg, stream);
 }
 

@@ -8,13 +8,18 @@
 //
 //   * a finished score is kept as u with t = A u + C, t the score in units of log2 and C one number per lane
 //     and step, so that the exponent's multiply-add takes in the rest:
-//       plain        u = scale log2 e q.k                      A = 1                C = 0
-//       cap          u = 1 / (2^{2 s / cap} + 1)               A = -2 cap log2 e    C = cap log2 e
-//       bias         u = scale log2 e q.k + slope row          A = 1                C = slope (first token - i)
-//       cap and bias u = -2 cap log2 e / (..) + slope row      A = 1                C = both
-//     (tanh(x) = 1 - 2 / (e^{2x} + 1); `row` is the token's place in the step).  A cap costs 24 issue cycles a score
-//     -- multiply, exp2, add, reciprocal -- beside the 20 of the plain softmax: this kernel is bound by vector
-//     issue where the plain one is bound by both pipes.
+//       plain        u = scale log2 e q.k             A = 1               C = 0
+//       cap          u = 1 / (2^{2 s / cap} + 1)      A = -2 cap log2 e   C = cap log2 e
+//       bias         u = q.k - (slope / A) row        A = scale log2 e    C = slope (step's first - i)
+//       cap and bias u = 1 / (..) - (slope / A) row   A = -2 cap log2 e   C = both
+//     (tanh(x) = 1 - 2 / (e^{2x} + 1); `row` is the token's place in the step, a literal of the multiply-add: as
+//     slope x row in registers the bias cost 200 us of a 780 us launch, sixteen registers too many).  A cap costs 24 issue
+//     cycles a score -- multiply, exp2, add, reciprocal -- beside the 20 of the plain softmax: this kernel is bound by
+//     vector issue where the plain one is bound by both pipes.
+//   * the tokens are streamed from the last one back (the page-table entries are staged in that order, nothing else
+//     changes): a bias makes the nearest tokens the largest, so going forward a steep slope raises the running maximum in
+//     every step, and every step then rescales the output (48 x 512 over 1536, 28 / 4 heads: 983 us forward, 768 back; without a
+//     bias there is no difference).
 //   * the workgroup streams the tokens from the first that any of its rows sees to the last: a document mask
 //     skips what lies before the document, a prefix mask reaches past the diagonal.  Steps that every row of
 //     a wave sees whole take no mask.
@@ -53,6 +58,12 @@ template <> struct Mma32<f16_tag> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
   }
 };
+
+// Capped scores need no running maximum where the cap itself keeps their exponentials in range: |t| <= cap log2 e, so
+// with the reference fixed at 0 a probability lies in 2^+-87 for a cap of 60, a sum of 2^18 of them times values of up to
+// 2^20 below 2^127, and the smallest row sum is normal; bf16 has the same exponents.  (f16 has not, and a bias has no
+// bound.)  It saves the maxima and the checks of every step.
+constexpr float kFixedCap = 60.f;
 
 // row of the 32x32 accumulator that register r of a lane in half `hi` holds
 __device__ __forceinline__ constexpr int acc_row(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
@@ -104,8 +115,9 @@ __device__ __forceinline__ void rescue_row(const PrefillArgs& a, int64_t q_row, 
 // workgroup).  16: for batches of short extends a wave's columns are 2 q heads x 16 positions and
 // the workgroup covers 16 positions x 8 q heads, so a kv head's K/V is streamed by ONE workgroup
 // for up to 8 q heads instead of once per pair of heads.
-// CAP, BIAS: which of the two the call has (see the head of this file).
-template <typename Tag, int PW, bool CAP, bool BIAS>
+// CAP, BIAS: which of the two the call has (see the head of this file).  FIXED (a cap, no bias, bf16): the softmax's reference is 0
+// throughout -- see kFixedCap.
+template <typename Tag, int PW, bool CAP, bool BIAS, bool FIXED = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void prefill_scored_kernel(PrefillArgs a) {
   using E = Elem<Tag>;
@@ -180,7 +192,6 @@ void prefill_scored_kernel(PrefillArgs a) {
   // one's) instead of leaving half their waves without work, and every second one of them retires.
   const bool two_blocks = PW == 32 && n_rt == 1;
   if (two_blocks && (bi & 1)) return;
-  const int q0_wg = (bg0 + nb - 1 - bi) * ROWS;
   const int hw = PW == 32 ? wave >> 1 : wave * CH;  // first of this wave's q heads among the workgroup's (or its block)
   const int my_bi = bi + (two_blocks ? hw : 0);
   const bool head_ok = two_blocks ? my_bi < nb : hw < n_rt;  // no such head / block: the wave only helps to load
@@ -228,14 +239,19 @@ void prefill_scored_kernel(PrefillArgs a) {
     last = max(last, __builtin_amdgcn_readfirstlane(s_rng[w].y));
   }
   if (last == 0) first = 0;  // nobody sees anything
-  // everything below counts tokens from `first`
+  // Everything below counts tokens in the order they are streamed, from the last one back (see the head of this
+  // file): place t is position last - 1 - t.
   const int kv_len = last - first;
-  const int wave_len = rng.y > 0 ? rng.y - first : 0;
-  full_from -= first;
-  full_to = min(full_to - first, kv_len);
-  const int my_lo = seen.x - first, my_hi = live ? my_lo + seen.y : 0x7fffffff;
-  const int my_pos = own - first;
-  const int ahead_from = BIAS ? prefix + q0 - first : 0;  // tokens behind this one stand ahead of some row of the wave
+  const int wave_len = rng.y > 0 ? last - rng.x : 0;
+  {
+    const int f = full_from;
+    full_from = last - min(full_to, last);
+    full_to = last - max(f, first);
+  }
+  const int my_lo = last - (seen.x + seen.y);
+  const int my_hi = live ? my_lo + seen.y : 0x7fffffff;
+  const int my_pos = last - 1 - own;
+  const int wave_pos = last - 1 - (prefix + q0);  // places before this one stand ahead of some row of the wave
   const int32_t* table_row = a.kv.table + req * a.kv.table_row_stride + first;
   const uint32_t max_slot = (uint32_t)(a.kv.n_slots - 1);
   const uint32_t row_units = (uint32_t)(a.kv.slab_row_stride * 2 / 16);
@@ -262,19 +278,21 @@ void prefill_scored_kernel(PrefillArgs a) {
   const float arg = CAP ? 2.f * scale_log2e / a.mods.cap : 0.f;
   const float top2 = CAP ? a.mods.cap * kLog2e : 0.f;
   const float slope = BIAS ? a.mods.slopes[min(head, a.n_q_heads - 1)] * kLog2e : 0.f;
-  const float A = CAP && !BIAS ? -2.f * top2 : 1.f;
+  const float A = CAP ? -2.f * top2 : BIAS ? scale_log2e : 1.f;
+  const float slope_u = BIAS ? slope / A : 0.f;
   // raw score of register r -> u (see the head of this file)
   auto shape = [&](float raw, int r) {
-    float u = CAP ? raw : raw * scale_log2e;
+    float u = raw;
     if constexpr (CAP) u = __builtin_amdgcn_rcpf(fast_exp2(raw * arg) + 1.f);
-    if constexpr (BIAS) u = fmaf(CAP ? u : raw, CAP ? -2.f * top2 : scale_log2e, slope * (float)acc_row(r, 0));
+    if constexpr (BIAS) u = fmaf(-slope_u, (float)acc_row(r, 0), u);
+    if constexpr (!CAP && !BIAS) u *= scale_log2e;
     return u;
   };
-  constexpr bool FLIP = CAP && !BIAS;  // A is negative: the largest score has the smallest u
+  constexpr bool FLIP = CAP;  // A is negative: the largest score has the smallest u
   constexpr float kHidden = FLIP ? -kNegInf : kNegInf;
   // the part of a score that the step and the lane decide
   auto step_c = [&](int step) {
-    return CAP && !BIAS ? top2 : BIAS ? fmaf(slope, (float)(step * STEP + 4 * hi - my_pos), top2) : 0.f;
+    return BIAS ? fmaf(-slope, (float)(step * STEP + 4 * hi - my_pos), top2) : CAP ? top2 : 0.f;
   };
   auto ext3 = [](float x, float y, float z) { return FLIP ? min3(x, y, z) : max3(x, y, z); };
 
@@ -322,7 +340,9 @@ void prefill_scored_kernel(PrefillArgs a) {
   // s_slots; block b + 1 is fetched while block b is being worked on, so the K/V stream never
   // drains between blocks.  Each thread fetches two entries of a block.
   const int n_steps = (kv_len + STEP - 1) / STEP;
-  auto entry_ptr = [&](int e) { return table_row + max(min(e, kv_len - 1), 0); };  // entries past the end repeat the last one
+  auto entry_ptr = [&](int e) {  // the entry of place e; places past the end repeat the last one
+    return table_row + max(kv_len - 1 - max(e, 0), 0);
+  };
   auto entry_off = [&](uint32_t s) { return (int32_t)((s > max_slot ? max_slot : s) * row_units); };
   {
     uint32_t e[EPT];
@@ -495,7 +515,7 @@ void prefill_scored_kernel(PrefillArgs a) {
       load_k(kf, smem + NEXT * STEP_BYTES);
 
       const bool hides = step * STEP < full_from || step * STEP + STEP > full_to;  // wave-uniform
-      const bool looks_ahead = BIAS && step * STEP + STEP - 1 > ahead_from;
+      const bool looks_ahead = BIAS && step * STEP < wave_pos;
       const float c_step = step_c(step);
       float ext = ext_nx;
       if (__builtin_expect(hides || looks_ahead, 0)) {  // (rare: the ends of the rows' intervals, and prefixes read both ways)
@@ -505,13 +525,13 @@ void prefill_scored_kernel(PrefillArgs a) {
         for (int r = 0; r < 16; ++r) {
           const int t = t0m + acc_row(r, 0);
           // (the bias above is slope * (j - i), which is what is wanted up to the row's own position)
-          if constexpr (BIAS) sc[r] = fmaf(-2.f * slope, (float)max(t - my_pos, 0), sc[r]);
+          if constexpr (BIAS) sc[r] = fmaf(-2.f * slope_u, (float)max(my_pos - t, 0), sc[r]);
           sc[r] = (t >= my_lo && t < my_hi) ? sc[r] : kHidden;
         }
-        ext = ext16(sc);
+        if (!FIXED) ext = ext16(sc);
       }
       const float lmax = fmaf(ext, A, c_step);
-      if (__builtin_expect(__any(lmax > m_run + kSlack), 0)) {  // (rare after the first steps)
+      if (!FIXED && __builtin_expect(__any(lmax > m_run + kSlack), 0)) {  // (rare after the first steps)
         float x = lmax, y = lmax;
         swap32(x, y);  // the partner lane holds the position's other 16 tokens
         const float m_new = max3(m_run, x, y);
@@ -529,7 +549,7 @@ void prefill_scored_kernel(PrefillArgs a) {
           for (int db = 0; db < 4; ++db) o_acc[db][r] *= ar;
         }
       }
-      const float c0 = c_step - m_sub;
+      const float c0 = FIXED ? c_step : c_step - m_sub;
 
       // ---- from here to the end of the step: one basic block, issued in the order written ----
       // (a scheduling barrier after every product: the compiler's own order puts the vector
@@ -579,12 +599,12 @@ void prefill_scored_kernel(PrefillArgs a) {
         if (i >= 2) {
 #pragma unroll
           for (int r = 3 * (i - 2); r < (i == 7 ? 16 : 3 * (i - 1)); ++r) sn[r] = shape(sn[r], r);
-          mx0 = ext3(mx0, sn[3 * (i - 2)], sn[3 * (i - 2) + 1]);
-          mx1 = i == 7 ? ext3(mx1, sn[14], sn[15]) : ext3(mx1, sn[3 * (i - 2) + 2], sn[3 * (i - 2) + 2]);
+          if (!FIXED) mx0 = ext3(mx0, sn[3 * (i - 2)], sn[3 * (i - 2) + 1]);
+          if (!FIXED) mx1 = i == 7 ? ext3(mx1, sn[14], sn[15]) : ext3(mx1, sn[3 * (i - 2) + 2], sn[3 * (i - 2) + 2]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      ext_nx = ext3(mx0, mx1, mx1);
+      if (!FIXED) ext_nx = ext3(mx0, mx1, mx1);
       __builtin_amdgcn_s_setprio(0);
     };
     static_assert(NSTAGE == 4, "the step loop below is unrolled over the ring");
@@ -651,6 +671,8 @@ template <typename Tag, int PW>
 void launch_shape(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
   const bool cap = a.mods.cap > 0.f, bias = a.mods.slopes != nullptr;
   if (cap && bias) hipLaunchKernelGGL((prefill_scored_kernel<Tag, PW, true, true>), grid, dim3(256), 0, stream, a);
+  else if (std::is_same<Tag, bf16_tag>::value && cap && a.mods.cap <= kFixedCap)
+    hipLaunchKernelGGL((prefill_scored_kernel<bf16_tag, PW, true, false, true>), grid, dim3(256), 0, stream, a);
   else if (cap) hipLaunchKernelGGL((prefill_scored_kernel<Tag, PW, true, false>), grid, dim3(256), 0, stream, a);
   else if (bias) hipLaunchKernelGGL((prefill_scored_kernel<Tag, PW, false, true>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((prefill_scored_kernel<Tag, PW, false, false>), grid, dim3(256), 0, stream, a);
@@ -660,6 +682,11 @@ void launch_shape(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
 
 // the extend kernels' conditions, with up to 16 q heads per kv head (a workgroup takes them two or eight at a time)
 bool prefill_scored_supported(const PrefillArgs& a, const char** why) {
+  // (without a cap the largest score is taken to be the largest product)
+  if (!(a.mods.cap > 0.f) && !(a.scale > 0.f)) {
+    *why = "the matrix-core kernel needs a positive scale";
+    return false;
+  }
   PrefillArgs b = a;
   if (a.n_kv_heads > 0 && a.n_q_heads % a.n_kv_heads == 0 && a.n_q_heads / a.n_kv_heads <= 16) b.n_q_heads = a.n_kv_heads;
   return prefill_mfma_supported(b, why);

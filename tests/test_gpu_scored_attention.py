@@ -420,6 +420,22 @@ def test_extend_launch_forms(gpu, kw):
     extend_case(gpu, "7b", torch.bfloat16, [65, 100, 7], [513, 0, 64], cap=30.0, kind="document", seed=23, only=50, **kw)
 
 
+@pytest.mark.parametrize("heads,dtype", [("7b", torch.bfloat16), ("0.5b", torch.float16), ("d64", torch.bfloat16), ("1.5b", torch.float32), ("one", torch.float16),
+                                         ("mha", torch.bfloat16)])
+@pytest.mark.parametrize("ext,prefix,kind", [([1], [0], None), ([1], [2500], None), ([3, 0, 2], [700, 9, 0], "both"), ([7, 11], [1300, 40], "document"),
+                                             ([5, 9, 20], [0, 600, 33], "wild"), ([8], [4000], "prefix")])
+def test_extend_a_few_tokens(gpu, heads, dtype, ext, prefix, kind):
+    """So few new tokens that they run as rows of the decode kernel; rows that no request owns stay as they were."""
+    if heads == "one" and dtype == torch.float32:
+        pytest.skip("f32 kernels take up to 8 q heads per kv head")
+    extend_case(gpu, heads, dtype, ext, prefix, cap=20.0, slopes=True, kind=kind, seed=36, extra_rows=3)
+
+
+@pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("0.5b", torch.bfloat16), ("7b", torch.float32)])
+def test_extend_unowned_rows(gpu, heads, dtype):
+    extend_case(gpu, heads, dtype, [150, 130], [0, 30], cap=20.0, seed=37, extra_rows=70, only=40)
+
+
 def test_extend_long(gpu):
     """Several blocks of page-table entries, many steps; ring and entry staging wrap."""
     extend_case(gpu, "one", torch.bfloat16, [700, 64], [2100, 1500], cap=20.0, slopes=True, seed=24, only=24)
@@ -455,6 +471,19 @@ def test_extend_scale_of_any_sign(gpu, scale):
                                         scale=scale, logit_cap=cap)
         want, mass, lse, _, top = orc.scored_exact(c["q"], c["k"], c["v"], c["table"][c["req"]], [100], [0] * 100, range(100), scale, cap)
         check_rows(out, want, mass, lse, top.abs(), cap, torch.bfloat16, torch.bfloat16, 2.0**-8, 100, 6.0, 128)
+
+
+@pytest.mark.parametrize("cap", [60.0, 61.0, 100.0])
+@pytest.mark.parametrize("side", [-1.0, 1.0])
+def test_extend_scores_at_the_cap(gpu, cap, side):
+    """Every visible score at one end of the cap's range, for some rows: the exponentials' range is the cap's (bf16 takes a
+    fixed reference up to 60); the others see ordinary scores."""
+    def poison(c, row_req, row_pos, st, sp):
+        c["k"][:] = c["k"].abs()  # so that a row of one sign has scores of one sign
+        c["q"][::2] = (c["q"][::2].abs() * 40.0 * side).to(c["q"].dtype)
+
+    extend_case(gpu, "1.5b", torch.bfloat16, [90, 33], [0, 70], cap=cap, seed=34, poison=poison)
+    extend_case(gpu, "1.5b", torch.bfloat16, [9, 3], [0, 70], cap=cap, slopes=True, seed=35, poison=poison)
 
 
 @pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("0.5b", torch.float16), ("7b", torch.float32)])
