@@ -154,6 +154,7 @@ struct MergeArgs {
   int32_t head_dim;
   int32_t dtype;
   const int4* owned = nullptr;  // ScoreMods::rows: rows whose last word is 0 are not written
+  const int64_t* row_end = nullptr;  // rows from *row_end on are not written
 };
 
 struct ScatterArgs {
@@ -215,6 +216,11 @@ struct PrefillArgs {
   float scale;
   int32_t dtype;
   ScoreMods mods;  // scored form only; from / to are per row of q
+  // scored form: every block's stream is cut into this many pieces, whose fp32 results go to parts_o [splits,
+  // total_q_tokens * n_q_heads, head_dim] and parts_lse and are merged by a launch of their own (0 or 1: not cut)
+  int32_t splits;
+  float* parts_o;
+  float* parts_lse;
 };
 
 inline bool decode_direct_out(const DecodeArgs& a) { return a.n_splits == 1 && a.out_dtype == a.dtype; }

@@ -612,7 +612,15 @@ size_t bsgl_prefill_workspace_bytes(int32_t batch, int32_t total_q_tokens, int32
   return bytes;
 }
 
-static constexpr int64_t kFewTokens = 32768;
+static constexpr int64_t kFewTokens = 32768;          // tokens * n_kv_heads * head_dim (at most 512 tokens: the ticket area holds them)
+static constexpr int64_t kFewStreamed = (int64_t)1 << 25;  // ... * page-table columns
+
+// at most this many workgroups of the scored extend kernel have work (>= 1)
+static int64_t scored_workgroups(int64_t blk_rows, int64_t tokens, int64_t batch, int64_t n_q_heads, int64_t n_kv_heads) {
+  const int64_t hpw = blk_rows == 64 ? 2 : 8, group = n_q_heads / n_kv_heads;
+  const int64_t blocks = (tokens + blk_rows - 1) / blk_rows + (batch < tokens ? batch : tokens) - 1;
+  return blocks * n_kv_heads * ((group + hpw - 1) / hpw);
+}
 
 static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
                          const void* k_slab, const void* v_slab, int64_t slab_row_stride, int64_t n_slots,
@@ -692,7 +700,9 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
     const int64_t per = (int64_t)pa.blk_rows * (batch > 0 ? batch : 1);
     const int64_t mean_blocks = ((int64_t)total_q_tokens + per - 1) / per;
     int grp = 1;
-    while (grp < 8 && grp < mean_blocks) grp *= 2;
+    // (scored form, launches that do not fill the machine: a group would put them on one of the eight XCDs)
+    const bool spread = mods != nullptr && scored_workgroups(pa.blk_rows, total_q_tokens, batch, n_q_heads, n_kv_heads) <= 512;
+    while (!spread && grp < 8 && grp < mean_blocks) grp *= 2;
     const int forced = bsgl::knob(bsgl::kKnobPrefillGroup);  // tuning override
     pa.grp_blocks = forced > 0 ? forced : grp;
   }
@@ -727,14 +737,30 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   }
   const bool mfma_ok = supported(pa, &why);
   if (kind == BSGL_DECODE_MFMA && !mfma_ok) return fail(BSGL_ERR_UNSUPPORTED, "matrix-core extend: %s", why);
-  // A few tokens (scored form): as rows of the decode kernel, which cuts every row over the machine.  The extend kernel gives
-  // a request's block one workgroup, 0.65 us per 32 tokens of its prefix whatever the block holds; as rows every token
-  // streams the prefix again, from L2 at some 6 TB/s.  Per token of prefix that is 20 ns against
-  // total_q_tokens * 4 n_kv_heads head_dim / 6e12 s, equal at total_q_tokens * n_kv_heads * head_dim = 32768.
-  // FEW_NOTE
-  const bool few = mods != nullptr && kind == BSGL_DECODE_AUTO && mfma_ok && (int64_t)total_q_tokens * n_kv_heads * head_dim <= kFewTokens;
+  // A few tokens (scored form): as rows of the decode kernel, which spreads every row over the machine and needs no
+  // second launch to merge; every token then streams its request's K/V again, from L2 at some 6 TB/s.  So it pays where
+  // tokens x row bytes x length is small; the length is not known here, the page table's width bounds it.  Measured
+  // against the extend kernel: 16 x 8 tokens over 500 20.8 / 22.6 us, 4 x 16 over 2000 (3.3e7 below) 24.8 / 29.9,
+  // 8 x 8 over 1000 (3.3e7) 30.6 / 33.2, 1 x 100 over 2000 (5.4e7) 48 / 28, 16 x 4 over 8192 (1.3e8) 80 / 39.
+  const int64_t streamed = (int64_t)total_q_tokens * n_kv_heads * head_dim;
+  const bool few = mods != nullptr && kind == BSGL_DECODE_AUTO && mfma_ok && streamed <= kFewTokens && streamed * table_cols <= kFewStreamed;
   if (kind != BSGL_DECODE_VALU && mfma_ok && !few) {
     ex.row_req = nullptr;  // only the running sums are needed
+    if (mods != nullptr) {
+      // Scored form: two workgroups fit a CU.  With room for more than twice the blocks there are at most, every
+      // block's stream is cut, into as many pieces as the workspace holds partial rows for (1024 rows or so) and none
+      // shorter than 512 tokens of the widest request the page table allows.  512 tokens over 8192, 12 / 2 heads: 190 us in one piece,
+      // 116 in two; 64 over 8192 195 and 31 (8 pieces); where there is nothing to stream the merge costs 2 - 4 us (200 over 200: 21).
+      int64_t s = 512 / scored_workgroups(pa.blk_rows, total_q_tokens, batch, pa.n_q_heads, pa.n_kv_heads);
+      const int64_t room = prefill_row_splits(total_q_tokens, 1 << 30), by_len = table_cols / 512;
+      if (s > room) s = room;
+      if (s > by_len) s = by_len;
+      if (s > 1) {
+        pa.splits = (int32_t)s;
+        pa.parts_o = (float*)(ws + kCounterBytes);
+        pa.parts_lse = (float*)(ws + kCounterBytes + align_up((size_t)room * total_q_tokens * n_q_heads * partial_row_width(head_dim) * 4, 256));
+      }
+    }
     hipError_t e = hipSuccess;
     if ((variant & BSGL_PREFILL_LIST_READY) == 0) {  // (else: an earlier call for this batch left them in the workspace)
       e = bsgl::launch_prefill_expand(ex, (hipStream_t)stream);

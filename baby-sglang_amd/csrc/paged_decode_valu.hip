@@ -268,6 +268,7 @@ __global__ __launch_bounds__(256) void merge_states_kernel(MergeArgs a) {
   const int64_t n_rh = (int64_t)a.rows * a.n_heads;
   const int64_t rh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (rh >= n_rh) return;
+  if (a.row_end != nullptr && rh / a.n_heads >= *a.row_end) return;
   if (a.owned != nullptr && a.owned[rh / a.n_heads].w == 0) return;
   const float my_lse = lane < a.n_parts ? a.parts_lse[(int64_t)lane * n_rh + rh] : kNegInf;
   const float mx = group_max<64>(my_lse);

@@ -23,6 +23,8 @@
 //   * the workgroup streams the tokens from the first that any of its rows sees to the last: a document mask
 //     skips what lies before the document, a prefix mask reaches past the diagonal.  Steps that every row of
 //     a wave sees whole take no mask.
+//   * where a launch has far fewer workgroups than the machine takes (one long request, say), every block's stream is cut into pieces
+//     (PrefillArgs::splits) whose normalised fp32 results a second launch merges.
 //   * rows that see nothing are left out of the ranges and written as zeros.
 //   * 0 * NaN: a token that one row must not see can share a step with a row that sees it, and P . V multiplies its
 //     values by an exact zero.  Where such a token holds NaN or an infinity the product is NaN; rows that come out NaN
@@ -74,7 +76,7 @@ __device__ __forceinline__ float min3(float a, float b, float c) { return fminf(
 // One query row of one head by itself, from the tokens [lo, hi) it sees: the wave's lanes hold two values of the
 // head each.  Slow, and only ever run for rows that came out NaN.
 template <typename Tag>
-__device__ __forceinline__ void rescue_row(const PrefillArgs& a, int64_t q_row, int head, int kvh, int64_t req, int pos, int lo, int hi) {
+__device__ __forceinline__ void rescue_row(const PrefillArgs& a, int64_t q_row, int head, int kvh, int64_t req, int pos, int lo, int hi, int split) {
   using E = Elem<Tag>;
   const int lane = threadIdx.x & 63;
   const bool on = a.fold_group == 0 || lane < 32;
@@ -108,6 +110,12 @@ __device__ __forceinline__ void rescue_row(const PrefillArgs& a, int64_t q_row, 
     o[1] = o[1] * alpha + p * v[1];
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (a.splits > 1) {
+    const int64_t part = ((int64_t)split * a.total_q_tokens + q_row) * a.n_q_heads + head;
+    if (on) *(float2*)(a.parts_o + part * dim + 2 * lane) = make_float2(o[0] * inv, o[1] * inv);
+    if (lane == 0) a.parts_lse[part] = l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    return;
+  }
   if (on) *(uint32_t*)((char*)a.out + (q_row * a.out_row_stride + (int64_t)head * dim + 2 * lane) * 2) = E::pack2(o[0] * inv, o[1] * inv);
 }
 
@@ -164,7 +172,8 @@ void prefill_scored_kernel(PrefillArgs a) {
   const int n_z = (G + HPW - 1) / HPW;
   const int per_group = a.grp_blocks * n_z;
   const unsigned slot = blockIdx.x >> 3;
-  const int64_t g = (int64_t)(slot / (unsigned)per_group) * 8 + (blockIdx.x & 7);
+  // (the pieces of a block's stream share nothing: each on the next XCD)
+  const int64_t g = (int64_t)(slot / (unsigned)per_group) * 8 + ((blockIdx.x + 8 - (blockIdx.y & 7)) & 7);
   if (g >= a.cu_blk[a.batch] * a.n_kv_heads) return;
   const int within = (int)(slot % (unsigned)per_group);
   const int kvh = (int)(g % a.n_kv_heads);
@@ -239,6 +248,14 @@ void prefill_scored_kernel(PrefillArgs a) {
     last = max(last, __builtin_amdgcn_readfirstlane(s_rng[w].y));
   }
   if (last == 0) first = 0;  // nobody sees anything
+  if (a.splits > 1) {
+    // this workgroup's piece of the stream: whole steps, counted from the last token back
+    const int all = last - first;
+    const int chunk = ((all + a.splits - 1) / a.splits + STEP - 1) / STEP * STEP;
+    const int s0 = min((int)blockIdx.y * chunk, all), s1 = min(s0 + chunk, all);
+    first = last - s1;
+    last -= s0;
+  }
   // Everything below counts tokens in the order they are streamed, from the last one back (see the head of this
   // file): place t is position last - 1 - t.
   const int kv_len = last - first;
@@ -627,6 +644,10 @@ void prefill_scored_kernel(PrefillArgs a) {
     const float inv = l_pos == 0.f ? 0.f : 1.f / l_pos;
     if (lane == 0) s_bad[wave] = 0;
     if (hi == 0) s_live[wave][lp] = live;
+    if (a.splits > 1 && hi == 0 && col_ok) {
+      const float lse = live && l_pos != 0.f ? (m_sub + __builtin_amdgcn_logf(l_pos)) * kLn2 : kNegInf;
+      a.parts_lse[((int64_t)blockIdx.y * a.total_q_tokens + q_row0 + pos) * a.n_q_heads + head] = lse;
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float ir = __shfl(inv, acc_row(r, 0) + 4 * hi);
@@ -647,8 +668,16 @@ void prefill_scored_kernel(PrefillArgs a) {
         f[k] = ok ? src[k] : 0.f;
         nan |= f[k] != f[k];
       }
-      const uint4 packed = E::pack(f);
       if (nan && (fold == 0 || (c8 * 8) / 64 == oh / fold)) atomicOr(&s_bad[wave], 1u << r);
+      if (a.splits > 1) {
+        const int dim = fold == 0 ? D : 64;
+        if (fold != 0 && (c8 * 8) / 64 != oh / fold) continue;
+        float* dst = a.parts_o + (((int64_t)blockIdx.y * a.total_q_tokens + orow) * a.n_q_heads + oh) * dim + (c8 * 8) % dim;
+        *(float4*)dst = make_float4(f[0], f[1], f[2], f[3]);
+        *(float4*)(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        continue;
+      }
+      const uint4 packed = E::pack(f);
       if (fold == 0) {
         *(uint4*)((char*)a.out + (orow * a.out_row_stride + (int64_t)oh * D + c8 * 8) * 2) = packed;
       } else if ((c8 * 8) / 64 == oh / fold) {
@@ -663,7 +692,7 @@ void prefill_scored_kernel(PrefillArgs a) {
     const int r = __ffs((int)bad) - 1;
     bad &= bad - 1;
     const int lo = __builtin_amdgcn_readlane(seen.x, r), n = __builtin_amdgcn_readlane(seen.y, r);
-    rescue_row<Tag>(a, q_row0 + r % PW, head0 + r / PW, kvh, req, prefix + q0 + r % PW, lo, lo + n);
+    rescue_row<Tag>(a, q_row0 + r % PW, head0 + r / PW, kvh, req, prefix + q0 + r % PW, max(lo, first), min(lo + n, last), (int)blockIdx.y);
   }
 }
 
@@ -700,10 +729,24 @@ hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream) {
   const int64_t local_groups = ((int64_t)a.max_groups * a.n_kv_heads + 7) / 8;
   const int64_t n_wg = 8 * local_groups * a.grp_blocks * n_z;
   if (n_wg > 0x7fffffffll) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)n_wg, 1, 1);
+  const dim3 grid((unsigned)n_wg, (unsigned)(a.splits > 1 ? a.splits : 1), 1);
   if (a.dtype == kBF16) a.blk_rows == 64 ? launch_shape<bf16_tag, 32>(a, grid, stream) : launch_shape<bf16_tag, 16>(a, grid, stream);
   else a.blk_rows == 64 ? launch_shape<f16_tag, 32>(a, grid, stream) : launch_shape<f16_tag, 16>(a, grid, stream);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits <= 1) return e;
+  MergeArgs mg;
+  mg.out = a.out;
+  mg.out_row_stride = a.out_row_stride;
+  mg.lse_out = nullptr;
+  mg.parts_o = a.parts_o;
+  mg.parts_lse = a.parts_lse;
+  mg.n_parts = a.splits;
+  mg.rows = a.total_q_tokens;
+  mg.n_heads = a.n_q_heads;
+  mg.head_dim = a.fold_group > 0 ? 64 : a.head_dim;
+  mg.dtype = a.dtype;
+  mg.row_end = a.cu_ext + a.batch;
+  return launch_merge(mg, stream);
 }
 
 }  // namespace bsgl

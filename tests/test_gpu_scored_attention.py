@@ -354,11 +354,11 @@ def intervals(kind, lens, ext, seed):
     return start, stop
 
 
-def extend_case(gpu, heads, dtype, ext, prefix, cap=0.0, slopes=False, kind=None, seed=0, layout="interleaved", extra_rows=0, only=None, poison=None, **kw):
+def extend_case(gpu, heads, dtype, ext, prefix, cap=0.0, slopes=False, kind=None, seed=0, layout="interleaved", extra_rows=0, only=None, poison=None, pad_cols=5, **kw):
     from baby_sglang_amd import _hip
 
     lens = [a + b for a, b in zip(ext, prefix)]
-    c = make(seed, heads, dtype, lens, layout, q_rows=sum(ext) + extra_rows)
+    c = make(seed, heads, dtype, lens, layout, pad_cols=pad_cols, q_rows=sum(ext) + extra_rows)
     st = sp = None
     if kind is not None:
         st, sp = (torch.tensor(x, dtype=torch.int32) for x in intervals(kind, lens, ext, seed))
@@ -434,6 +434,25 @@ def test_extend_a_few_tokens(gpu, heads, dtype, ext, prefix, kind):
 @pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("0.5b", torch.bfloat16), ("7b", torch.float32)])
 def test_extend_unowned_rows(gpu, heads, dtype):
     extend_case(gpu, heads, dtype, [150, 130], [0, 30], cap=20.0, seed=37, extra_rows=70, only=40)
+
+
+@pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("0.5b", torch.float16), ("7b", torch.float16), ("one", torch.bfloat16)])
+@pytest.mark.parametrize("ext,prefix,kind,cap", [([300], [2000], None, 20.0), ([260, 0, 90], [1500, 40, 700], "document", 0.0), ([280], [1800], "wild", 70.0),
+                                                 ([200, 150], [0, 2100], "prefix", 0.0), ([513], [1100], "empty", 30.0)])
+def test_extend_long_streams_in_pieces(gpu, heads, dtype, ext, prefix, kind, cap):
+    """Few blocks over long prefixes: the streams are cut and merged (page table of more than 2000 columns); short requests beside
+    long ones leave pieces empty; rows that no request owns stay as they were."""
+    extend_case(gpu, heads, dtype, ext, prefix, cap=cap, slopes=cap != 20.0, kind=kind, seed=38, extra_rows=9, only=24, pad_cols=800)
+
+
+def test_extend_pieces_keep_hidden_tokens_out(gpu):
+    """A NaN value in one piece of a cut stream: rows that do not see it are right, whichever piece it is in."""
+    def poison(c, row_req, row_pos, st, sp):
+        for at in (3, 700, 2100):
+            c["v"][c["table"][c["req"][0], at].long()] = float("nan")
+        st[:], sp[:] = torch.tensor([[4, 700], [701, 2100], [2101, 2300], [10, 600]]).t().repeat(1, 70)[:, : len(st)].to(torch.int32)
+
+    extend_case(gpu, "1.5b", torch.bfloat16, [280], [2020], cap=20.0, kind="wild", seed=39, only=30, poison=poison, pad_cols=800)
 
 
 def test_extend_long(gpu):
