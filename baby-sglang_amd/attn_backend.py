@@ -19,6 +19,11 @@ Behaviour kept from the reference, deliberately:
     (repeat_interleave, attn_backend.py:63-66, :132-135);
   * extend rows see page-table positions ``0 .. prefix_len + row``
     (attn_backend.py:74-92); requests with no extend tokens own no rows.
+
+Not in the reference: scored attention.  A layer with ``logit_cap`` (a number) or ``distance_slopes`` (float32
+per q head), and a batch with ``visible_from`` / ``visible_to`` / ``token_weights``
+(``SimplifiedForwardBatch``), take the scored kernels (``_hip.paged_decode_scored`` /
+``paged_prefill_scored``); everything else about the call is the same.
 """
 
 from __future__ import annotations
@@ -95,6 +100,7 @@ class SimpleAttentionBackend:
     # share split-merge tickets; likewise one extend workspace per stream
     _workspaces = _PerStream()
     _prefill_workspaces = _PerStream()
+    _scored_workspaces = _PerStream()  # (scored decode: larger by the scores, so kept apart)
 
     @staticmethod
     def forward(
@@ -112,14 +118,52 @@ class SimpleAttentionBackend:
         if forward_batch.is_prefill:
             if write_kv:
                 pool.set_kv_buffer(layer_id, forward_batch.out_cache_loc, k, v)
-            return SimpleAttentionBackend._prefill_attention(q, forward_batch, layer_id)
+            return SimpleAttentionBackend._prefill_attention(q, forward_batch, layer_id, attention_layer)
         if write_kv and k.dtype != pool.dtype:
             # the pool casts on write (memory_pool.py:163-165); keep that path separate
             pool.set_kv_buffer(layer_id, forward_batch.out_cache_loc, k, v)
             write_kv = False
+        scored = SimpleAttentionBackend._score_options(attention_layer, forward_batch)
+        if scored is not None:
+            return SimpleAttentionBackend._decode_scored(q, k if write_kv else None, v if write_kv else None, forward_batch, layer_id, scored)
         return SimpleAttentionBackend._decode_attention(
             q, k if write_kv else None, v if write_kv else None, forward_batch, layer_id
         )
+
+    @staticmethod
+    def _score_options(attention_layer, forward_batch):
+        """The scored kernels' keyword arguments for this layer and batch, or None for plain attention."""
+        cap = getattr(attention_layer, "logit_cap", None)
+        slopes = getattr(attention_layer, "distance_slopes", None)
+        lo, hi = getattr(forward_batch, "visible_from", None), getattr(forward_batch, "visible_to", None)
+        weights = None if forward_batch.is_prefill else getattr(forward_batch, "token_weights", None)
+        if not cap and slopes is None and lo is None and hi is None and weights is None:
+            return None
+        options = dict(logit_cap=cap or 0.0, slopes=slopes, visible_from=lo, visible_to=hi)
+        if weights is not None:
+            options["token_weights"] = weights
+        return options
+
+    @staticmethod
+    def _decode_scored(q, k, v, forward_batch: SimplifiedForwardBatch, layer_id: int, options):
+        cls = SimpleAttentionBackend
+        pool = forward_batch.token_to_kv_pool
+        if pool.store_dtype != pool.dtype:
+            raise NotImplementedError("float8 KV cache write is not supported in baby-sglang MVP")
+        fuses = k is not None and cls._fuses(forward_batch)
+        if fuses and cls.check_fused_kv_invariant:
+            cls._check_fused_kv(forward_batch)
+        k_slab, v_slab = pool.get_kv_buffer(layer_id)
+        table = forward_batch.req_to_token_pool.req_to_token
+        batch, hq, dim = q.shape
+        n_splits = _hip.decode_num_splits(batch, k_slab.shape[1], table.shape[1])
+        need = _hip.decode_scored_workspace_bytes(batch, hq, dim, n_splits, table.shape[1], "token_weights" in options)
+        ws = cls._scored_workspaces.get((q.device, _hip.current_stream_handle(q.device.index)), need,
+                                        lambda n: _hip.new_decode_workspace(max(n, 1 << 20), q.device))
+        return _hip.paged_decode_scored(
+            q, k_slab, v_slab, table, forward_batch.req_pool_indices, forward_batch.seq_lens, n_splits=n_splits, variant=cls.decode_variant,
+            workspace=ws, k_new=k, v_new=v, out_cache_loc=forward_batch.out_cache_loc if k is not None else None, fuse_kv_write=fuses,
+            max_seq_len=getattr(forward_batch, "max_seq_len", 0) or 0, **options)
 
     # (batch, heads, dim, columns) -> (n_splits, workspace bytes): two library calls per shape, not per layer
     _plans = {}
@@ -309,7 +353,8 @@ class SimpleAttentionBackend:
         )
 
     @staticmethod
-    def _prefill_attention(q, forward_batch: SimplifiedForwardBatch, layer_id: int):
+    def _prefill_attention(q, forward_batch: SimplifiedForwardBatch, layer_id: int, attention_layer=None):
+        scored = SimpleAttentionBackend._score_options(attention_layer, forward_batch)
         k_slab, v_slab = forward_batch.token_to_kv_pool.get_kv_buffer(layer_id)
         workspace = None
         list_ready = False
@@ -327,11 +372,15 @@ class SimpleAttentionBackend:
             # a LATER layer takes the list over, so a caller that keeps one batch object and rewrites its
             # tensors in place from step to step gets a new list with the first layer of every forward.
             ext = forward_batch.extended_lens
-            facts = (tuple(q.shape), q.dtype, k_slab.shape[1], _hip.knob_epoch)
+            facts = (tuple(q.shape), q.dtype, k_slab.shape[1], _hip.knob_epoch, scored is not None)
             held = getattr(workspace, "_bsgl_list_of", None)
             list_ready = (held is not None and held[0]() is forward_batch and held[1]() is ext and held[2] == facts
                           and layer_id > held[3])
             workspace._bsgl_list_of = (weakref.ref(forward_batch), weakref.ref(ext), facts, layer_id)
+        if scored is not None:
+            return _hip.paged_prefill_scored(
+                q, k_slab, v_slab, forward_batch.req_to_token_pool.req_to_token, forward_batch.req_pool_indices, forward_batch.seq_lens,
+                forward_batch.prefix_lens, forward_batch.extended_lens, workspace=workspace, list_ready=list_ready, **scored)
         return _hip.paged_prefill(
             q,
             k_slab,

@@ -48,6 +48,16 @@ class SimplifiedForwardBatch:
     # the cache, which is right for any page table (reference order: attn_backend.py:20-23).
     private_decode_slots: bool = False
 
+    # Not in the reference: scored attention.  The positions [visible_from, visible_to) of its own request
+    # that a row of q sees -- per extend token of a prefill batch, per request of a decode batch; int32 on
+    # the device, None = from 0 / to the row's own position (prefix, document and window masks).
+    visible_from: Optional[torch.Tensor] = None
+    visible_to: Optional[torch.Tensor] = None
+    # The table beside the page table that a decode batch's attention adds every visible token's softmax
+    # weight to, layer by layer, summed over the q heads (ReqToTokenPool.token_weights; prefill batches leave
+    # it alone).
+    token_weights: Optional[torch.Tensor] = None
+
     @classmethod
     def create_prefill_batch(
         cls,

@@ -74,6 +74,27 @@ class ReqToTokenPool:
     def clear(self) -> None:
         self.free_slots = list(range(self.size))
 
+    # ---- not in the reference: accumulated attention weights and eviction by them ----------------------
+    token_weights: Optional[torch.Tensor] = None
+
+    def enable_token_weights(self) -> torch.Tensor:
+        """The float32 table beside the page table that decode attention accumulates weights in
+        (``SimplifiedForwardBatch.token_weights``); made, all zero, on first use.  A weight belongs to a
+        COLUMN: whoever gives a row to another request, or appends a token, clears what the column held."""
+        if self.token_weights is None:
+            self.token_weights = torch.zeros((self.size, self.max_context_len), dtype=torch.float32, device=self.device)
+        return self.token_weights
+
+    def evict_tokens(self, req_pool_indices: torch.Tensor, seq_lens: torch.Tensor, budget: int, recent: int = 0, sinks: int = 0,
+                     max_seq_len: int = 0):
+        """Cut every longer request down to ``budget`` tokens -- the first ``sinks``, the last ``recent`` and the
+        heaviest others -- in place, page-table and weight rows together; ``(new_lens, evicted)`` as
+        ``_hip.evict_tokens`` gives them.  Freeing the evicted slots is the caller's business: some may be shared."""
+        from . import _hip  # raises if the HIP library is not built
+
+        return _hip.evict_tokens(self.req_to_token, self.enable_token_weights(), req_pool_indices, seq_lens, budget, recent, sinks,
+                                 max_seq_len=max_seq_len)
+
 
 class BaseTokenToKVPool:
     """Slot allocator: FIFO over a CPU int32 tensor of free slot ids.

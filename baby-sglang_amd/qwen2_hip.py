@@ -22,6 +22,10 @@ projections, row-parallel ``o_proj`` and ``down_proj`` each followed by ``tp_all
 (tp_runtime.py:28-33) -- over a KV pool of ``tp_layout.local_kv_heads`` heads; embeddings, norms and
 the vocabulary projection are replicated.  ``shard_state_dict`` cuts a whole (reference)
 ``state_dict`` down to a rank's.
+
+Scored attention (not in the reference): ``config.attn_logit_softcapping`` (a number) caps every layer's
+scores by a tanh, ``config.distance_slopes`` (one number per q head) biases them by distance; the attention
+shim carries both to the backend.
 """
 
 from __future__ import annotations
@@ -103,14 +107,27 @@ class GateUpLinear(nn.Module):
 class BabyRadixAttention(nn.Module):
     """The shim the backend reads ``layer_id`` / ``scaling`` from (qwen2.py:292-315)."""
 
-    def __init__(self, num_heads: int, head_dim: int, scaling: float, num_kv_heads: int, layer_id: int):
+    def __init__(self, num_heads: int, head_dim: int, scaling: float, num_kv_heads: int, layer_id: int,
+                 logit_cap: Optional[float] = None, distance_slopes=None):
         super().__init__()
+        if distance_slopes is not None and len(distance_slopes) != num_heads:
+            raise ValueError(f"{len(distance_slopes)} distance slopes for {num_heads} q heads")
+        self.logit_cap = float(logit_cap) if logit_cap else 0.0
+        # (on the module's device but in fp32 whatever its dtype: made anew from the numbers, see _apply)
+        self._slopes = None if distance_slopes is None else [float(x) for x in distance_slopes]
+        self.register_buffer("distance_slopes", None if self._slopes is None else torch.tensor(self._slopes, dtype=torch.float32), persistent=False)
         self.tp_q_head_num = num_heads
         self.tp_k_head_num = num_kv_heads
         self.tp_v_head_num = num_kv_heads
         self.head_dim = head_dim
         self.scaling = scaling
         self.layer_id = layer_id
+
+    def _apply(self, fn, recurse: bool = True):
+        super()._apply(fn, recurse)
+        if self.distance_slopes is not None and self.distance_slopes.dtype != torch.float32:
+            self.distance_slopes = torch.tensor(self._slopes, dtype=torch.float32, device=self.distance_slopes.device)
+        return self
 
     def forward(self, q, k, v, forward_batch: SimplifiedForwardBatch, save_kv_cache: bool = True):
         return SimpleAttentionBackend.forward(q, k, v, self, forward_batch, save_kv_cache)
@@ -119,7 +136,8 @@ class BabyRadixAttention(nn.Module):
 class Qwen2Attention(nn.Module):
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, layer_id: int = 0,
                  rope_theta: float = 1000000, rope_scaling=None, max_position_embeddings: int = 32768,
-                 tp_layout: Optional[TPLayout] = None, tp_group=None):  # fmt: skip
+                 tp_layout: Optional[TPLayout] = None, tp_group=None, logit_cap: Optional[float] = None,
+                 distance_slopes=None):  # fmt: skip
         super().__init__()
         self.head_dim = hidden_size // num_heads
         self.tp_layout, self.tp_group = _model_layout(tp_layout), tp_group
@@ -127,13 +145,15 @@ class Qwen2Attention(nn.Module):
             # this rank's heads: the projections are cut by output column (q / k / v) and input
             # column (o_proj) accordingly
             num_heads, num_kv_heads = self.tp_layout.local_q_heads, self.tp_layout.local_kv_heads
+            if distance_slopes is not None:
+                distance_slopes = distance_slopes[slice(*self.tp_layout.q_head_range)]
         self.num_heads = num_heads
         self.num_kv_heads = num_kv_heads
         self.scaling = self.head_dim**-0.5
         self.qkv_proj = QKVLinear(hidden_size, num_heads, num_kv_heads, self.head_dim, bias=True)
         self.o_proj = nn.Linear(num_heads * self.head_dim, hidden_size, bias=False)
         self.rotary_emb = RotaryEmbedding(self.head_dim, max_position_embeddings, rope_theta, rope_scaling)
-        self.attn = BabyRadixAttention(num_heads, self.head_dim, self.scaling, num_kv_heads, layer_id)
+        self.attn = BabyRadixAttention(num_heads, self.head_dim, self.scaling, num_kv_heads, layer_id, logit_cap, distance_slopes)
 
     def forward(self, positions: torch.Tensor, hidden_states: torch.Tensor, forward_batch: SimplifiedForwardBatch):
         qkv = self.qkv_proj.qkv_proj(hidden_states)
@@ -193,6 +213,8 @@ class Qwen2DecoderLayer(nn.Module):
             max_position_embeddings=getattr(config, "max_position_embeddings", 32768),
             tp_layout=tp_layout,
             tp_group=tp_group,
+            logit_cap=getattr(config, "attn_logit_softcapping", None),
+            distance_slopes=getattr(config, "distance_slopes", None),
         )
         self.mlp = Qwen2MLP(config.hidden_size, config.intermediate_size, getattr(config, "hidden_act", "silu"),
                             tp_layout=tp_layout, tp_group=tp_group)

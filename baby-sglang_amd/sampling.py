@@ -10,12 +10,17 @@ top-k and top-p share ONE descending sort: masking the values below the k-th onl
 tail of the sorted row into -inf, which is exactly the sorted row of the masked logits.
 The random draw itself (``torch.multinomial``) depends on the generator state and is not
 comparable across implementations.
+
+Not in the reference: presence and frequency penalties, sparse biases and token masks
+(``SamplingParams``, ``LogitControls``), applied to the logits ahead of all that by one HIP launch
+(``_hip.logit_controls``); the tokens a request has produced then live in a table on the device, so a step
+moves none of them.
 """
 
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import Dict, Optional, Sequence
 
 import torch
 
@@ -32,6 +37,89 @@ class SamplingParams:
     eos_id: int = -1
     do_sample: bool = False
     repetition_penalty: float = 1.0
+    # not in the reference: over the tokens a request has produced, x - frequency * count - presence
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Optional[Dict[int, float]] = None  # token id -> what is added to its logit
+    allowed_token_ids: Optional[Sequence[int]] = None  # every other token is left out
+
+    def needs_controls(self) -> bool:
+        return bool(self.presence_penalty or self.frequency_penalty or self.logit_bias or self.allowed_token_ids is not None)
+
+
+def pack_token_mask(allowed: torch.Tensor) -> torch.Tensor:
+    """``allowed`` (bool [..., vocab]) as the int32 words ``_hip.logit_controls`` takes: bit t % 32 of word t / 32."""
+    vocab = allowed.shape[-1]
+    padded = torch.nn.functional.pad(allowed.to(torch.int64), (0, -vocab % 32))
+    words = (padded.view(*allowed.shape[:-1], -1, 32) << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+
+
+class LogitControls:
+    """What ``SamplingParams`` asks of the logits of a serving loop's steps, and the tokens its requests have produced:
+    an int32 table ``[rows, columns]`` on the GPU, row r belonging to whoever owns page-table row r.  ``note``
+    appends a step's ids, ``apply`` gives the controlled logits; neither reads anything back."""
+
+    def __init__(self, params: SamplingParams, rows: int, columns: int, vocab: int, device: torch.device):
+        if torch.device(device).type != "cuda":
+            raise NotImplementedError("presence / frequency penalties, logit biases and token masks run on the GPU only")
+        self.params = params
+        self.vocab = vocab
+        self.history = torch.zeros((rows, columns), dtype=torch.int32, device=device)
+        fill = lambda x: torch.full((rows,), float(x), dtype=torch.float32, device=device)  # noqa: E731
+        self.repetition = fill(params.repetition_penalty) if (params.repetition_penalty or 1.0) > 1.0 else None
+        self.presence = fill(params.presence_penalty) if params.presence_penalty else None
+        self.frequency = fill(params.frequency_penalty) if params.frequency_penalty else None
+        self.bias_ids = self.bias_values = self.token_mask = None
+        if params.logit_bias:
+            ids, values = zip(*sorted(params.logit_bias.items()))
+            if min(ids) < 0 or max(ids) >= vocab:
+                raise ValueError(f"logit_bias names a token outside the vocabulary of {vocab}")
+            self.bias_ids = torch.tensor([ids], dtype=torch.int32, device=device).repeat(rows, 1)
+            self.bias_values = torch.tensor([values], dtype=torch.float32, device=device).repeat(rows, 1)
+        if params.allowed_token_ids is not None:
+            allowed = torch.zeros(vocab, dtype=torch.bool)
+            ids = torch.as_tensor(list(params.allowed_token_ids), dtype=torch.long)
+            if ids.numel() == 0 or int(ids.min()) < 0 or int(ids.max()) >= vocab:
+                raise ValueError(f"allowed_token_ids must name at least one token, all of them inside the vocabulary of {vocab}")
+            allowed[ids] = True
+            self.token_mask = pack_token_mask(allowed)[None].to(device)
+            self._first = torch.zeros(rows, dtype=torch.int32, device=device)
+
+        # (without a mask or a bias of -inf every token keeps a chance)
+        self._can_empty = params.allowed_token_ids is not None or bool(params.logit_bias and min(params.logit_bias.values()) == float("-inf"))
+
+    def note(self, rows: torch.Tensor, counts: torch.Tensor, ids: torch.Tensor) -> None:
+        """Token ``ids[i]`` is number ``counts[i]`` (from 0) that row ``rows[i]``'s request produced."""
+        self.history[rows, counts] = ids.to(torch.int32)
+
+    def apply(self, logits: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The logits of requests on ``rows`` that have produced ``counts`` tokens each.  ``token_mask`` (int32 words, one row
+        per request) narrows the parameters' own.  Controls that leave a request no token raise (a draw from nothing
+        ends the process); telling takes a read of the device, made only where masks or infinite biases are in play."""
+        from . import _hip
+
+        n, words = logits.shape[0], (self.vocab + 31) // 32
+        kw = {}
+        if self.repetition is not None or self.presence is not None or self.frequency is not None:
+            cut = lambda t: None if t is None else t[:n]  # noqa: E731
+            kw = dict(history=self.history, history_rows=rows, history_lens=counts, repetition=cut(self.repetition), presence=cut(self.presence),
+                      frequency=cut(self.frequency))
+        if self.bias_ids is not None:
+            kw.update(bias_ids=self.bias_ids[:n], bias_values=self.bias_values[:n])
+        if token_mask is not None:
+            if token_mask.dtype != torch.int32 or token_mask.dim() != 2 or token_mask.shape[0] != n or token_mask.shape[1] < words:
+                raise ValueError(f"token_mask must be int32 [{n}, {words}] (pack_token_mask), got {token_mask.dtype} {tuple(token_mask.shape)}")
+            token_mask = token_mask.to(logits.device).contiguous()
+            kw["token_mask"] = token_mask if self.token_mask is None else token_mask[:, :words] & self.token_mask
+        elif self.token_mask is not None:
+            kw.update(token_mask=self.token_mask, mask_rows=self._first[:n])
+        controlled = _hip.logit_controls(logits, **kw)
+        if self._can_empty or token_mask is not None:
+            empty = (controlled.amax(-1) == float("-inf")).tolist()
+            if any(empty):
+                raise ValueError(f"masks and biases leave no token to pick for request {empty.index(True)} of the batch")
+        return controlled
 
 
 def apply_repetition_penalty_(logits: torch.Tensor, prev_ids: Sequence[Sequence[int]], penalty: float) -> torch.Tensor:

@@ -48,6 +48,18 @@ tokens each.  Admission, slots and page-table rows are exactly those of the unch
 batch -- every row is written up front -- and a chunk is an extend over
 ``prefix_len + tokens already run``; a request cut by a chunk border continues in the
 next call, and a request is sampled from the call that holds its last prompt token.
+
+Bounded cache (not in the reference): with ``kv_budget = N`` a request never holds more than N cached tokens plus
+``kv_slack`` for long.  Decode attention accumulates what weight every cached token received; when a request has
+grown to N + ``kv_slack`` tokens, the ones with the least weight are evicted down to N (``ReqToTokenPool.evict_tokens``; the
+first ``kv_sinks`` and the last ``kv_recent`` always stay).  Kept keys keep the positions they were rotated to,
+and new tokens go on counting from where the request really is; a distance bias counts cached tokens.  Evicted slots
+that the prefix tree holds stay with the tree, and a request that has lost tokens is not put into it at its end.
+Off, nothing of this runs.
+
+Controlled logits (not in the reference): presence / frequency penalties, biases and allowed tokens of
+``SamplingParams``, and ``token_mask_fn(batch)`` for masks that change from step to step (a grammar): int32 words
+[len(batch), ceil(vocab / 32)] (``sampling.pack_token_mask``) or None.
 """
 
 from __future__ import annotations
@@ -63,7 +75,7 @@ import torch
 from .forward_batch import SimplifiedForwardBatch
 from .memory_pool import MHATokenToKVPool, ReqToTokenPool
 from .prefix_cache import PrefixCache, PrefixNode
-from .sampling import SamplingParams, sample_next_ids
+from .sampling import LogitControls, SamplingParams, sample_next_ids
 
 
 @dataclass(eq=False)
@@ -82,8 +94,15 @@ class Sequence_:
     last_node: Optional[PrefixNode] = None
     num_cached: int = 0
     in_flight: int = 0  # steps launched whose ids have not been looked at yet (overlap mode)
+    evicted: int = 0  # tokens given up to the cache budget: the next position is seq_len + evicted
+
+    def own_slots(self) -> List[int]:
+        """The slots of the row that are not the prefix tree's."""
+        shared = set(self.prefix_slots.tolist())
+        return [t for t in self.table if t not in shared]
 
     def reset(self) -> None:
+        self.evicted = 0
         self.output_ids, self.finished, self.row, self.seq_len, self.table = [], False, None, 0, []
         self.prefix_slots, self.last_node, self.num_cached = torch.empty(0, dtype=torch.int32), None, 0
 
@@ -176,8 +195,20 @@ class _ForwardWorker:
 
 class ServingLoop:
     def __init__(self, model, max_total_tokens: Optional[int] = None, max_requests: Optional[int] = None,
-                 chunked_prefill_size: Optional[int] = None, overlap_worker: Optional[bool] = None):
+                 chunked_prefill_size: Optional[int] = None, overlap_worker: Optional[bool] = None,
+                 kv_budget: Optional[int] = None, kv_recent: Optional[int] = None, kv_sinks: Optional[int] = None, kv_slack: Optional[int] = None):
         self.model = model
+        self.kv_budget = kv_budget
+        if kv_budget is not None:
+            if kv_budget < 1:
+                raise ValueError("kv_budget must be positive")
+            if any(getattr(m, "tp_layout", None) is not None for m in model.modules()):
+                raise NotImplementedError("kv_budget: a tensor-parallel rank sees its own heads' weights only, the ranks would evict different tokens")
+            self.kv_sinks = min(4, kv_budget // 2) if kv_sinks is None else kv_sinks
+            self.kv_recent = kv_budget // 4 if kv_recent is None else kv_recent
+            self.kv_slack = max(1, kv_budget // 8) if kv_slack is None else kv_slack
+            if self.kv_recent < 0 or self.kv_sinks < 0 or self.kv_sinks + self.kv_recent > kv_budget or self.kv_slack < 1:
+                raise ValueError(f"kv_budget {kv_budget} must hold {self.kv_sinks} sinks and {self.kv_recent} recent tokens; kv_slack is at least 1")
         if chunked_prefill_size is not None and chunked_prefill_size < 1:
             raise ValueError("chunked_prefill_size must be positive")
         self.chunked_prefill_size = chunked_prefill_size
@@ -202,6 +233,14 @@ class ServingLoop:
         self.finished: List[Sequence_] = []
         self.est_new_token_ratio = self.r_init
         self.on_batch = None  # optional hook: on_batch(mode, forward_batch) before every model call
+        self.token_mask_fn = None  # optional hook: token_mask_fn(batch) -> int32 words [len(batch), ceil(vocab / 32)] or None
+        self._controls: Optional[LogitControls] = None
+        if kv_budget is not None:
+            if kv_budget + self.kv_slack > self.req_to_token_pool.max_context_len:
+                raise ValueError(f"kv_budget {kv_budget} and kv_slack {self.kv_slack} do not fit a page-table row of {self.req_to_token_pool.max_context_len}")
+            if self.device.type != "cuda":
+                raise NotImplementedError("kv_budget needs a GPU: the weights come out of its attention kernels")
+            self.req_to_token_pool.enable_token_weights()
         # pinned staging for host-to-device copies that must not block (three arenas in rotation:
         # one per step being built, in flight, and just finished)
         self._staging = None
@@ -254,6 +293,7 @@ class ServingLoop:
     def run_batch(self, requests: Sequence[torch.Tensor], sampling: Optional[SamplingParams] = None) -> List[List[int]]:
         sampling = sampling or SamplingParams()
         self._sampling = sampling
+        self._start_controls(sampling)
         self.waiting, self.decoding, self.finished = [], [], []
         self.est_new_token_ratio = self.r_init
         order = []
@@ -272,7 +312,15 @@ class ServingLoop:
                 fb = self._decode_batch(batch)
                 next_ids = self._pick(self._forward(mode, fb), batch).tolist()
             self._finish_step(next_ids, batch, mode)
+            if self.kv_budget is not None and mode == "decode":
+                self._evict_over_budget(batch)
         return [s.output_ids for s in order]
+
+    def _start_controls(self, sampling: SamplingParams) -> None:
+        self._controls = None
+        if sampling.needs_controls() or self.token_mask_fn is not None:
+            columns = max(1, min(sampling.max_new_tokens, self.max_total_tokens))  # (a request never produces more)
+            self._controls = LogitControls(sampling, self.max_requests, columns, self.model.config.vocab_size, self.device)
 
     def run_batch_overlap(self, requests: Sequence[torch.Tensor], sampling: Optional[SamplingParams] = None) -> List[List[int]]:
         """``run_batch`` with a batch's ids looked at one step late, so that selecting,
@@ -284,6 +332,9 @@ class ServingLoop:
         self._sampling = SamplingParams(**{**sampling.__dict__, "repetition_penalty": 1.0})
         if self.chunked_prefill_size is not None:
             raise NotImplementedError("overlap mode runs whole-prompt prefill batches")
+        if self.kv_budget is not None or sampling.needs_controls() or self.token_mask_fn is not None:
+            raise NotImplementedError("overlap mode has neither a cache budget nor controlled logits: both need the ids of the step in flight")
+        self._controls = None
         self.waiting, self.decoding, self.finished = [], [], []
         self.est_new_token_ratio = self.r_init
         if self._last_ids is None:
@@ -446,6 +497,15 @@ class ServingLoop:
         """One id per request from its row of ``logits``: the whole batch at once, on the device
         (scheduler.py:523-546 does it request by request)."""
         sp = self._sampling
+        if self._controls is not None:
+            # (the repetition penalty is among the controls then, over the same tokens)
+            rows = self._h2d([s.row for s in batch], torch.long)
+            counts = self._h2d([len(s.output_ids) for s in batch], torch.long)
+            mask = self.token_mask_fn(batch) if self.token_mask_fn is not None else None
+            logits = self._controls.apply(logits, rows, counts, mask)
+            ids = sample_next_ids(logits, sp.do_sample, sp.temperature, sp.top_k, sp.top_p, generator=self.generator)
+            self._controls.note(rows, counts, ids)
+            return ids
         prev = [s.output_ids for s in batch] if sp.repetition_penalty > 1.0 else None
         return sample_next_ids(logits, sp.do_sample, sp.temperature, sp.top_k, sp.top_p, prev, sp.repetition_penalty,
                                generator=self.generator)
@@ -531,7 +591,8 @@ class ServingLoop:
         admitted: List[Sequence_] = []
         for s in self.waiting:
             tree.inc_lock_ref(s.last_node)  # its own prefix does not count as evictable
-            need = len(s.input_ids) - len(s.prefix_slots) + s.max_new_tokens
+            grows_by = s.max_new_tokens if self.kv_budget is None else min(s.max_new_tokens, self.kv_budget + self.kv_slack)
+            need = len(s.input_ids) - len(s.prefix_slots) + grows_by
             fits = len(admitted) + 1 <= rows_free and need <= budget + tree.evictable_size()
             if fits:
                 budget -= need
@@ -555,7 +616,7 @@ class ServingLoop:
             if not self.decoding:
                 break
             s = self.decoding.pop()
-            pool.free(torch.tensor(s.table[s.num_cached : s.seq_len], dtype=torch.int32))
+            pool.free(torch.tensor(s.own_slots() if self.kv_budget is not None else s.table[s.num_cached : s.seq_len], dtype=torch.int32))
             self.req_to_token_pool.free(s.row)
             tree.dec_lock_ref(s.last_node)
             s.reset()
@@ -604,6 +665,8 @@ class ServingLoop:
             used += n_new
         rows_t = self._h2d(rows, torch.long)
         r2t.write(rows_t, self._h2d(mapping, torch.int32))
+        if self.kv_budget is not None:
+            r2t.token_weights[rows_t] = 0.0  # (the rows' last owners' weights)
         return SimplifiedForwardBatch.create_prefill_batch(
             input_ids=self._h2d(new_ids, torch.long),
             req_pool_indices=rows_t,
@@ -646,10 +709,36 @@ class ServingLoop:
             token_to_kv_pool=self.token_to_kv_pool,
         )
         fb.max_seq_len = max(s.seq_len for s in batch)  # (known here without asking the device)
+        if self.kv_budget is not None:
+            weights = self.req_to_token_pool.token_weights
+            weights[rows_t, seq_t - 1] = 0.0  # (an evicted token may have stood in the column)
+            fb.token_weights = weights
+            if any(s.evicted for s in batch):
+                fb.positions = self._h2d([s.seq_len - 1 + s.evicted for s in batch], torch.long)
         # every new slot comes straight from the free list and is written into its own request's row
         # only; a slot the prefix tree shares is never a decode step's new slot
         fb.private_decode_slots = True
         return fb
+
+    # ---------------------------------------------------------------------------- the cache budget
+    def _evict_over_budget(self, batch: List[Sequence_]) -> None:
+        """Bring the requests of a decode step that have outgrown the budget by the slack back to it.  Waits for the
+        device (the host's copies of the page-table rows have to follow), once per ``kv_slack`` tokens of a request."""
+        over = [s for s in batch if not s.finished and s.seq_len >= self.kv_budget + self.kv_slack]
+        if not over:
+            return
+        longest = max(s.seq_len for s in over)
+        _, evicted = self.req_to_token_pool.evict_tokens(
+            self._h2d([s.row for s in over], torch.long), self._h2d([s.seq_len for s in over], torch.long), self.kv_budget,
+            recent=self.kv_recent, sinks=self.kv_sinks, max_seq_len=longest)
+        for s, gone in zip(over, evicted.tolist()):
+            gone = set(gone[: s.seq_len - self.kv_budget])
+            shared = set(s.prefix_slots.tolist())
+            self.token_to_kv_pool.free(torch.tensor([t for t in s.table if t in gone and t not in shared], dtype=torch.int32))
+            s.table = [t for t in s.table if t not in gone]
+            s.evicted += s.seq_len - self.kv_budget
+            s.seq_len = self.kv_budget
+            assert len(s.table) == s.seq_len
 
     # ---------------------------------------------------------------------------- results
     def _finish_step(self, next_ids: List[int], batch: List[Sequence_], mode: str) -> None:
@@ -671,6 +760,12 @@ class ServingLoop:
     def _cache_finished(self, s: Sequence_) -> None:
         """radix_cache.py:141-173: the tokens whose K/V are written (all but the last
         generated one) go into the tree; duplicates of already cached slots are freed."""
+        if s.evicted:
+            # (what is left is no prefix of anything: its own slots go back, the tree keeps its prompt)
+            self.token_to_kv_pool.free(torch.tensor(s.own_slots(), dtype=torch.int32))
+            self.req_to_token_pool.free(s.row)
+            self.tree_cache.dec_lock_ref(s.last_node)
+            return
         tokens = (s.input_ids + s.output_ids)[:-1] if s.output_ids else list(s.input_ids)
         if tokens:
             slots = torch.tensor(s.table[: len(tokens)], dtype=torch.int32)
