@@ -777,6 +777,9 @@ def evict_tokens(
 
 # ---- logit controls -----------------------------------------------------------------------------
 
+LOGIT_MAX_BIAS = 4096  # biases per request
+LOGIT_MAX_HISTORY = 262143  # columns of a history
+
 
 def logit_controls(
     logits: torch.Tensor,
@@ -846,6 +849,8 @@ def logit_controls(
 
     long, int_ = (torch.int64, torch.int32), (torch.int32, torch.int64)
     past = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    if history is not None and history.dim() == 2 and history.shape[1] == 0:  # (no column: nothing to penalise, and no address)
+        history = history_rows = history_lens = prompt_lens = repetition = presence = frequency = None
     if history is not None:
         if history_lens is None:
             raise ValueError("history needs history_lens")

@@ -389,6 +389,10 @@ int scratch_of_current_device(void** out, bool capturing) {
 // the description of a scored call into a launch's arguments
 int take_mods(bsgl::DecodeArgs& a, const bsgl_score_mods& m) {
   if (!(m.logit_cap >= 0.f) || m.logit_cap > 3.0e38f) return fail(BSGL_ERR_BAD_ARG, "logit_cap %g is negative or not finite", (double)m.logit_cap);
+  // (tanh is good to 2^-22 of the cap: 0.004 of a score at the upper end, beyond it the cap's own error would show; below
+  // the lower end 1 / cap runs out of range)
+  if (m.logit_cap != 0.f && (m.logit_cap < 0x1p-20f || m.logit_cap > 16384.f))
+    return fail(BSGL_ERR_BAD_ARG, "logit_cap %g is outside [2^-20, 2^14]", (double)m.logit_cap);
   a.scored = true;
   a.mods.cap = m.logit_cap;
   a.mods.slopes = m.slopes;
@@ -501,6 +505,7 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
   if (mods != nullptr) {
     if (int rc = take_mods(a, *mods)) return rc;
     if (mods->token_weights != nullptr) {
+      if (batch > 65535) return fail(BSGL_ERR_UNSUPPORTED, "token weights of a batch of %d requests, up to 65535 are taken", batch);
       const size_t all = bsgl_decode_scored_workspace_bytes(batch, n_q_heads, head_dim, asked_splits, f32_out, table_cols, 1);
       if (workspace == nullptr || workspace_bytes < all || !aligned16(workspace))
         return fail(BSGL_ERR_WORKSPACE, "scored decode with token weights needs a 16-byte aligned workspace of %zu bytes (got %zu)", all, workspace ? workspace_bytes : (size_t)0);
@@ -883,7 +888,13 @@ int bsgl_evict_tokens(int32_t* out_table, float* out_weights, const int32_t* req
   if (batch == 0) return BSGL_OK;
   if (!out_table || !out_weights || !req_to_token || !token_weights || !req_pool_indices || !seq_lens || !new_lens)
     return fail(BSGL_ERR_BAD_ARG, "null device pointer (tables / req_pool_indices / seq_lens / new_lens)");
-  if (table_rows <= 0 || table_cols <= 0 || table_cols > 0x7fffffff) return fail(BSGL_ERR_BAD_ARG, "page-table extents must be positive and below 2^31 columns");
+  // (a chunk's last positions have to fit 32 bits as well)
+  if (table_rows <= 0 || table_cols <= 0 || table_cols > 0x7fff0000) return fail(BSGL_ERR_BAD_ARG, "page-table extents must be positive and below 2^31 - 2^16 columns");
+  {
+    // (workgroups of a request read its length after others have written the new one)
+    const uintptr_t s0 = (uintptr_t)seq_lens, n0 = (uintptr_t)new_lens, bytes = (uintptr_t)batch * 8;
+    if (s0 < n0 + bytes && n0 < s0 + bytes) return fail(BSGL_ERR_BAD_ARG, "new_lens must not overlap seq_lens");
+  }
   if (table_row_stride < table_cols || weights_row_stride < table_cols)
     return fail(BSGL_ERR_BAD_ARG, "a row stride is shorter than the page table's column count");
   if (evicted_cols < 0 || (evicted != nullptr && evicted_row_stride < evicted_cols))
@@ -928,6 +939,8 @@ int bsgl_logit_controls(const bsgl_logit_call* c) {
   if (c->vocab > (1 << 30)) return fail(BSGL_ERR_UNSUPPORTED, "vocabulary of %d tokens above 2^30", c->vocab);
   if (!c->out || !c->logits) return fail(BSGL_ERR_BAD_ARG, "null device pointer (out/logits)");
   if (c->out_row_stride < c->vocab || c->logits_row_stride < c->vocab) return fail(BSGL_ERR_BAD_ARG, "logit row stride shorter than the vocabulary");
+  if (c->out == c->logits && c->batch > 1 && c->out_row_stride != c->logits_row_stride)
+    return fail(BSGL_ERR_BAD_ARG, "logits controlled in place must keep their row stride");
   if (c->history != nullptr) {
     if (!c->history_lens) return fail(BSGL_ERR_BAD_ARG, "history without history_lens");
     if (c->history_n_rows <= 0 || c->history_cols < 0 || c->history_row_stride < c->history_cols)

@@ -169,8 +169,7 @@ __global__ __launch_bounds__(kThreads) void logit_controls_kernel(LogitArgs a) {
   auto finish = [&](float x, uint32_t c) {
     const uint32_t made = c & kCount;
     if (c & (kPrompt | kCount)) x *= x > 0.f ? inv : rep;
-    x -= freq * (float)made;
-    if (made != 0) x -= pres;
+    if (made != 0) x = (x - freq * (float)made) - pres;  // (only then: an infinite penalty times 0 is NaN)
     if (c & kBiased) x += s_sums[(c >> kCountBits) & kEntry];
     return x;
   };

@@ -711,8 +711,8 @@ void launch_shape(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
 
 // the extend kernels' conditions, with up to 16 q heads per kv head (a workgroup takes them two or eight at a time)
 bool prefill_scored_supported(const PrefillArgs& a, const char** why) {
-  // (without a cap the largest score is taken to be the largest product)
-  if (!(a.mods.cap > 0.f) && !(a.scale > 0.f)) {
+  // (without a cap the largest score is taken to be the largest product, and a bias is carried in units of the scale)
+  if (!(a.mods.cap > 0.f) && !(a.scale > 1e-30f)) {
     *why = "the matrix-core kernel needs a positive scale";
     return false;
   }

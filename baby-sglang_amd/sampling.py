@@ -63,6 +63,12 @@ class LogitControls:
     def __init__(self, params: SamplingParams, rows: int, columns: int, vocab: int, device: torch.device):
         if torch.device(device).type != "cuda":
             raise NotImplementedError("presence / frequency penalties, logit biases and token masks run on the GPU only")
+        from . import _hip
+
+        if columns > _hip.LOGIT_MAX_HISTORY and (params.presence_penalty or params.frequency_penalty or (params.repetition_penalty or 1.0) > 1.0):
+            raise NotImplementedError(f"penalties over more than {_hip.LOGIT_MAX_HISTORY} tokens of a request (max_new_tokens is {columns})")
+        if params.logit_bias and len(params.logit_bias) > _hip.LOGIT_MAX_BIAS:
+            raise NotImplementedError(f"{len(params.logit_bias)} logit biases, up to {_hip.LOGIT_MAX_BIAS} are taken")
         self.params = params
         self.vocab = vocab
         self.history = torch.zeros((rows, columns), dtype=torch.int32, device=device)

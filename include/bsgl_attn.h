@@ -254,7 +254,7 @@ int bsgl_paged_decode_static(void* out /*device*/, int64_t out_row_stride,
  * Scored attention: what happens to a score between q . k and the softmax, in this order.  For the
  * query at position i of its request, the cached token at position j and q head h
  *   s = scale * q_h . k_j
- *   s = logit_cap * tanh(s / logit_cap)        when logit_cap > 0 (0 = none; negative or not finite is refused)
+ *   s = logit_cap * tanh(s / logit_cap)        when logit_cap > 0 (0 = none; 2^-20 to 2^14, anything else is refused)
  *   s = s - slopes[h] * |i - j|                when slopes is given (fp32 [n_q_heads])
  * and the row attends to j in [visible_from, visible_to) only: int32 per ROW of q (request of a decode
  * call, extend token of a prefill call), in positions of the request's page-table row, clamped to
@@ -303,7 +303,7 @@ int bsgl_paged_decode_scored(const bsgl_decode_call* call, const bsgl_score_mods
  * its input), new_lens[i] = min(seq_lens[i], budget) receives their number, and evicted (optional, [batch, evicted_cols])
  * the slots of the others in their order, as many as fit, then -1.  Entries behind new_lens[i], and rows that no request
  * names, are left as they are.  A row named by several requests is compacted for the first of them; the others get an
- * empty evicted list.  max_seq_len (0 = unknown) shapes the launch only.  workspace: bsgl_evict_workspace_bytes, may be
+ * empty evicted list.  new_lens must not overlap seq_lens.  max_seq_len (0 = unknown) shapes the launch only.  workspace: bsgl_evict_workspace_bytes, may be
  * NULL when that is 0.
  */
 size_t bsgl_evict_workspace_bytes(int32_t batch, int64_t table_cols, int32_t budget);

@@ -163,3 +163,55 @@ def test_refusals(gpu):
         _hip.evict_tokens(t.cpu(), w, req, lens, 4)
     got, gone = _hip.evict_tokens(t, w, req[:0], lens[:0], 4)
     assert got.shape == (0,) and gone.shape == (0, 28)
+
+
+def test_long_rows_in_a_graph_and_on_two_streams(gpu):
+    """The form over several workgroups: replays with a workspace of their own, and two calls at once on two streams."""
+    from baby_sglang_amd import _hip
+
+    g = torch.Generator().manual_seed(9)
+    cols, budget = 40000, 9000
+    t0 = torch.randint(0, 1 << 30, (2, cols), generator=g, dtype=torch.int32).to(gpu)
+    w0 = torch.rand(2, cols, generator=g).to(gpu)
+    req, lens = torch.tensor([1, 0], device=gpu), torch.tensor([39999, 25000], device=gpu)
+    ws = [torch.empty(_hip.evict_workspace_bytes(2, cols, budget), dtype=torch.uint8, device=gpu) for _ in range(2)]
+    table, w = t0.clone(), w0.clone()
+    new_lens, gone = torch.zeros(2, dtype=torch.int64, device=gpu), torch.zeros((2, cols - budget), dtype=torch.int32, device=gpu)
+
+    def call(t, x, ws, **kw):
+        return _hip.evict_tokens(t, x, req, lens, budget, recent=100, sinks=4, workspace=ws, **kw)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(t0.clone(), w0.clone(), ws[0])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(table, w, ws[0], new_lens=new_lens, evicted=gone)
+    for i in range(3):
+        table.copy_(t0)
+        w.copy_((w0 * (i + 1)).frac())
+        et, ew = table.clone(), w.clone()
+        want = call(et, ew, None)
+        gone.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(table, et) and torch.equal(w, ew) and torch.equal(gone, want[1]) and torch.equal(new_lens, want[0])
+    pairs = [(t0.clone(), w0.clone()) for _ in range(2)]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(*pairs[0], ws[0])
+    call(*pairs[1], ws[1])
+    torch.cuda.synchronize()
+    assert torch.equal(pairs[0][0], pairs[1][0]) and torch.equal(pairs[0][1], pairs[1][1])
+
+
+def test_new_lengths_over_the_old_ones_are_refused(gpu):
+    from baby_sglang_amd import _hip
+
+    t, w = torch.zeros(4, 32, dtype=torch.int32, device=gpu), torch.zeros(4, 32, device=gpu)
+    lens = torch.tensor([30, 3], device=gpu)
+    with pytest.raises(ValueError, match="overlap"):
+        _hip.evict_tokens(t, w, torch.tensor([0, 1], device=gpu), lens, 4, new_lens=lens)

@@ -208,3 +208,33 @@ def test_refusals(gpu):
     with pytest.raises(RuntimeError):
         _hip.logit_controls(x.cpu())
     assert _hip.logit_controls(x[:0]).shape == (0, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_penalties_touch_produced_tokens_only(gpu, dtype):
+    """A penalty of inf forbids what was produced; the prompt's tokens and biased ones stay numbers."""
+    from baby_sglang_amd import _hip
+
+    x = torch.ones(1, 64, dtype=dtype, device=gpu)
+    h = torch.tensor([[3, 4, 5]], dtype=torch.int32, device=gpu)
+    ids, vals = torch.tensor([[9]], dtype=torch.int32, device=gpu), torch.tensor([[2.0]], device=gpu)
+    inf = float("inf")
+    for kw in (dict(frequency=inf), dict(presence=inf)):
+        got = _hip.logit_controls(x, history=h, history_lens=torch.tensor([3], device=gpu), prompt_lens=torch.tensor([2], device=gpu), bias_ids=ids,
+                                  bias_values=vals, **kw)[0]
+        want = torch.ones(64)
+        want[5], want[9] = -inf, 3.0
+        assert torch.equal(got.float().cpu(), want)
+
+
+def test_as_many_biases_as_are_taken(gpu):
+    case(gpu, 2, 9000, torch.float32, seed=11, bias=4096, hist=20)
+
+
+def test_a_history_without_columns(gpu):
+    from baby_sglang_amd import _hip
+
+    x = torch.randn(2, 40, device=gpu)
+    got = _hip.logit_controls(x, history=torch.zeros((2, 0), dtype=torch.int32, device=gpu), history_lens=torch.zeros(2, dtype=torch.int64, device=gpu),
+                              repetition=1.5, presence=1.0)
+    assert torch.equal(got, x)

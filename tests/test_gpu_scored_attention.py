@@ -600,3 +600,43 @@ def test_extend_refusals(gpu):
         _hip.paged_prefill_scored(*args[:6], args[6][:1], args[7])
     with pytest.raises(RuntimeError):
         _hip.paged_prefill_scored(*args[:7], args[7].cpu())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_decode_writes_new_rows_nobody_sees(gpu, dtype):
+    """Intervals that end before the new token, and empty ones: its K/V row is written all the same, fused or not."""
+    from baby_sglang_amd import _hip
+
+    lens = [40, 700, 1, 90]
+    c = make(51, "1.5b", dtype, lens)
+    st, sp = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0, 30, 1, 60], [39, 600, 1, 20]))
+    for fuse in (False, True):
+        d = to_gpu(c, gpu)
+        kn, vn = torch.full((4, 2, 128), 3.0, dtype=dtype, device=gpu), torch.full((4, 2, 128), float("nan"), dtype=dtype, device=gpu)
+        loc = torch.stack([d["table"][d["req"][i], lens[i] - 1] for i in range(4)])
+        w = torch.zeros(d["table"].shape, device=gpu)
+        out = _hip.paged_decode_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], logit_cap=8.0, visible_from=st, visible_to=sp, k_new=kn,
+                                       v_new=vn, out_cache_loc=loc, fuse_kv_write=fuse, token_weights=w)
+        assert torch.equal(d["k"][loc.long()], kn) and bool(d["v"][loc.long()].isnan().all())
+        assert bool(out.isfinite().all()) and not bool(out[2:].any()) and bool(w.isfinite().all())
+
+
+@pytest.mark.parametrize("cap", [2.0**-20, 1e-3, 16384.0])
+def test_smallest_and_largest_caps(gpu, cap):
+    decode_case(gpu, "1.5b", torch.bfloat16, [300, 20], cap=cap, seed=52)
+    decode_case(gpu, "mha", torch.float32, [300, 20], cap=cap, seed=53)
+    extend_case(gpu, "1.5b", torch.bfloat16, [90, 33], [0, 70], cap=cap, seed=54)
+    extend_case(gpu, "1.5b", torch.bfloat16, [90, 33], [0, 70], cap=cap, slopes=True, seed=55)
+
+
+def test_extend_tiny_scale_with_a_bias(gpu):
+    from baby_sglang_amd import _hip
+
+    c = make(56, "1.5b", torch.bfloat16, [100], q_rows=100)
+    d = to_gpu(c, gpu)
+    sl = slopes_of(12)
+    for scale in (1e-36, 1e-20):
+        out = _hip.paged_prefill_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.zeros(1, dtype=torch.int64, device=gpu), d["seq"],
+                                        scale=scale, slopes=sl.to(gpu))
+        want, mass, lse, _, top = orc.scored_exact(c["q"], c["k"], c["v"], c["table"][c["req"]], [100], [0] * 100, range(100), scale, 0.0, sl)
+        check_rows(out, want, mass, lse, top + 100.0, 0.0, torch.bfloat16, torch.bfloat16, 2.0**-8, 100, 6.0, 128)

@@ -43,6 +43,29 @@ def test_scored_decode_refusals():
     assert f(decode_call(batch=0), mods(logit_cap=1.0)) == _hip.BSGL_OK  # nothing to do
 
 
+def test_scored_caps_out_of_range():
+    for cap in (1e-9, 2.0**-21, 16385.0, 1e30):
+        assert lib.bsgl_paged_decode_scored(decode_call(), mods(logit_cap=cap)) == _hip.BSGL_ERR_BAD_ARG and b"logit_cap" in lib.bsgl_last_error()
+    big = decode_call(batch=65536)
+    assert lib.bsgl_paged_decode_scored(big, mods(token_weights=256, token_weights_out=256, weights_row_stride=64)) == _hip.BSGL_ERR_UNSUPPORTED
+
+
+def test_evict_lengths_must_not_overlap():
+    def f(seq, new, batch=4, cols=64):
+        return lib.bsgl_evict_tokens(P, P, P, cols, P, cols, 2, cols, P, ctypes.c_void_p(seq), ctypes.c_void_p(new), None, 0, 0, batch, 4, 0, 0, 0, None, 0, None)
+
+    for new in (4096, 4096 - 24, 4096 + 24):
+        assert f(4096, new) == _hip.BSGL_ERR_BAD_ARG and b"overlap" in lib.bsgl_last_error()
+    assert f(4096, 8192, cols=2**31 - 5) == _hip.BSGL_ERR_BAD_ARG
+
+
+def test_logits_in_place_keep_their_stride():
+    c = _hip.LogitCall()
+    for k, v in dict(out=256, logits=256, out_row_stride=100, logits_row_stride=104, batch=2, vocab=100, dtype=2).items():
+        setattr(c, k, v)
+    assert lib.bsgl_logit_controls(ctypes.byref(c)) == _hip.BSGL_ERR_BAD_ARG
+
+
 def test_scored_decode_workspace():
     plain = _hip.decode_workspace_bytes(4, 12, 128, 32)  # (up to four times the splits for a long request)
     assert _hip.decode_scored_workspace_bytes(4, 12, 128, 8, 1000, False) == plain
