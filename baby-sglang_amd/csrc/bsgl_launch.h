@@ -348,5 +348,8 @@ hipError_t launch_prefill_mfma32(const PrefillArgs& a, hipStream_t stream);
 // scored extend attention where prefill_scored_supported says so
 bool prefill_scored_supported(const PrefillArgs& a, const char** why);
 hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream);
+// its f32 form, which the two above pick by the type
+bool prefill_scored_f32_supported(const PrefillArgs& a, const char** why);
+hipError_t launch_prefill_scored_f32(const PrefillArgs& a, dim3 grid, hipStream_t stream);
 
 }  // namespace bsgl

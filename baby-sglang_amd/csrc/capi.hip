@@ -748,7 +748,7 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   // against the extend kernel: 16 x 8 tokens over 500 20.8 / 22.6 us, 4 x 16 over 2000 (3.3e7 below) 24.8 / 29.9,
   // 8 x 8 over 1000 (3.3e7) 30.6 / 33.2, 1 x 100 over 2000 (5.4e7) 48 / 28, 16 x 4 over 8192 (1.3e8) 80 / 39.
   const int64_t streamed = (int64_t)total_q_tokens * n_kv_heads * head_dim;
-  const bool few = mods != nullptr && kind == BSGL_DECODE_AUTO && mfma_ok && streamed <= kFewTokens && streamed * table_cols <= kFewStreamed;
+  const bool few = mods != nullptr && dtype != BSGL_DTYPE_F32 && kind == BSGL_DECODE_AUTO && mfma_ok && streamed <= kFewTokens && streamed * table_cols <= kFewStreamed;
   if (kind != BSGL_DECODE_VALU && mfma_ok && !few) {
     ex.row_req = nullptr;  // only the running sums are needed
     if (mods != nullptr) {
@@ -757,7 +757,7 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
       // shorter than 512 tokens of the widest request the page table allows.  512 tokens over 8192, 12 / 2 heads: 190 us in one piece,
       // 116 in two; 64 over 8192 195 and 31 (8 pieces); where there is nothing to stream the merge costs 2 - 4 us (200 over 200: 21).
       int64_t s = 512 / scored_workgroups(pa.blk_rows, total_q_tokens, batch, pa.n_q_heads, pa.n_kv_heads);
-      const int64_t room = prefill_row_splits(total_q_tokens, 1 << 30), by_len = table_cols / 512;
+      const int64_t room = prefill_row_splits(total_q_tokens, 1 << 30), by_len = table_cols / (dtype == BSGL_DTYPE_F32 ? 64 : 512);
       if (s > room) s = room;
       if (s > by_len) s = by_len;
       if (s > 1) {

@@ -711,6 +711,7 @@ void launch_shape(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
 
 // the extend kernels' conditions, with up to 16 q heads per kv head (a workgroup takes them two or eight at a time)
 bool prefill_scored_supported(const PrefillArgs& a, const char** why) {
+  if (a.dtype == kF32) return prefill_scored_f32_supported(a, why);
   // (without a cap the largest score is taken to be the largest product, and a bias is carried in units of the scale)
   if (!(a.mods.cap > 0.f) && !(a.scale > 1e-30f)) {
     *why = "the matrix-core kernel needs a positive scale";
@@ -730,7 +731,8 @@ hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream) {
   const int64_t n_wg = 8 * local_groups * a.grp_blocks * n_z;
   if (n_wg > 0x7fffffffll) return hipErrorInvalidValue;
   const dim3 grid((unsigned)n_wg, (unsigned)(a.splits > 1 ? a.splits : 1), 1);
-  if (a.dtype == kBF16) a.blk_rows == 64 ? launch_shape<bf16_tag, 32>(a, grid, stream) : launch_shape<bf16_tag, 16>(a, grid, stream);
+  if (a.dtype == kF32) (void)launch_prefill_scored_f32(a, grid, stream);
+  else if (a.dtype == kBF16) a.blk_rows == 64 ? launch_shape<bf16_tag, 32>(a, grid, stream) : launch_shape<bf16_tag, 16>(a, grid, stream);
   else a.blk_rows == 64 ? launch_shape<f16_tag, 32>(a, grid, stream) : launch_shape<f16_tag, 16>(a, grid, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits <= 1) return e;
