@@ -348,6 +348,9 @@ hipError_t launch_prefill_mfma32(const PrefillArgs& a, hipStream_t stream);
 // scored extend attention where prefill_scored_supported says so
 bool prefill_scored_supported(const PrefillArgs& a, const char** why);
 hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream);
+// scored decode of f32 rows; DecodeArgs::counters as for launch_decode_mfma, balance_target unused
+bool decode_scored_f32_supported(const DecodeArgs& a);
+hipError_t launch_decode_scored_f32(const DecodeArgs& a, hipStream_t stream);
 // its f32 form, which the two above pick by the type
 bool prefill_scored_f32_supported(const PrefillArgs& a, const char** why);
 hipError_t launch_prefill_scored_f32(const PrefillArgs& a, dim3 grid, hipStream_t stream);

@@ -139,8 +139,10 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   } else if (variant != BSGL_DECODE_VALU) {
     return fail(BSGL_ERR_BAD_ARG, "unknown decode variant %d", variant);
   }
+  // (uniform pieces keep the sums of the plain decode: a call without a cap, a bias and an interval then agrees with it bit for bit)
+  const bool use_f32 = variant == BSGL_DECODE_AUTO && !use_mfma && !uniform_splits && bsgl::decode_scored_f32_supported(a);
   if (!use_mfma && a.base_splits > 0) a.n_splits = a.base_splits;  // (every row is cut into n_splits equal pieces there)
-  if (!use_mfma && !bsgl::decode_valu_supported(a, &why)) return fail(BSGL_ERR_UNSUPPORTED, "decode: %s", why);
+  if (!use_mfma && !use_f32 && !bsgl::decode_valu_supported(a, &why)) return fail(BSGL_ERR_UNSUPPORTED, "decode: %s", why);
   // KV write of the new tokens: inside the matrix-core kernel when the caller
   // allows it and the rows qualify, otherwise as its own launch first
   if (a.new_loc != nullptr) {
@@ -171,7 +173,7 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   const int32_t wanted = a.base_splits > 0 ? a.base_splits : a.n_splits;
   const bool tickets_fit = (size_t)a.rows * (size_t)a.n_kv_heads * 4 <= kCounterBytes &&
                            (size_t)a.n_splits * a.rows * a.n_q_heads * a.head_dim * 4 < (1ull << 31);
-  a.counters = (use_mfma && tickets_fit && (a.fold_group > 0 || bsgl::knob(bsgl::kKnobNoFusedMerge) == 0)) ? counters : nullptr;
+  a.counters = ((use_mfma || use_f32) && tickets_fit && (a.fold_group > 0 || bsgl::knob(bsgl::kKnobNoFusedMerge) == 0)) ? counters : nullptr;
   if (a.fold_group > 0 && a.counters == nullptr && !bsgl::decode_direct_out(a))
     return fail(BSGL_ERR_UNSUPPORTED, "folded kv heads need the in-kernel merge (batch too large for the ticket area)");
   // length-balanced pieces: needs the in-kernel merge (a row's piece count varies) and a
@@ -179,7 +181,7 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   a.balance_target = 0;
   a.balance_target_hi = 0;
   a.whole_len = 0;
-  if (a.counters != nullptr && a.n_splits > 1 && a.rows <= 1024 && a.kv.table_cols <= (1 << 20) && !uniform_splits && bsgl::knob(bsgl::kKnobDecodeBalance) != 0)
+  if (a.counters != nullptr && !use_f32 && a.n_splits > 1 && a.rows <= 1024 && a.kv.table_cols <= (1 << 20) && !uniform_splits && bsgl::knob(bsgl::kKnobDecodeBalance) != 0)
     a.balance_target = (wanted + 1) / 2;
   if (a.balance_target > 0) {
     // Small batches get many splits, but pieces much shorter than 256 tokens cost more in the merge
@@ -240,7 +242,9 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
     a.balance_target = wanted < cap ? wanted : cap;
     a.balance_target_hi = 0;
   }
-  const hipError_t e = use_mfma ? bsgl::launch_decode_mfma(a, stream) : bsgl::launch_decode_valu(a, stream);
+  const hipError_t e = use_mfma ? bsgl::launch_decode_mfma(a, stream)
+                       : use_f32 ? bsgl::launch_decode_scored_f32(a, stream)
+                                 : bsgl::launch_decode_valu(a, stream);
   if (e != hipSuccess) return hip_fail("decode launch", e);
   return BSGL_OK;
 }

@@ -640,3 +640,59 @@ def test_extend_tiny_scale_with_a_bias(gpu):
                                         scale=scale, slopes=sl.to(gpu))
         want, mass, lse, _, top = orc.scored_exact(c["q"], c["k"], c["v"], c["table"][c["req"]], [100], [0] * 100, range(100), scale, 0.0, sl)
         check_rows(out, want, mass, lse, top + 100.0, 0.0, torch.bfloat16, torch.bfloat16, 2.0**-8, 100, 6.0, 128)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(n_splits=1), dict(n_splits=3), dict(n_splits=64), dict(variant=0x200), dict(variant=1)])
+@pytest.mark.parametrize("heads", ["1.5b", "d64", "7b"])
+def test_decode_f32_launch_forms(gpu, heads, kw):
+    """The matrix-core form in one piece, some and as many as there are, and the generic kernel."""
+    decode_case(gpu, heads, torch.float32, [1, 2, 15, 16, 17, 63, 64, 65, 300, 900], cap=8.0, slopes=True, seed=61, **kw)
+
+
+def test_decode_f32_up_to_16_heads_per_kv_head(gpu):
+    decode_case(gpu, "one", torch.float32, [1, 33, 700], cap=8.0, slopes=True, seed=62)
+    decode_case(gpu, "one", torch.float32, [50, 33, 700], start=[0, 33, 650], stop=[50, 33, 651], seed=63)
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_decode_f32_numbers_that_are_none(gpu, where, bad):
+    """A value that is not finite in the last visible token (which also stands in for the places behind it) spreads as the
+    definition has it and stays in its request."""
+    from baby_sglang_amd import _hip
+
+    c = make(64, "mha", torch.float32, [37, 100])
+    d = to_gpu(c, gpu)
+    clean = _hip.paged_decode_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"]).view(2, 3, 128)
+    d[where][d["table"][d["req"][0], 36].long()] = bad
+    got = _hip.paged_decode_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"]).view(2, 3, 128)
+    assert torch.equal(got[1], clean[1])
+    if where == "v":
+        assert bool(got[0].isinf().all() if bad == float("inf") else got[0].isnan().all())
+    elif bad != bad:
+        assert bool(got[0].isnan().all())
+
+
+def test_decode_f32_more_rows_than_tickets(gpu):
+    """8200 requests of 3 kv heads in two pieces each: their results are merged by a launch of its own."""
+    from baby_sglang_amd import _hip
+
+    r = random.Random(65)
+    lens = [r.randint(1, 3) for _ in range(8200)]
+    lens[4000], lens[8199] = 150, 0
+    g = torch.Generator().manual_seed(65)
+    k, v = (torch.randn(500, 3, 128, generator=g) for _ in range(2))
+    table = torch.randint(0, 500, (8200, 160), generator=g, dtype=torch.int32)
+    q = torch.randn(8200, 3, 128, generator=g)
+    out = _hip.paged_decode_scored(q.to(gpu), k.to(gpu), v.to(gpu), table.to(gpu), torch.arange(8200, device=gpu), torch.tensor(lens, device=gpu),
+                                   logit_cap=9.0, n_splits=2)
+    rows = [0, 4000, 8198, 8199] + r.sample(range(8200), 60)
+    want, mass, lse, _, top = orc.scored_exact(q[rows], k, v, table[rows], [lens[i] for i in rows], range(len(rows)), [lens[i] - 1 for i in rows], 128**-0.5, 9.0)
+    check_rows(out[rows], want, mass, lse, top, 9.0, torch.float32, torch.float32, 0.0, 150, 6.0, 128)
+
+
+@pytest.mark.parametrize("heads", ["1.5b", "0.5b", "one"])
+@pytest.mark.parametrize("ext,prefix", [([1], [0]), ([31, 33, 64, 65], [0, 5, 64, 1]), ([200], [900]), ([3, 0, 1, 2], [1000, 5, 0, 31])])
+def test_extend_f32_blocks_and_pieces(gpu, heads, ext, prefix):
+    for kind in (None, "window", "wild"):
+        extend_case(gpu, heads, torch.float32, ext, prefix, cap=7.0, slopes=True, kind=kind, seed=66)
