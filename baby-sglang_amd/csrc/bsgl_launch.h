@@ -302,8 +302,9 @@ struct EvictArgs {
   // set by launch_evict
   int32_t slices;
   int64_t counts_at, staged_at, staged_row;
+  bool staged;  // the rows are copied into the workspace first
 };
-size_t evict_workspace(int64_t batch, int64_t longest, int32_t budget, int64_t* counts_at, int64_t* staged_at, int64_t* staged_row);
+size_t evict_workspace(int64_t batch, int64_t longest, int64_t* counts_at, int64_t* staged_at, int64_t* staged_row);
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 
 constexpr int kLogitMaxBias = 1 << 12;           // biases per request

@@ -13,8 +13,9 @@
 //                   behind what has been read: the rows may be compacted in place.  Bound by latency: four trips to memory and
 //                   a dozen barriers; the bytes (8 per token) hardly count.
 //   split_* kernels for longer rows (kSplitFrom): a row is dealt over workgroups of 2048 tokens.  Each pass of the selection
-//                   is a launch; the last workgroup of a row to arrive scans the row's histogram.  In place, the kept entries go
-//                   through the workspace (a workgroup would otherwise write where another has not read yet).
+//                   is a launch; the last workgroup of a row to arrive scans the row's histogram.  In place, the launch that
+//                   clears the histograms also copies the row into the workspace, which everything behind it reads (a workgroup
+//                   would otherwise write where another has not read yet).  Bound by its six launches.
 #include "bsgl_device.h"
 #include "bsgl_launch.h"
 
@@ -311,7 +312,7 @@ struct SplitState {
   uint32_t arrived[3];
   Pick pick[3];  // after each pass
 };
-// behind the batch's states: per request [slices] counts, then [budget] slots and [budget] weights
+// behind the batch's states: per request [slices] counts, then the row's slots and weights
 
 __device__ __forceinline__ SplitState* state_of(const EvictArgs& a, int row) { return (SplitState*)a.workspace + row; }
 __device__ __forceinline__ int2* counts_of(const EvictArgs& a, int row) {
@@ -321,9 +322,32 @@ __device__ __forceinline__ int32_t* staged_of(const EvictArgs& a, int row) {
   return (int32_t*)((char*)a.workspace + a.staged_at) + (int64_t)row * 2 * a.staged_row;
 }
 
-__global__ __launch_bounds__(kNT) void split_clear_kernel(EvictArgs a) {
-  uint32_t* dst = (uint32_t*)state_of(a, blockIdx.y);
+__global__ __launch_bounds__(kNT) void split_start_kernel(EvictArgs a) {
+  const int row = blockIdx.y;
+  uint32_t* dst = (uint32_t*)state_of(a, row);
   for (int i = blockIdx.x * kNT + threadIdx.x; i < (int)(sizeof(SplitState) / 4); i += gridDim.x * kNT) dst[i] = 0;
+  if (!a.staged) return;
+  const Row r = take_row<kNT>(a, row);
+  const int base = blockIdx.x * kSlice;
+  if (!r.mine || r.n <= a.budget || base >= r.n) return;
+  int32_t* t = staged_of(a, row);
+  float* w = (float*)(t + a.staged_row);
+  const int end = min(r.n, base + kSlice);
+  for (int i = base + (int)threadIdx.x; i < end; i += kNT) {
+    t[i] = r.t_in[i];
+    w[i] = r.w_in[i];
+  }
+}
+
+// a row of the kernels behind that one, if it is to be cut: read from its copy where there is one
+__device__ __forceinline__ Row take_staged_row(const EvictArgs& a, int row) {
+  Row r = take_row<kNT>(a, row);
+  if (a.staged && r.n > a.budget) {
+    r.t_in = staged_of(a, row);
+    r.w_in = (const float*)(r.t_in + a.staged_row);
+    r.rows16 = true;
+  }
+  return r;
 }
 
 // the selection as it stood before `pass`
@@ -341,7 +365,7 @@ __global__ __launch_bounds__(kNT) void split_pass_kernel(EvictArgs a, int pass) 
   const int row = blockIdx.y;
   const int base = blockIdx.x * kSlice;
   for (int i = tid; i < kBins; i += kNT) s_hist[i] = 0;
-  const Row r = take_row<kNT>(a, row);
+  const Row r = take_staged_row(a, row);
   SplitState* st = state_of(a, row);
   const Pick before = pick_before(st, r, pass);
   // (nothing to select, or the selection has ended: the same for every workgroup of the row)
@@ -383,7 +407,7 @@ __global__ __launch_bounds__(kNT) void split_count_kernel(EvictArgs a) {
   __shared__ int2 s_wave[kNT / 64];
   const int row = blockIdx.y;
   const int base = blockIdx.x * kSlice;
-  const Row r = take_row<kNT>(a, row);
+  const Row r = take_staged_row(a, row);
   if (!r.mine || r.n <= a.budget || base >= r.n) return;
   const Pick p = r.m > 0 ? state_of(a, row)->pick[2] : Pick{0, 0, 0, false};
   float w[kV];
@@ -401,13 +425,13 @@ __global__ __launch_bounds__(kNT) void split_count_kernel(EvictArgs a) {
   }
 }
 
-__global__ __launch_bounds__(kNT) void split_deal_kernel(EvictArgs a, bool staged) {
+__global__ __launch_bounds__(kNT) void split_deal_kernel(EvictArgs a) {
   __shared__ int2 s_wave[kNT / 64];
   __shared__ int2 s_before[kNT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.y;
   const int base = blockIdx.x * kSlice;
-  const Row r = take_row<kNT>(a, row);
+  const Row r = take_staged_row(a, row);
   const int n = r.n;
   const int n_gone = r.mine ? n - r.n_keep : 0;
   if (blockIdx.x == 0 && tid == 0) a.new_lens[row] = r.n_keep;
@@ -452,34 +476,16 @@ __global__ __launch_bounds__(kNT) void split_deal_kernel(EvictArgs a, bool stage
     kept += s_wave[v].x + equals_kept(eq, s_wave[v].y, p.left);
     eq += s_wave[v].y;
   }
-  int32_t* t_out = r.t_out;
-  float* w_out = r.w_out;
-  if (staged) {
-    t_out = staged_of(a, row);
-    w_out = (float*)(t_out + a.staged_row);
-  }
-  deal_out<kNT, kV>(w, slot, r, p, base, kept, eq, t_out, w_out, a.evicted_cols);
-}
-
-__global__ __launch_bounds__(kNT) void split_copy_kernel(EvictArgs a) {
-  const int row = blockIdx.y;
-  const Row r = take_row<kNT>(a, row);
-  if (!r.mine || r.n <= a.budget) return;
-  const int32_t* t = staged_of(a, row);
-  const float* w = (const float*)(t + a.staged_row);
-  for (int64_t i = (int64_t)blockIdx.x * kNT + threadIdx.x; i < r.n_keep; i += (int64_t)gridDim.x * kNT) {
-    r.t_out[i] = t[i];
-    r.w_out[i] = w[i];
-  }
+  deal_out<kNT, kV>(w, slot, r, p, base, kept, eq, r.t_out, r.w_out, a.evicted_cols);
 }
 
 }  // namespace
 
 // Rows longer than kSplitFrom are split; the workspace is for them.
-size_t evict_workspace(int64_t batch, int64_t longest, int32_t budget, int64_t* counts_at, int64_t* staged_at, int64_t* staged_row) {
+size_t evict_workspace(int64_t batch, int64_t longest, int64_t* counts_at, int64_t* staged_at, int64_t* staged_row) {
   if (longest <= kSplitFrom || batch <= 0) return 0;
   const int64_t slices = (longest + kSlice - 1) / kSlice;
-  const int64_t row = ((budget < longest ? budget : longest) + 63) / 64 * 64;
+  const int64_t row = (longest + 63) / 64 * 64;
   const int64_t counts = (batch * (int64_t)sizeof(SplitState) + 255) / 256 * 256;
   const int64_t staged = counts + (batch * slices * 8 + 255) / 256 * 256;
   if (counts_at != nullptr) *counts_at = counts;
@@ -492,16 +498,15 @@ hipError_t launch_evict(const EvictArgs& a_in, hipStream_t stream) {
   EvictArgs a = a_in;
   if (a.batch == 0) return hipSuccess;
   if (a.longest > kSplitFrom) {
-    // one workgroup takes 1.2 us per 1000 tokens there, the split form's six launches 20 - 25 us whatever the length
+    // one workgroup takes 1.2 us per 1000 tokens there, the split form's six launches some 20 us whatever the length
     a.slices = (int32_t)((a.table_cols + kSlice - 1) / kSlice);  // (a hint that is too small must not cost a token)
-    evict_workspace(a.batch, a.table_cols, a.budget, &a.counts_at, &a.staged_at, &a.staged_row);
-    const bool staged = a.out_table == a.table || a.out_weights == a.weights;
+    evict_workspace(a.batch, a.table_cols, &a.counts_at, &a.staged_at, &a.staged_row);
+    a.staged = a.out_table == a.table || a.out_weights == a.weights;
     const dim3 grid((unsigned)a.slices, (unsigned)a.batch);
-    hipLaunchKernelGGL(split_clear_kernel, dim3(4, (unsigned)a.batch), dim3(kNT), 0, stream, a);
+    hipLaunchKernelGGL(split_start_kernel, grid, dim3(kNT), 0, stream, a);
     for (int pass = 0; pass < 3; ++pass) hipLaunchKernelGGL(split_pass_kernel, grid, dim3(kNT), 0, stream, a, pass);
     hipLaunchKernelGGL(split_count_kernel, grid, dim3(kNT), 0, stream, a);
-    hipLaunchKernelGGL(split_deal_kernel, grid, dim3(kNT), 0, stream, a, staged);
-    if (staged) hipLaunchKernelGGL(split_copy_kernel, dim3((unsigned)((a.staged_row + kSlice - 1) / kSlice), (unsigned)a.batch), dim3(kNT), 0, stream, a);
+    hipLaunchKernelGGL(split_deal_kernel, grid, dim3(kNT), 0, stream, a);
     return hipGetLastError();
   }
   const dim3 grid((unsigned)a.batch);
