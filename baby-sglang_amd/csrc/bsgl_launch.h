@@ -88,9 +88,10 @@ struct DecodeArgs {
   int32_t dtype;
   int32_t out_dtype;  // dtype, or kF32 (then results always pass through the merge kernel)
   int32_t n_splits;
-  // scored form, > 0: pieces wanted per request as if n_splits were this (n_splits itself then only bounds how finely
-  // the longest requests may be cut); what the kernels that cut every request alike use
+  // scored form, > 0: pieces wanted per request of a batch of one length (n_splits itself then only bounds how finely
+  // the longest requests may be cut); what the launches that cut every request alike use
   int32_t base_splits;
+  bool uniform;       // scored form: every request into n_splits pieces
   float* ws_o;    // [n_splits, rows * n_q_heads, head_dim]   (unless direct)
   float* ws_lse;  // [n_splits, rows * n_q_heads]
   uint32_t* counters;  // [rows, head groups] tickets of the in-kernel merge; zero between launches; may be NULL
@@ -122,6 +123,7 @@ struct DecodeArgs {
   // configuration only): 8 x uint64 per workgroup (in launch order): start, after
   // the prologue, after the streaming loop, end (100 MHz ticks), XCC id, HW id, row, piece
   uint64_t* trace;
+  int32_t piece_len;  // set by launch_decode_scored: no piece of a request that is cut is wanted shorter
   bool scored;  // the scored forms of the kernels, with these:
   ScoreMods mods;
 };
@@ -349,9 +351,9 @@ hipError_t launch_prefill_mfma32(const PrefillArgs& a, hipStream_t stream);
 // scored extend attention where prefill_scored_supported says so
 bool prefill_scored_supported(const PrefillArgs& a, const char** why);
 hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream);
-// scored decode of f32 rows; DecodeArgs::counters as for launch_decode_mfma, balance_target unused
-bool decode_scored_f32_supported(const DecodeArgs& a);
-hipError_t launch_decode_scored_f32(const DecodeArgs& a, hipStream_t stream);
+// scored decode; DecodeArgs::counters as for launch_decode_mfma
+bool decode_scored_supported(const DecodeArgs& a);
+hipError_t launch_decode_scored(const DecodeArgs& a, hipStream_t stream);
 // its f32 form, which the two above pick by the type
 bool prefill_scored_f32_supported(const PrefillArgs& a, const char** why);
 hipError_t launch_prefill_scored_f32(const PrefillArgs& a, dim3 grid, hipStream_t stream);

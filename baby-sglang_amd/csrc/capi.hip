@@ -109,6 +109,28 @@ int check_paged(const void* out, int64_t out_row_stride, const void* q, int64_t 
 // does not move when one workspace serves calls of different batch sizes
 constexpr size_t kCounterBytes = 65536;
 
+// the new tokens' K/V rows into the slabs, ahead of the attention launch
+int write_new_rows(bsgl::DecodeArgs& a, hipStream_t stream) {
+  const int eb = bsgl::dtype_bytes(a.dtype);
+  bsgl::ScatterArgs sc;
+  sc.k_slab = const_cast<void*>(a.kv.k_slab);
+  sc.v_slab = const_cast<void*>(a.kv.v_slab);
+  sc.slab_row_stride = a.kv.slab_row_stride;
+  sc.n_slots = a.kv.n_slots;
+  sc.loc = a.new_loc;
+  sc.k_new = a.k_new;
+  sc.v_new = a.v_new;
+  sc.k_row_stride = a.k_new_stride;
+  sc.v_row_stride = a.v_new_stride;
+  sc.n_tok = a.rows;
+  sc.row_bytes = a.n_kv_heads * a.head_dim * eb;
+  sc.elem_bytes = eb;
+  const hipError_t es = bsgl::launch_kv_scatter(sc, stream);
+  if (es != hipSuccess) return hip_fail("kv_scatter launch", es);
+  a.new_loc = nullptr;
+  return BSGL_OK;
+}
+
 int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStream_t stream) {
   const char* why = "";
   bool use_mfma = false;
@@ -139,10 +161,7 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   } else if (variant != BSGL_DECODE_VALU) {
     return fail(BSGL_ERR_BAD_ARG, "unknown decode variant %d", variant);
   }
-  // (uniform pieces keep the sums of the plain decode: a call without a cap, a bias and an interval then agrees with it bit for bit)
-  const bool use_f32 = variant == BSGL_DECODE_AUTO && !use_mfma && !uniform_splits && bsgl::decode_scored_f32_supported(a);
-  if (!use_mfma && a.base_splits > 0) a.n_splits = a.base_splits;  // (every row is cut into n_splits equal pieces there)
-  if (!use_mfma && !use_f32 && !bsgl::decode_valu_supported(a, &why)) return fail(BSGL_ERR_UNSUPPORTED, "decode: %s", why);
+  if (!use_mfma && !bsgl::decode_valu_supported(a, &why)) return fail(BSGL_ERR_UNSUPPORTED, "decode: %s", why);
   // KV write of the new tokens: inside the matrix-core kernel when the caller
   // allows it and the rows qualify, otherwise as its own launch first
   if (a.new_loc != nullptr) {
@@ -150,30 +169,13 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
     const bool rows_ok = (((uintptr_t)a.k_new | (uintptr_t)a.v_new) % 256 == 0) &&
                          (a.k_new_stride * eb) % 256 == 0 && (a.v_new_stride * eb) % 256 == 0;
     if (!(use_mfma && may_fuse_kv && rows_ok && bsgl::knob(bsgl::kKnobNoFusedKV) == 0)) {
-      bsgl::ScatterArgs sc;
-      sc.k_slab = const_cast<void*>(a.kv.k_slab);
-      sc.v_slab = const_cast<void*>(a.kv.v_slab);
-      sc.slab_row_stride = a.kv.slab_row_stride;
-      sc.n_slots = a.kv.n_slots;
-      sc.loc = a.new_loc;
-      sc.k_new = a.k_new;
-      sc.v_new = a.v_new;
-      sc.k_row_stride = a.k_new_stride;
-      sc.v_row_stride = a.v_new_stride;
-      sc.n_tok = a.rows;
-      sc.row_bytes = a.n_kv_heads * a.head_dim * eb;
-      sc.elem_bytes = eb;
-      const hipError_t es = bsgl::launch_kv_scatter(sc, stream);
-      if (es != hipSuccess) return hip_fail("kv_scatter launch", es);
-      a.new_loc = nullptr;
+      if (int rc = write_new_rows(a, stream)) return rc;
     }
   }
   // one ticket per (row, kv head): fall back to the merge kernel when they do not fit
-  if (a.base_splits > 0 && ((size_t)a.n_splits * a.rows * a.n_q_heads * a.head_dim * 4 >= (1ull << 31) || a.rows > 1024)) a.n_splits = a.base_splits;
-  const int32_t wanted = a.base_splits > 0 ? a.base_splits : a.n_splits;
   const bool tickets_fit = (size_t)a.rows * (size_t)a.n_kv_heads * 4 <= kCounterBytes &&
                            (size_t)a.n_splits * a.rows * a.n_q_heads * a.head_dim * 4 < (1ull << 31);
-  a.counters = ((use_mfma || use_f32) && tickets_fit && (a.fold_group > 0 || bsgl::knob(bsgl::kKnobNoFusedMerge) == 0)) ? counters : nullptr;
+  a.counters = (use_mfma && tickets_fit && (a.fold_group > 0 || bsgl::knob(bsgl::kKnobNoFusedMerge) == 0)) ? counters : nullptr;
   if (a.fold_group > 0 && a.counters == nullptr && !bsgl::decode_direct_out(a))
     return fail(BSGL_ERR_UNSUPPORTED, "folded kv heads need the in-kernel merge (batch too large for the ticket area)");
   // length-balanced pieces: needs the in-kernel merge (a row's piece count varies) and a
@@ -181,8 +183,8 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   a.balance_target = 0;
   a.balance_target_hi = 0;
   a.whole_len = 0;
-  if (a.counters != nullptr && !use_f32 && a.n_splits > 1 && a.rows <= 1024 && a.kv.table_cols <= (1 << 20) && !uniform_splits && bsgl::knob(bsgl::kKnobDecodeBalance) != 0)
-    a.balance_target = (wanted + 1) / 2;
+  if (a.counters != nullptr && a.n_splits > 1 && a.rows <= 1024 && a.kv.table_cols <= (1 << 20) && !uniform_splits && bsgl::knob(bsgl::kKnobDecodeBalance) != 0)
+    a.balance_target = (a.n_splits + 1) / 2;
   if (a.balance_target > 0) {
     // Small batches get many splits, but pieces much shorter than 256 tokens cost more in the merge
     // than they gain (a piece can be shared by up to four waves instead): no more pieces than
@@ -200,7 +202,7 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
     // slower that way at 3000 - 4095 tokens.)
     if (a.rows > 2 && (int64_t)a.rows * a.n_kv_heads <= 16) {
       const int64_t fine = a.kv.table_cols / 256;
-      const int64_t hi = fine < (wanted + 1) / 2 ? fine : (wanted + 1) / 2;
+      const int64_t hi = fine < (a.n_splits + 1) / 2 ? fine : (a.n_splits + 1) / 2;
       if (hi > a.balance_target) a.balance_target_hi = (int32_t)hi;
     }
     // (where a piece is shared by four waves: 256 pieces or fewer, as launch_decode_mfma decides)
@@ -239,13 +241,35 @@ int run_decode(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
   // -- and with half as many kv heads to cut, up to n_splits pieces are wanted below that
   if (a.fold_group > 0 && a.balance_target > 0 && a.hint_waves == 0) {
     const int cap = bsgl::knob(bsgl::kKnobFoldPieces);
-    a.balance_target = wanted < cap ? wanted : cap;
+    a.balance_target = a.n_splits < cap ? a.n_splits : cap;
     a.balance_target_hi = 0;
   }
-  const hipError_t e = use_mfma ? bsgl::launch_decode_mfma(a, stream)
-                       : use_f32 ? bsgl::launch_decode_scored_f32(a, stream)
-                                 : bsgl::launch_decode_valu(a, stream);
+  const hipError_t e = use_mfma ? bsgl::launch_decode_mfma(a, stream) : bsgl::launch_decode_valu(a, stream);
   if (e != hipSuccess) return hip_fail("decode launch", e);
+  return BSGL_OK;
+}
+
+// Scored decode: requests, or extend tokens (ScoreMods::rows).  base_splits: as many pieces as the caller asked for, for requests of
+// one length; n_splits: the most a long one among short ones may be cut into.
+int run_scored(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStream_t stream) {
+  const char* why = "needs 1..16 query heads per kv head of 64 or 128 values and 16-byte aligned rows";
+  const int32_t kind = variant & 0xff;
+  if (kind != BSGL_DECODE_AUTO && kind != BSGL_DECODE_VALU && kind != BSGL_DECODE_MFMA) return fail(BSGL_ERR_BAD_ARG, "unknown decode variant %d", kind);
+  const bool direct = kind != BSGL_DECODE_VALU && bsgl::decode_scored_supported(a);
+  if (kind == BSGL_DECODE_MFMA && !direct) return fail(BSGL_ERR_UNSUPPORTED, "matrix-core scored decode %s", why);
+  if (!direct && !bsgl::decode_valu_supported(a, &why)) return fail(BSGL_ERR_UNSUPPORTED, "scored decode: %s", why);
+  if (a.new_loc != nullptr && !(direct && (variant & BSGL_DECODE_FUSE_KV_WRITE) != 0 && bsgl::knob(bsgl::kKnobNoFusedKV) == 0)) {
+    if (int rc = write_new_rows(a, stream)) return rc;
+  }
+  // in-kernel merge: one ticket per (row, kv head), partial rows within 31 bits of each other
+  auto fits = [&](int32_t splits) { return (size_t)splits * a.rows * a.n_q_heads * a.head_dim * 4 < (1ull << 31); };
+  if (a.base_splits > 0 && !fits(a.n_splits)) a.n_splits = a.base_splits;
+  const bool tickets = direct && (size_t)a.rows * (size_t)a.n_kv_heads * 4 <= kCounterBytes && fits(a.n_splits) && bsgl::knob(bsgl::kKnobNoFusedMerge) == 0;
+  a.counters = tickets ? counters : nullptr;
+  if (a.counters == nullptr && a.base_splits > 0) a.n_splits = a.base_splits;  // (every row is cut into n_splits equal pieces then)
+  a.uniform = (variant & BSGL_DECODE_UNIFORM_SPLITS) != 0;
+  const hipError_t e = direct ? bsgl::launch_decode_scored(a, stream) : bsgl::launch_decode_valu(a, stream);
+  if (e != hipSuccess) return hip_fail("scored decode launch", e);
   return BSGL_OK;
 }
 
@@ -411,9 +435,7 @@ int take_mods(bsgl::DecodeArgs& a, const bsgl_score_mods& m) {
 size_t scored_head_bytes(size_t decode_need) { return align_up(decode_need > kCounterBytes ? decode_need : kCounterBytes, 256); }
 // The most pieces a request of a scored call may be cut into.  n_splits is made for requests of one length; visible
 // intervals (documents, windows) make the lengths of a batch differ far more, and the longest request, cut into
-// n_splits pieces, then sets the time of the launch: 96 requests, 4 kv heads, visible lengths 1 - 4095 (mean 730):
-// 46 us with 6 pieces at most, 38 with 24.  Which requests get them is the kernel's rule (pieces of one length); batches of
-// one length are cut as before.
+// n_splits pieces, then sets the time of the launch.  Which requests get them is the kernel's rule (pieces of one length).
 int32_t scored_splits(int32_t n_splits) { return n_splits <= 1 ? n_splits : n_splits < 16 ? 4 * n_splits : 64; }
 int64_t score_row(int64_t table_cols) { return (table_cols + 15) / 16 * 16; }
 
@@ -455,6 +477,10 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
   if (f32_out && (((uintptr_t)out & 15u) || (out_row_stride * 4) % 16))
     return fail(BSGL_ERR_BAD_ARG, "f32 out must be 16-byte aligned with a 16-byte-multiple row stride");
   const int32_t asked_splits = n_splits;
+  // nothing that a score goes through, cut as the caller says: the plain decode, bit for bit
+  if (mods != nullptr && (variant & BSGL_DECODE_UNIFORM_SPLITS) != 0 && mods->logit_cap == 0.f && mods->slopes == nullptr && mods->visible_from == nullptr &&
+      mods->visible_to == nullptr && mods->token_weights == nullptr)
+    mods = nullptr;
   a.base_splits = 0;
   if (mods != nullptr && (variant & BSGL_DECODE_UNIFORM_SPLITS) == 0) {
     a.base_splits = n_splits;
@@ -538,7 +564,8 @@ int decode_entry(void* out, int64_t out_row_stride, float* lse, const void* q, i
     w.len_hint = a.len_hint;
     w.mods = a.mods;
   }
-  const int rc = run_decode(a, variant, need ? (uint32_t*)workspace : nullptr, (hipStream_t)stream);
+  const int rc = mods != nullptr ? run_scored(a, variant, need ? (uint32_t*)workspace : nullptr, (hipStream_t)stream)
+                                 : run_decode(a, variant, need ? (uint32_t*)workspace : nullptr, (hipStream_t)stream);
   if (rc != BSGL_OK || w.out == nullptr) return rc;
   const hipError_t ew = bsgl::launch_token_weights(w, (hipStream_t)stream);
   if (ew != hipSuccess) return hip_fail("token weight launch", ew);
@@ -818,7 +845,8 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   const size_t cb = kCounterBytes;
   a.ws_o = (float*)(ws + cb);
   a.ws_lse = splits > 1 ? (float*)(ws + cb + align_up((size_t)splits * rh * partial_row_width(head_dim) * 4, 256)) : nullptr;
-  if (few) return run_decode(a, BSGL_DECODE_AUTO, splits > 1 ? (uint32_t*)ws : nullptr, (hipStream_t)stream);
+  if (few) return run_scored(a, BSGL_DECODE_AUTO, splits > 1 ? (uint32_t*)ws : nullptr, (hipStream_t)stream);
+  if (mods != nullptr) return run_scored(a, kind, nullptr, (hipStream_t)stream);
   return run_decode(a, BSGL_DECODE_VALU, nullptr, (hipStream_t)stream);
 }
 

@@ -51,16 +51,9 @@
 // are zero before and after every launch.  (Drawing the ticket early and letting
 // the last drawer wait for a "ready" count was measured and is slower: under
 // load every trip to memory costs about 2.3 us, and the wait adds trips.)
-//
-// Scored form (SCORED, DecodeArgs::mods): the scores go through cap * tanh(s / cap), minus slope[head] * distance,
-// and a row sees the positions [from, to) of its request only.  The interval is cut out before anything else
-// -- a row's length is to - from and its page-table row starts at `from` -- so tokens outside it are never
-// read, whatever they hold.  The finished scores can be kept (mods.scores, 16 bytes per lane and tile) for
-// token_weights.hip.  A build of its own: the plain form's code is what it was.
 #include "bsgl_device.h"
 #include "bsgl_launch.h"
 #include "bsgl_mfma.h"
-#include "bsgl_score.h"
 
 #include <type_traits>
 
@@ -89,7 +82,7 @@ __device__ __forceinline__ int small_div(int x, int d) {
 // ring of its own -- a wave's tile rate is set by its 8 LDS-DMA instructions per tile, so W waves
 // stream a piece W times as fast -- and wave 0 adds up their (m, l, O) in LDS before the piece's
 // result is stored, so the number of parts the split merge sees does not grow.
-template <typename Tag, int HPT, int NSTAGE, bool NT, int W = 1, bool TRACE = false, bool SCORED = false>
+template <typename Tag, int HPT, int NSTAGE, bool NT, int W = 1, bool TRACE = false>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2)))
 void decode_mfma_kernel(DecodeArgs a) {
   using E = Elem<Tag>;
@@ -132,33 +125,16 @@ void decode_mfma_kernel(DecodeArgs a) {
   int flat_req = -1, flat_seq = 0;  // the row's page-table row and length, when found by the flat search
   // flat grid: lane i's request length and page-table row, requested first so that the
   // lane-only arithmetic below runs while they travel
-  const int32_t* const rows4 = SCORED ? (const int32_t*)a.mods.rows : nullptr;  // (scored form) four words per row, or NULL
   auto len_of = [&](int i) {
-    int64_t s64 = 0;
-    if (i < a.rows) s64 = SCORED && rows4 != nullptr ? (int64_t)rows4[4 * i + 1] : a.seq_lens[i];
+    const int64_t s64 = i < a.rows ? a.seq_lens[i] : 0;
     const int64_t cap = a.kv.table_cols < (1 << 20) ? a.kv.table_cols : (1 << 20);
     return (int)(s64 < 0 ? 0 : (s64 > cap ? cap : s64));
   };
-  // (scored form) the first visible position of a request, where its length is cut down to the visible ones
-  auto cut_len = [&](int i, int& s) {
-    if constexpr (SCORED) {
-      const int j = i < a.rows ? i : 0;
-      int to = s;
-      if (rows4 != nullptr) to = min(s, rows4[4 * j + 2] + 1);
-      const int2 seen = visible_range(a.mods, j, s, to);
-      s = i < a.rows ? seen.y : 0;
-      return seen.x;
-    } else {
-      return 0;
-    }
-  };
   auto req_of = [&](int i) {
-    int64_t r64 = 0;
-    if (i < a.rows) r64 = SCORED && rows4 != nullptr ? (int64_t)rows4[4 * i] : a.req_idx[i];
+    const int64_t r64 = i < a.rows ? a.req_idx[i] : 0;
     return (int)(r64 < 0 ? 0 : (r64 >= a.kv.table_rows ? a.kv.table_rows - 1 : r64));
   };
-  int len0 = 0, req0 = 0, low0 = 0;
-  int row_first = 0;  // (scored form) the first position the row sees
+  int len0 = 0, req0 = 0;
   if (a.balance_target > 0) {
 #ifdef BSGL_CUT_KNOWN_LEN
     // timing experiment (tools/phase_cut.sh, CUTS=KNOWN_LEN=2048; only right for a batch of that one
@@ -169,7 +145,6 @@ void decode_mfma_kernel(DecodeArgs a) {
 #else
     len0 = len_of(lane);
     req0 = req_of(lane);
-    low0 = cut_len(lane, len0);
 #endif
   }
   const int lq = lane & 15;   // q head (column of S^T / row of O) or d column
@@ -228,12 +203,10 @@ void decode_mfma_kernel(DecodeArgs a) {
       n_parts = parts;
       flat_seq = len_first;
       flat_req = __builtin_amdgcn_readlane(req0, row);
-      if constexpr (SCORED) row_first = __builtin_amdgcn_readlane(low0, row);
     } else {
     int tot = 0, longest = 0;
     for (int r0 = 0; r0 < a.rows; r0 += 64) {
-      int s = r0 == 0 ? len0 : len_of(r0 + lane);
-      if (SCORED && r0 != 0) cut_len(r0 + lane, s);
+      const int s = r0 == 0 ? len0 : len_of(r0 + lane);
       tot += __builtin_amdgcn_readlane(wave_inclusive_scan<ScanAdd>(s), 63);
       longest = max(longest, __builtin_amdgcn_readlane(wave_inclusive_scan<ScanMax>(s), 63));
     }
@@ -254,9 +227,7 @@ void decode_mfma_kernel(DecodeArgs a) {
       int base = 0;
       row = -1;
       for (int r0 = 0; r0 < a.rows; r0 += 64) {
-        int s = r0 == 0 ? len0 : len_of(r0 + lane);
-        int low = low0;
-        if (SCORED && r0 != 0) low = cut_len(r0 + lane, s);
+        const int s = r0 == 0 ? len0 : len_of(r0 + lane);
         const int parts = r0 + lane >= a.rows ? 0 : s <= a.whole_len ? 1 : min(a.n_splits, max(1, small_div(s + piece_len - 1, piece_len)));
         const int incl = wave_inclusive_scan<ScanAdd>(parts);
         const int blk_total = __builtin_amdgcn_readlane(incl, 63);
@@ -269,7 +240,6 @@ void decode_mfma_kernel(DecodeArgs a) {
           n_parts = __builtin_amdgcn_readlane(parts, src);
           flat_seq = __builtin_amdgcn_readlane(s, src);
           flat_req = __builtin_amdgcn_readlane(r0 == 0 ? req0 : req_of(r0 + lane), src);
-          if constexpr (SCORED) row_first = __builtin_amdgcn_readlane(low, src);
         }
         base += blk_total;
       }
@@ -296,19 +266,17 @@ void decode_mfma_kernel(DecodeArgs a) {
     req = flat_req;
     seq = flat_seq;
   } else {
-    const bool listed = SCORED && rows4 != nullptr;
-    req = listed ? (int64_t)rows4[4 * row] : a.req_idx[row];
+    req = a.req_idx[row];
     req = req < 0 ? 0 : (req >= a.kv.table_rows ? a.kv.table_rows - 1 : req);
-    const int64_t seq64 = listed ? (int64_t)rows4[4 * row + 1] : a.seq_lens[row];
+    const int64_t seq64 = a.seq_lens[row];
     seq = (int)(seq64 < 0 ? 0 : (seq64 > a.kv.table_cols ? a.kv.table_cols : seq64));
-    row_first = cut_len(row, seq);
   }
   // the row's pieces are equal among themselves (a piece past the end is empty)
   int chunk = a.balance_target > 0 ? small_div(seq + n_parts - 1, n_parts) : (seq + n_parts - 1) / n_parts;  // (flat grid: seq <= 2^20)
   chunk = (chunk + kTile - 1) / kTile * kTile;
   const int start = split * chunk;
   const int end = (split == n_parts - 1) ? seq : min(seq, start + chunk);
-  const int32_t* table_row = a.kv.table + req * a.kv.table_row_stride + (SCORED ? row_first : 0);
+  const int32_t* table_row = a.kv.table + req * a.kv.table_row_stride;
   const uint32_t max_slot = (uint32_t)(a.kv.n_slots - 1);
   const uint32_t row_units = (uint32_t)(a.kv.slab_row_stride * 2 / 16);
 
@@ -355,28 +323,6 @@ void decode_mfma_kernel(DecodeArgs a) {
       }
   }
   const float scale_log2e = a.scale * kLog2e;
-  ScoreShape shape[HPT];  // (scored form) one q head per lane
-  float* score_dst[HPT];
-  float far = 0.f;  // distance of the first visible token
-  if constexpr (SCORED) {
-    // (only the bias needs it, and no address depends on it: it travels beside the first requests)
-    int pos;
-    if (rows4 != nullptr) {
-      if (rows4[4 * row + 3] == 0) return;  // (all of the row's pieces: no ticket is drawn)
-      pos = rows4[4 * row + 2];
-    } else {
-      const int64_t s64 = a.seq_lens[row];
-      pos = (int)(s64 < 0 ? 0 : (s64 > a.kv.table_cols ? a.kv.table_cols : s64)) - 1;
-    }
-    far = (float)(pos - row_first);
-#pragma unroll
-    for (int hh = 0; hh < HPT; ++hh) {
-      const int h = (head0 + hh) * G + min(lq, G - 1);
-      shape[hh] = ScoreShape(a.mods, a.scale, h);
-      score_dst[hh] = a.mods.scores == nullptr ? nullptr
-                                               : a.mods.scores + ((int64_t)row * a.n_q_heads + h) * a.mods.score_stride + 4 * lg;
-    }
-  }
 
   // ---- per-lane DMA source: which piece of a token record this lane moves ----------
   const int piece = lane % (REC / 16);             // 16-byte piece inside the record
@@ -479,21 +425,15 @@ void decode_mfma_kernel(DecodeArgs a) {
     for (int t = 0; t < NSTAGE - 1; ++t)
       if (wave + t * W < n_tiles) issue_tile(wave + t * W);
 
-    bool stored = false;  // (scored form) the tile before this one left a store behind
     for (int tile = wave; tile < n_tiles; tile += W) {
       const int ahead = (n_tiles - 1 - tile) / W;  // this wave's tiles after this one (capped below)
       if (ahead >= NSTAGE - 1) {
         issue_tile(tile + (NSTAGE - 1) * W);
-        // (a score store of the tile before counts in vmcnt between this tile's requests and the next one's; operations
-        // retire in order, so it may stay out as well)
-        if (SCORED && NSTAGE == 2 && HPT == 1 && stored) dma_wait<DMA_PER_TILE + 1>();
-        else dma_wait<(NSTAGE - 1) * DMA_PER_TILE>();
+        dma_wait<(NSTAGE - 1) * DMA_PER_TILE>();
       } else if (NSTAGE > 3 && ahead == 2) {
         dma_wait<2 * DMA_PER_TILE>();
       } else if (NSTAGE > 2 && ahead == 1) {
         dma_wait<1 * DMA_PER_TILE>();
-      } else if (SCORED && NSTAGE == 2 && HPT == 1 && stored) {
-        dma_wait<1>();
       } else {
         dma_wait<0>();
       }
@@ -513,18 +453,8 @@ void decode_mfma_kernel(DecodeArgs a) {
         float tmax = kNegInf;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if constexpr (SCORED) {
-            const int t = blk + tile * kTile + 4 * lg + r;  // token of the visible ones
-            sv[r] = (4 * lg + r < n_valid) ? shape[hh].fast(sc[r], fabsf(far - (float)t)) : kNegInf;
-          } else {
-            sv[r] = (4 * lg + r < n_valid) ? sc[r] * scale_log2e : kNegInf;
-          }
+          sv[r] = (4 * lg + r < n_valid) ? sc[r] * scale_log2e : kNegInf;
           tmax = fmaxf(tmax, sv[r]);
-        }
-        if constexpr (SCORED) {
-          // the tile's finished scores, four tokens of a head per lane (a row of the buffer has room for whole tiles)
-          stored = score_dst[hh] != nullptr;
-          if (stored && lq < G) *(f32x4*)(score_dst[hh] + blk + tile * kTile) = f32x4{sv[0], sv[1], sv[2], sv[3]};
         }
         tmax = quad_group_max(tmax);
         if (__any(tmax > m_run[hh])) {
@@ -711,9 +641,7 @@ void decode_mfma_kernel(DecodeArgs a) {
   // The weights: lane (head k of a load, part p) = P2 * k + p holds lse and weight of its (head,
   // part), P2 = 8 lanes per head for up to 8 parts (64 otherwise), so one
   // load instruction fetches 64 / P2 heads' values and the maxima and sums run inside P2 lanes.
-  // (inlined whatever the compiler makes of their size: a call would put the whole argument block on the stack, and every wave of
-  // the launch, merging or not, then runs twice as long)
-  auto merge_rows = [&](auto pair_c, auto p2_c) __attribute__((always_inline)) {
+  auto merge_rows = [&](auto pair_c, auto p2_c) {
     constexpr int PAIR = decltype(pair_c)::value;
     constexpr int P2 = decltype(p2_c)::value;
     constexpr int HPI = 64 / P2;  // heads per lse load
@@ -808,7 +736,7 @@ void decode_mfma_kernel(DecodeArgs a) {
       }
     }
   };
-  auto merge_p2 = [&](auto pair_c) __attribute__((always_inline)) {
+  auto merge_p2 = [&](auto pair_c) {
     // (16 lanes per head for 9 - 16 parts was measured too: slower than one head per load)
     if (n_parts <= 8) merge_rows(pair_c, std::integral_constant<int, 8>{});
     else merge_rows(pair_c, std::integral_constant<int, 64>{});
@@ -820,33 +748,6 @@ void decode_mfma_kernel(DecodeArgs a) {
 }
 
 uint64_t* g_trace = nullptr;
-
-// the waves that share a piece: see launch_tag
-int decode_waves(const DecodeArgs& a) {
-  const int64_t n_pieces = (int64_t)a.rows * a.n_kv_heads * (a.balance_target > 0 ? a.balance_target : a.n_splits);
-  int waves = n_pieces > 512 ? 1 : 4;
-  // (folded kv heads keep a wave busier per tile -- up to 16 q heads -- and gain from a second wave a
-  // little longer: 80 - 96 requests of the 0.5B shapes, 1024 / 2048 / 4095 tokens: -8..-11 % / -2..-6 % / +-1 %)
-  if (a.fold_group > 0 && n_pieces > 512 && n_pieces <= 768) waves = 2;
-  if (a.balance_target > 0 && (a.hint_waves == 1 || a.hint_waves == 2 || a.hint_waves == 4)) waves = a.hint_waves;
-  const int forced = knob(kKnobMfmaWaves);  // tuning override
-  if (forced == 1 || forced == 2 || forced == 4) waves = forced;
-  return waves;
-}
-
-// the scored form: the default ring (two stages, non-temporal requests, one kv head per workgroup) in all
-// three widths; the plain form's rules for the launch
-template <typename Tag>
-hipError_t launch_scored(const DecodeArgs& a, hipStream_t stream) {
-  const int waves = decode_waves(a);
-  const int target = waves > 1 ? max(a.balance_target, a.balance_target_hi) : a.balance_target;
-  dim3 grid(a.rows, a.n_kv_heads, a.n_splits);
-  if (a.balance_target > 0) grid = dim3((unsigned)((int64_t)a.rows * (target + 1) * a.n_kv_heads), 1, 1);
-  if (waves == 1) hipLaunchKernelGGL((decode_mfma_kernel<Tag, 1, 2, true, 1, false, true>), grid, dim3(64), 0, stream, a);
-  else if (waves == 2) hipLaunchKernelGGL((decode_mfma_kernel<Tag, 1, 2, true, 2, false, true>), grid, dim3(128), 0, stream, a);
-  else hipLaunchKernelGGL((decode_mfma_kernel<Tag, 1, 2, true, 4, false, true>), grid, dim3(256), 0, stream, a);
-  return hipGetLastError();
-}
 
 template <typename Tag, int HPT, int NSTAGE>
 hipError_t launch_inst(const DecodeArgs& a, hipStream_t stream) {
@@ -879,7 +780,16 @@ hipError_t launch_tag(const DecodeArgs& a, hipStream_t stream) {
   // else four waves share a piece.  (Two waves for 257 - 512 pieces were the rule before; four are
   // 2 - 8 % faster there: 24 requests x 2048 tokens 16.9 -> 15.6 us, 32 requests 17.9 -> 17.6.  Between
   // 512 and 1024 pieces two waves win at 1024 tokens and lose at 2048 and beyond.)
-  const int waves = decode_waves(a);
+  const int64_t n_pieces = (int64_t)a.rows * a.n_kv_heads * (a.balance_target > 0 ? a.balance_target : a.n_splits);
+  int waves = n_pieces > 512 ? 1 : 4;
+  // (folded kv heads keep a wave busier per tile -- up to 16 q heads -- and gain from a second wave a
+  // little longer: 80 - 96 requests of the 0.5B shapes, 1024 / 2048 / 4095 tokens: -8..-11 % / -2..-6 % / +-1 %)
+  if (a.fold_group > 0 && n_pieces > 512 && n_pieces <= 768) waves = 2;
+  if (a.balance_target > 0 && (a.hint_waves == 1 || a.hint_waves == 2 || a.hint_waves == 4)) waves = a.hint_waves;
+  {
+    const int forced = knob(kKnobMfmaWaves);  // tuning override
+    if (forced == 1 || forced == 2 || forced == 4) waves = forced;
+  }
   if (waves > 1 && knob(kKnobMfmaNT)) {
     dim3 grid(a.rows, a.n_kv_heads, a.n_splits);
     if (a.balance_target > 0) grid = dim3((unsigned)((int64_t)a.rows * (max(a.balance_target, a.balance_target_hi) + 1) * a.n_kv_heads), 1, 1);
@@ -925,9 +835,7 @@ hipError_t launch_decode_mfma(const DecodeArgs& a_in, hipStream_t stream) {
   if (a_in.rows == 0) return hipSuccess;
   DecodeArgs a = a_in;
   a.trace = g_trace;
-  hipError_t e;
-  if (a.scored) e = a.dtype == kBF16 ? launch_scored<bf16_tag>(a, stream) : launch_scored<f16_tag>(a, stream);
-  else e = a.dtype == kBF16 ? launch_tag<bf16_tag>(a, stream) : launch_tag<f16_tag>(a, stream);
+  hipError_t e = a.dtype == kBF16 ? launch_tag<bf16_tag>(a, stream) : launch_tag<f16_tag>(a, stream);
   if (e != hipSuccess || decode_direct_out(a) || a.counters != nullptr) return e;
   MergeArgs mg;
   mg.out = a.out;
@@ -940,7 +848,6 @@ hipError_t launch_decode_mfma(const DecodeArgs& a_in, hipStream_t stream) {
   mg.n_heads = a.n_q_heads;
   mg.head_dim = a.head_dim;
   mg.dtype = a.out_dtype;
-  if (a.scored) mg.owned = a.mods.rows;
   return launch_merge(mg, stream);
 }
 
