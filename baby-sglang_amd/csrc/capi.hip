@@ -648,8 +648,8 @@ size_t bsgl_prefill_workspace_bytes(int32_t batch, int32_t total_q_tokens, int32
   return bytes;
 }
 
-static constexpr int64_t kFewTokens = 32768;          // tokens * n_kv_heads * head_dim (at most 512 tokens: the ticket area holds them)
-static constexpr int64_t kFewStreamed = (int64_t)1 << 25;  // ... * page-table columns
+static constexpr int64_t kFewTokens = 65536;  // tokens * n_kv_heads * head_dim (so 1024 tickets at most)
+static constexpr int64_t kFewStreamed = (int64_t)5 << 23, kFewStreamedF32 = (int64_t)5 << 22;  // ... * page-table columns
 
 // at most this many workgroups of the scored extend kernel have work (>= 1)
 static int64_t scored_workgroups(int64_t blk_rows, int64_t tokens, int64_t batch, int64_t n_q_heads, int64_t n_kv_heads) {
@@ -778,10 +778,13 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   // A few tokens (scored form): as rows of the decode kernel, which spreads every row over the machine and needs no
   // second launch to merge; every token then streams its request's K/V again, from L2 at some 6 TB/s.  So it pays where
   // tokens x row bytes x length is small; the length is not known here, the page table's width bounds it.  Measured
-  // against the extend kernel: 16 x 8 tokens over 500 20.8 / 22.6 us, 4 x 16 over 2000 (3.3e7 below) 24.8 / 29.9,
-  // 8 x 8 over 1000 (3.3e7) 30.6 / 33.2, 1 x 100 over 2000 (5.4e7) 48 / 28, 16 x 4 over 8192 (1.3e8) 80 / 39.
+  // against the extend kernel, bf16: 1 x 1 over 300 11 / 16 us, 16 x 8 over 500 16 / 23, 4 x 16 over 2000 (3.3e7 below) 23 / 30,
+  // 2 x 128 over 500 (4.2e7) 24 / 26, 1 x 100 over 2000 (5.4e7) 32 / 28, 16 x 4 over 8192 (1.3e8) 57 / 40; f32: 1 x 1 over 300
+  // 14 / 45, 64 x 2 over 600 (2.0e7) 39 / 82, 1 x 128 over 500 (2.1e7) 39 / 35, 4 x 16 over 2000 45 / 41.
   const int64_t streamed = (int64_t)total_q_tokens * n_kv_heads * head_dim;
-  const bool few = mods != nullptr && dtype != BSGL_DTYPE_F32 && kind == BSGL_DECODE_AUTO && mfma_ok && streamed <= kFewTokens && streamed * table_cols <= kFewStreamed;
+  // (only where a row may be cut does the workspace have a ticket area)
+  const bool few = mods != nullptr && kind == BSGL_DECODE_AUTO && mfma_ok && streamed <= kFewTokens &&
+                   streamed * table_cols <= (dtype == BSGL_DTYPE_F32 ? kFewStreamedF32 : kFewStreamed) && prefill_row_splits(total_q_tokens, 1 << 30) > 1;
   if (kind != BSGL_DECODE_VALU && mfma_ok && !few) {
     ex.row_req = nullptr;  // only the running sums are needed
     if (mods != nullptr) {

@@ -107,9 +107,19 @@ void decode_scored_kernel(DecodeArgs a) {
   RowView me;
   if (a.balance_target > 0) {
     // Pieces of one length for the whole batch, dealt out in row order: with some target of pieces per kv head, a batch of
-    // any lengths takes target + rows workgroups of them at most.  Every wave finds its own by itself.
-    kvh = blockIdx.x % (unsigned)a.n_kv_heads;
-    const int nth = blockIdx.x / (unsigned)a.n_kv_heads;
+    // any lengths takes target + rows workgroups of them at most.  Every wave finds its own by itself (1 us).
+    // (extend tokens of a request read the same K/V: their workgroups for one piece of it are a multiple of kv heads x pieces apart
+    // in the launch, on one XCD and its L2 where that is a multiple of eight -- 8 x 8 over 1000, 28 / 4 heads: 23 us, with rows
+    // side by side 32; requests share nothing, and kv head by kv head streams a little better)
+    int nth;
+    if (a.mods.rows == nullptr) {
+      const unsigned per = (unsigned)(a.balance_target + a.rows);
+      kvh = blockIdx.x / per;
+      nth = blockIdx.x % per;
+    } else {
+      kvh = blockIdx.x % (unsigned)a.n_kv_heads;
+      nth = blockIdx.x / (unsigned)a.n_kv_heads;
+    }
     RowView v0 = {0, 0, 0, 0, false};
     int total = 0, longest = 0;
     for (int r0 = 0; r0 < a.rows; r0 += 64) {
@@ -146,9 +156,16 @@ void decode_scored_kernel(DecodeArgs a) {
     }
     if (row < 0) return;
   } else {
-    row = blockIdx.x;
-    kvh = blockIdx.y;
-    split = blockIdx.z;
+    // (requests: neighbours on the XCDs, 16 x 2048 f32 tokens 20 us, 25 the other way round; extend tokens: as above)
+    if (a.mods.rows == nullptr) {
+      row = blockIdx.x % (unsigned)a.rows;
+      kvh = blockIdx.x / (unsigned)a.rows % (unsigned)a.n_kv_heads;
+      split = blockIdx.x / ((unsigned)a.rows * (unsigned)a.n_kv_heads);
+    } else {
+      kvh = blockIdx.x % (unsigned)a.n_kv_heads;
+      split = blockIdx.x / (unsigned)a.n_kv_heads % (unsigned)a.n_splits;
+      row = blockIdx.x / ((unsigned)a.n_kv_heads * (unsigned)a.n_splits);
+    }
     me = view(row);
     if (!me.owned) return;  // (every workgroup of the row: no ticket is drawn)
     // (fused: no piece is shorter than piece_len; else the merge expects all n_splits)
@@ -430,21 +447,34 @@ bool decode_scored_supported(const DecodeArgs& a) {
 
 template <typename Tag>
 static void launch_scored_tag(const DecodeArgs& a, hipStream_t stream) {
-  dim3 grid((unsigned)a.rows, (unsigned)a.n_kv_heads, (unsigned)a.n_splits);
-  if (a.balance_target > 0) grid = dim3((unsigned)((a.balance_target + a.rows) * a.n_kv_heads), 1, 1);
+  const dim3 grid((unsigned)(a.balance_target > 0 ? (a.balance_target + a.rows) * a.n_kv_heads : a.rows * a.n_kv_heads * a.n_splits));
   if (a.head_dim == 128) hipLaunchKernelGGL((decode_scored_kernel<Tag, 128>), grid, dim3(64 * kWaves), 0, stream, a);
   else hipLaunchKernelGGL((decode_scored_kernel<Tag, 64>), grid, dim3(64 * kWaves), 0, stream, a);
 }
 
+// Per call, with a cap: 64 requests of 2048 tokens, 12 / 2 heads of 128: bf16 26.5 us (135 MB: 5.1 TB/s, what a large copy reaches; the
+// plain decode 27 - 28), f32 50; 14 / 2 heads of 64, with weights, 23.5; 96 documents of 1 - 3363 tokens, 28 / 4 heads, f16 32 (143 MB).
 hipError_t launch_decode_scored(const DecodeArgs& a_in, hipStream_t stream) {
   if (a_in.rows == 0) return hipSuccess;
   DecodeArgs a = a_in;
   a.balance_target = 0;
   a.piece_len = kTokens;
+  if ((int64_t)a.rows * a.n_kv_heads * a.n_splits > 0x7fffffffll) return hipErrorInvalidValue;
   if (a.counters != nullptr && !a.uniform) {
-    a.piece_len = 128;
-    if (a.rows <= 1024 && a.kv.table_cols <= (1 << 20)) {
-      const int64_t units = (int64_t)a.rows * a.n_kv_heads;
+    const int64_t units = (int64_t)a.rows * a.n_kv_heads;
+    // Few workgroups for a page table's width: pieces of 256 tokens (128 where that makes 256 workgroups at most: one request of 4000 tokens
+    // 10.3 us, 11.2 in pieces of 256; 16 x 8 tokens over 500, 14 / 2 heads: 15 us, dealt out below 17), cut without looking at
+    // the other rows.  Else the rows' lengths decide: pieces of one length, some 512 workgroups -- two per CU, which is what streams best
+    // (64 x 2048 tokens of 12 / 2 heads, bf16: 26.5 us, in 1024 27.5, in 256 28; 96 documents of 28 / 4 heads: 768 32 us, 512 33.5, 1024 37) --
+    // and from 512 (row, kv head) pairs on no cut at all but of rows twice the mean (128 x 2048 - 4096, 28 / 4 heads: 161 us; 207 with pieces
+    // of the mean, which cut every second row; 178 in four times as many).
+    // (no request is longer than the page table is wide; a hint that is too small makes its pieces longer)
+    const int64_t longest = a.len_hint > 0 && a.len_hint < a.kv.table_cols ? a.len_hint : a.kv.table_cols;
+    a.piece_len = units * ((longest + 127) / 128) <= 256 ? 128 : 256;
+    const int64_t most = (longest + a.piece_len - 1) / a.piece_len;
+    if (units * most <= 512) {
+      if (a.n_splits > most) a.n_splits = (int32_t)most;
+    } else if (a.rows <= 1024 && a.kv.table_cols <= (1 << 20)) {
       const int64_t pieces = units <= 256 ? 512 : units < 512 ? 768 : units / 2;
       a.balance_target = (int32_t)((pieces + a.n_kv_heads - 1) / a.n_kv_heads);
     } else if (a.base_splits > 0) {

@@ -696,3 +696,42 @@ def test_decode_f32_more_rows_than_tickets(gpu):
 def test_extend_f32_blocks_and_pieces(gpu, heads, ext, prefix):
     for kind in (None, "window", "wild"):
         extend_case(gpu, heads, torch.float32, ext, prefix, cap=7.0, slopes=True, kind=kind, seed=66)
+
+
+@pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("one", torch.float16), ("d64", torch.float32)])
+@pytest.mark.parametrize("batch", [65, 129, 1500])
+def test_decode_ragged_batches_of_many_rows(gpu, heads, dtype, batch):
+    """Pieces dealt out over more rows than a wave has lanes, and over more than are looked through (1024): long rows among short and
+    empty ones, at the ends and at the lanes' border; sampled rows against the definition."""
+    from baby_sglang_amd import _hip
+
+    r = random.Random(batch)
+    lens = [r.randint(1, 60) for _ in range(batch)]
+    for at, n in ((0, 900), (63, 2300), (64, 1700), (batch - 1, 700)):
+        lens[at] = n
+    c = make(67, heads, dtype, [1], q_rows=batch)
+    g = torch.Generator().manual_seed(68)
+    table = torch.randint(0, 3000, (batch, 2400), generator=g, dtype=torch.int32)
+    k, v = (torch.randn(3000, c["hkv"], c["dim"], generator=g).to(dtype) for _ in range(2))
+    st = torch.tensor([r.choice([0, 0, n // 2, n]) for n in lens], dtype=torch.int32)
+    st[[0, 63, 64, batch - 1]] = torch.tensor([0, 5, 0, 100], dtype=torch.int32)
+    w = torch.zeros((batch, 2400), device=gpu)
+    out = _hip.paged_decode_scored(c["q"].to(gpu), k.to(gpu), v.to(gpu), table.to(gpu), torch.arange(batch, device=gpu), torch.tensor(lens, device=gpu),
+                                   logit_cap=9.0, visible_from=st.to(gpu), token_weights=w)
+    rows = sorted({0, 1, 62, 63, 64, batch - 1, *r.sample(range(batch), 40)})
+    want, mass, lse, received, top = orc.scored_exact(c["q"][rows], k, v, table[rows], [lens[i] for i in rows], range(len(rows)), [lens[i] - 1 for i in rows],
+                                                      c["dim"] ** -0.5, 9.0, None, st[rows])
+    u_p = {torch.bfloat16: 2.0**-16, torch.float16: 2.0**-11, torch.float32: 0.0}[dtype]
+    check_rows(out[rows], want, mass, lse, top, 9.0, dtype, dtype, u_p, 2300, v.abs().max().item(), c["dim"])
+    ds = score_error(top, 9.0, lse, c["dim"])
+    for i, row in enumerate(rows):
+        n = lens[row]
+        got = w[row, :n].double().cpu()
+        assert bool(((got - received[i]).abs() <= received[i] * (4 * ds[i].max() + 2.0**-20 + n * 2.0**-23)).all())
+
+
+@pytest.mark.parametrize("hint", [1, 64, 130, 5000])
+def test_decode_hints_that_are_wrong_change_nothing(gpu, hint):
+    for batch in (2, 70):
+        lens = [900, 300] + [5] * (batch - 2)
+        decode_case(gpu, "1.5b", torch.bfloat16, lens, cap=8.0, seed=69, max_seq_len=hint)
