@@ -190,6 +190,15 @@ def _load() -> ctypes.CDLL:
 
 lib = _load()
 
+try:  # the ordinary case of the small calls without their Python (csrc/fast_calls.cpp); the wrappers work without it
+    from . import _fast_calls as _fast
+
+    _fast.bind(*(ctypes.cast(getattr(lib, name), _vp).value for name in (
+        "bsgl_paged_decode_scored", "bsgl_decode_scored_workspace_bytes", "bsgl_evict_tokens", "bsgl_evict_workspace_bytes", "bsgl_logit_controls",
+        "bsgl_paged_prefill_scored", "bsgl_prefill_workspace_bytes")))
+except ImportError:
+    _fast = None
+
 
 def _check(rc: int, what: str) -> None:
     if rc == BSGL_OK:
@@ -604,6 +613,18 @@ def paged_decode_scored(
     ``decode_scored_workspace_bytes``; like every decode workspace it must have been created zero-filled.
     The other arguments are ``paged_decode``'s.
     """
+    if _fast is not None and lse is None and out_dtype is None and q.is_cuda:
+        if out is None and q.dim() == 3:
+            out = torch.empty((q.shape[0], q.shape[1] * q.shape[2]), dtype=q.dtype, device=q.device)
+        index = _current_device()
+        rc = _fast.decode_scored(
+            index, current_stream_handle(index), q, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens, scale, logit_cap, slopes, visible_from,
+            visible_to, token_weights, token_weights_out, n_splits, variant | DECODE_FUSE_KV_WRITE if fuse_kv_write and k_new is not None else variant, out,
+            workspace, max_seq_len, k_new, v_new, out_cache_loc)
+        if rc is not None:
+            if rc:
+                _check(rc, "bsgl_paged_decode_scored")
+            return out
     index = q.get_device()
     _need_gpu(q)
     _same_gpu(index, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens)
@@ -726,6 +747,14 @@ def evict_tokens(
     The page-table and weight rows are compacted in place, or into ``out_table`` / ``out_weights`` (same shape
     and strides).  ``evicted`` may be given with any width; by default it has room for every slot that can go
     (``max_seq_len``, 0 = the table's width, less the budget)."""
+    if _fast is not None and evicted is not None and new_lens is not None and req_to_token.is_cuda:
+        index = _current_device()
+        rc = _fast.evict(index, current_stream_handle(index), req_to_token, token_weights, req_pool_indices, seq_lens, budget, recent, sinks, out_table,
+                         out_weights, evicted, new_lens, max_seq_len)
+        if rc is not None:
+            if rc:
+                _check(rc, "bsgl_evict_tokens")
+            return new_lens, evicted
     index = req_to_token.get_device()
     _need_gpu(req_to_token)
     _same_gpu(index, token_weights, req_pool_indices, seq_lens)
@@ -805,6 +834,16 @@ def logit_controls(
     [batch] or one number).  ``bias_ids`` / ``bias_values`` [batch, n] (int32, float32; ids outside the
     vocabulary are unused places).  ``token_mask`` int32 [rows, ceil(vocab / 32)], bit t % 32 of word t / 32 set =
     token t allowed; ``mask_rows`` int32 [batch] (default i; negative = no mask)."""
+    if _fast is not None and logits.is_cuda:
+        if out is None and logits.dim() == 2:
+            out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        index = _current_device()
+        rc = _fast.logits(index, current_stream_handle(index), logits, history, history_rows, history_lens, prompt_lens, repetition, presence, frequency,
+                          bias_ids, bias_values, token_mask, mask_rows, out)
+        if rc is not None:
+            if rc:
+                _check(rc, "bsgl_logit_controls")
+            return out
     index = logits.get_device()
     _need_gpu(logits)
     shape, stride = logits.shape, logits.stride()
@@ -970,6 +1009,17 @@ def paged_prefill_scored(
     interval as in ``paged_decode_scored``, the interval (int32 [T]) per row of q in positions of its
     request; the default sees everything up to the row's own position.  Rows behind the last request's are left as
     they were."""
+    if _fast is not None and workspace is not None and q.is_cuda:
+        if out is None and q.dim() == 3:
+            out = torch.empty((q.shape[0], q.shape[1] * q.shape[2]), dtype=q.dtype, device=q.device)
+        index = _current_device()
+        rc = _fast.prefill_scored(
+            index, current_stream_handle(index), q, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens, prefix_lens, extended_lens, scale, logit_cap,
+            slopes, visible_from, visible_to, variant | PREFILL_LIST_READY if list_ready else variant, out, workspace)
+        if rc is not None:
+            if rc:
+                _check(rc, "bsgl_paged_prefill_scored")
+            return out
     index = q.get_device()
     _need_gpu(q)
     _same_gpu(index, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens, prefix_lens, extended_lens)
