@@ -138,7 +138,7 @@ void decode_scored_kernel(DecodeArgs a) {
       RowView v = {0, 0, 0, 0, false};
       if (r0 == 0) v = v0;
       else if (r0 + lane < a.rows) v = view(r0 + lane);
-      const int parts = v.owned ? max(1, (v.seq + piece - 1) / piece) : 0;
+      const int parts = !v.owned ? 0 : v.seq <= a.whole_len ? 1 : (v.seq + piece - 1) / piece;
       const int incl = wave_inclusive_scan<ScanAdd>(parts);
       const int all = __builtin_amdgcn_readlane(incl, 63);
       if (nth < before + all) {
@@ -169,7 +169,7 @@ void decode_scored_kernel(DecodeArgs a) {
     me = view(row);
     if (!me.owned) return;  // (every workgroup of the row: no ticket is drawn)
     // (fused: no piece is shorter than piece_len; else the merge expects all n_splits)
-    n_parts = fused ? max(1, min(a.n_splits, (me.seq + a.piece_len - 1) / a.piece_len)) : a.n_splits;
+    n_parts = !fused ? a.n_splits : me.seq <= a.whole_len ? 1 : min(a.n_splits, (me.seq + a.piece_len - 1) / a.piece_len);
     if (split >= n_parts) return;
   }
   const int64_t req = me.req;
@@ -458,20 +458,24 @@ hipError_t launch_decode_scored(const DecodeArgs& a_in, hipStream_t stream) {
   if (a_in.rows == 0) return hipSuccess;
   DecodeArgs a = a_in;
   a.balance_target = 0;
+  a.whole_len = 0;
   a.piece_len = kTokens;
   if ((int64_t)a.rows * a.n_kv_heads * a.n_splits > 0x7fffffffll) return hipErrorInvalidValue;
   if (a.counters != nullptr && !a.uniform) {
     const int64_t units = (int64_t)a.rows * a.n_kv_heads;
+    // Short rows are not cut: one piece has no merge to wait for.  131 tokens 6.2 us, in two pieces 8.1, 200 7.2 / 8.3, 300 8.1 / 8.3;
+    // five turns of 3 - 41 tokens over 333 11.8 / 13.8; 500 10.9 / 8.4, f32 16 / 10, whose tiles take longer.
     // Few workgroups for a page table's width: pieces of 256 tokens (128 where that makes 256 workgroups at most: one request of 4000 tokens
-    // 10.3 us, 11.2 in pieces of 256; 16 x 8 tokens over 500, 14 / 2 heads: 15 us, dealt out below 17), cut without looking at
-    // the other rows.  Else the rows' lengths decide: pieces of one length, some 512 workgroups -- two per CU, which is what streams best
+    // 10.1 us, 10.6 in pieces of 256; 64 where that makes 64: one of 500 7.5 us, 8.4 in pieces of 128, 8 of 1000 10.6 / 9.5), cut without
+    // looking at the other rows (1 us less than finding a piece).  Else the rows' lengths decide: pieces of one length, some 512 workgroups -- two per CU, which is what streams best
     // (64 x 2048 tokens of 12 / 2 heads, bf16: 26.5 us, in 1024 27.5, in 256 28; 96 documents of 28 / 4 heads: 768 32 us, 512 33.5, 1024 37) --
     // and from 512 (row, kv head) pairs on no cut at all but of rows twice the mean (128 x 2048 - 4096, 28 / 4 heads: 161 us; 207 with pieces
     // of the mean, which cut every second row; 178 in four times as many).
     // (no request is longer than the page table is wide; a hint that is too small makes its pieces longer)
     const int64_t longest = a.len_hint > 0 && a.len_hint < a.kv.table_cols ? a.len_hint : a.kv.table_cols;
-    a.piece_len = units * ((longest + 127) / 128) <= 256 ? 128 : 256;
-    const int64_t most = (longest + a.piece_len - 1) / a.piece_len;
+    a.whole_len = a.dtype == kF32 ? 128 : 384;
+    a.piece_len = units * ((longest + 63) / 64) <= 64 ? 64 : units * ((longest + 127) / 128) <= 256 ? 128 : 256;
+    const int64_t most = longest <= a.whole_len ? 1 : (longest + a.piece_len - 1) / a.piece_len;
     if (units * most <= 512) {
       if (a.n_splits > most) a.n_splits = (int32_t)most;
     } else if (a.rows <= 1024 && a.kv.table_cols <= (1 << 20)) {
