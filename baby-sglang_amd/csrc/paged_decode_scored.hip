@@ -53,7 +53,8 @@ template <typename Tag> __device__ __forceinline__ f32x4v score_product(u32x4v k
 // waves per SIMD the registers of an instance allow
 template <typename Tag, int D> constexpr int occupancy() { return std::is_same<Tag, f32_tag>::value && D == 128 ? 3 : 4; }
 
-template <typename Tag, int D>
+// ROWS: extend tokens as rows (ScoreMods::rows), else requests
+template <typename Tag, int D, bool ROWS>
 __global__ __launch_bounds__(64 * kWaves, (occupancy<Tag, D>()))
 void decode_scored_kernel(DecodeArgs a) {
   using E = Elem<Tag>;
@@ -85,7 +86,7 @@ void decode_scored_kernel(DecodeArgs a) {
     int own = 0;
     RowView v;
     v.owned = true;
-    if (a.mods.rows != nullptr) {
+    if constexpr (ROWS) {
       const int4 r4 = a.mods.rows[i];
       req = r4.x;
       len64 = r4.y;
@@ -97,7 +98,7 @@ void decode_scored_kernel(DecodeArgs a) {
     }
     v.req = (int)(req < 0 ? 0 : (req >= a.kv.table_rows ? a.kv.table_rows - 1 : req));
     const int len = (int)(len64 < 0 ? 0 : (len64 > a.kv.table_cols ? a.kv.table_cols : len64));
-    v.own = a.mods.rows != nullptr ? own : len - 1;
+    v.own = ROWS ? own : len - 1;
     const int2 seen = visible_range(a.mods, i, len, min(len, v.own + 1));
     v.first = seen.x;
     v.seq = v.owned ? seen.y : 0;
@@ -112,7 +113,7 @@ void decode_scored_kernel(DecodeArgs a) {
     // in the launch, on one XCD and its L2 where that is a multiple of eight -- 8 x 8 over 1000, 28 / 4 heads: 23 us, with rows
     // side by side 32; requests share nothing, and kv head by kv head streams a little better)
     int nth;
-    if (a.mods.rows == nullptr) {
+    if constexpr (!ROWS) {
       const unsigned per = (unsigned)(a.balance_target + a.rows);
       kvh = blockIdx.x / per;
       nth = blockIdx.x % per;
@@ -156,8 +157,8 @@ void decode_scored_kernel(DecodeArgs a) {
     }
     if (row < 0) return;
   } else {
-    // (requests: neighbours on the XCDs, 16 x 2048 f32 tokens 20 us, 25 the other way round; extend tokens: as above)
-    if (a.mods.rows == nullptr) {
+    // (requests side by side on the XCDs: 16 x 2048 f32 tokens 20 us, 25 the other way round; extend tokens: as above)
+    if constexpr (!ROWS) {
       row = blockIdx.x % (unsigned)a.rows;
       kvh = blockIdx.x / (unsigned)a.rows % (unsigned)a.n_kv_heads;
       split = blockIdx.x / ((unsigned)a.rows * (unsigned)a.n_kv_heads);
@@ -219,11 +220,16 @@ void decode_scored_kernel(DecodeArgs a) {
     const uint32_t e = (uint32_t)table_row[min(start + tile * kTokens + c, end - 1)];
     return (int)(e > max_slot ? max_slot : e);
   };
-  // (cached loads: a line comes in two pieces; non-temporal, 64 x 2048 f32 tokens of 12 / 2 heads took 67 us instead of 53)
+  // (K/V of a request are read once: non-temporal, 64 x 2048 bf16 tokens of 12 / 2 heads 30.5 us from memory, 33 through the caches.  f32
+  // is not: its lines come in more pieces, 62 us against 59.5; nor is what the rows of an extend share)
+  auto fetch = [&](auto* p) {
+    if constexpr (!F32 && !ROWS) return __builtin_nontemporal_load(p);
+    else return *p;
+  };
   auto load_k = [&](int slot) {
     const char* p = slot == new_slot ? k_new + 16 * u : k_lane + slot * slab_row;
 #pragma unroll
-    for (int j = 0; j < KN; ++j) xk[j] = *(const u32x4v*)(p + 64 * j);
+    for (int j = 0; j < KN; ++j) xk[j] = fetch((const u32x4v*)(p + 64 * j));
   };
   auto load_v = [&](int slot) {
 #pragma unroll
@@ -231,13 +237,13 @@ void decode_scored_kernel(DecodeArgs a) {
       const int of = __shfl(slot, 4 * u + i);
       const char* p = of == new_slot ? v_new + VB * c : v_lane + of * slab_row;
       if constexpr (VB == 8) {
-        const u32x2v x = *(const u32x2v*)p;
+        const u32x2v x = fetch((const u32x2v*)p);
         xv[i][0] = x[0];
         xv[i][1] = x[1];
       } else {
 #pragma unroll
         for (int n = 0; n < VB / 16; ++n) {
-          const u32x4v x = *(const u32x4v*)(p + 16 * n);
+          const u32x4v x = fetch((const u32x4v*)(p + 16 * n));
 #pragma unroll
           for (int k = 0; k < 4; ++k) xv[i][4 * n + k] = x[k];
         }
@@ -448,12 +454,14 @@ bool decode_scored_supported(const DecodeArgs& a) {
 template <typename Tag>
 static void launch_scored_tag(const DecodeArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)(a.balance_target > 0 ? (a.balance_target + a.rows) * a.n_kv_heads : a.rows * a.n_kv_heads * a.n_splits));
-  if (a.head_dim == 128) hipLaunchKernelGGL((decode_scored_kernel<Tag, 128>), grid, dim3(64 * kWaves), 0, stream, a);
-  else hipLaunchKernelGGL((decode_scored_kernel<Tag, 64>), grid, dim3(64 * kWaves), 0, stream, a);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, stream, a); };
+  if (a.mods.rows != nullptr) a.head_dim == 128 ? go(decode_scored_kernel<Tag, 128, true>) : go(decode_scored_kernel<Tag, 64, true>);
+  else a.head_dim == 128 ? go(decode_scored_kernel<Tag, 128, false>) : go(decode_scored_kernel<Tag, 64, false>);
 }
 
-// Per call, with a cap: 64 requests of 2048 tokens, 12 / 2 heads of 128: bf16 26.5 us (135 MB: 5.1 TB/s, what a large copy reaches; the
-// plain decode 27 - 28), f32 50; 14 / 2 heads of 64, with weights, 23.5; 96 documents of 1 - 3363 tokens, 28 / 4 heads, f16 32 (143 MB).
+// Per call, with a cap, K/V from memory: 64 requests of 2048 tokens, 12 / 2 heads of 128: bf16 30.5 us (135 MB; the plain decode 29), f32
+// 59.5 (270 MB; the plain generic kernel 66); 128 of 2048 - 4096, 28 / 4 heads, 161 (the copy rate); 96 documents of 1 - 3363 tokens, 28 / 4
+// heads, f16, 40 (143 MB); one request of 4000 tokens 11 (the plain decode 13.4).
 hipError_t launch_decode_scored(const DecodeArgs& a_in, hipStream_t stream) {
   if (a_in.rows == 0) return hipSuccess;
   DecodeArgs a = a_in;
@@ -467,10 +475,11 @@ hipError_t launch_decode_scored(const DecodeArgs& a_in, hipStream_t stream) {
     // five turns of 3 - 41 tokens over 333 11.8 / 13.8; 500 10.9 / 8.4, f32 16 / 10, whose tiles take longer.
     // Few workgroups for a page table's width: pieces of 256 tokens (128 where that makes 256 workgroups at most: one request of 4000 tokens
     // 10.1 us, 10.6 in pieces of 256; 64 where that makes 64: one of 500 7.5 us, 8.4 in pieces of 128, 8 of 1000 10.6 / 9.5), cut without
-    // looking at the other rows (1 us less than finding a piece).  Else the rows' lengths decide: pieces of one length, some 512 workgroups -- two per CU, which is what streams best
-    // (64 x 2048 tokens of 12 / 2 heads, bf16: 26.5 us, in 1024 27.5, in 256 28; 96 documents of 28 / 4 heads: 768 32 us, 512 33.5, 1024 37) --
-    // and from 512 (row, kv head) pairs on no cut at all but of rows twice the mean (128 x 2048 - 4096, 28 / 4 heads: 161 us; 207 with pieces
-    // of the mean, which cut every second row; 178 in four times as many).
+    // looking at the other rows (1 us less than finding a piece).  Else the rows' lengths decide: pieces of one length, some 512 workgroups -- two
+    // per CU (64 x 2048 tokens of 12 / 2 heads of 128: 30.5 us from memory, 32 in 1024, 37.5 in 768; heads of 64, with weights, 1024 27 us,
+    // 512 30.5) --, 768 from 257 (row, kv head) pairs on (96 documents of 28 / 4 heads: 40 us, 48 in 512, 45.5 in 1024) and
+    // from 512 pairs on no cut at all but of rows twice the mean (128 x 2048 - 4096, 28 / 4 heads: 161 us; 221 with pieces of the
+    // mean, which cut every second row; 171 in four times as many).
     // (no request is longer than the page table is wide; a hint that is too small makes its pieces longer)
     const int64_t longest = a.len_hint > 0 && a.len_hint < a.kv.table_cols ? a.len_hint : a.kv.table_cols;
     a.whole_len = a.dtype == kF32 ? 128 : 384;
@@ -479,7 +488,7 @@ hipError_t launch_decode_scored(const DecodeArgs& a_in, hipStream_t stream) {
     if (units * most <= 512) {
       if (a.n_splits > most) a.n_splits = (int32_t)most;
     } else if (a.rows <= 1024 && a.kv.table_cols <= (1 << 20)) {
-      const int64_t pieces = units <= 256 ? 512 : units < 512 ? 768 : units / 2;
+      const int64_t pieces = units > 256 ? (units < 512 ? 768 : units / 2) : a.head_dim == 64 && a.dtype != kF32 ? 1024 : 512;
       a.balance_target = (int32_t)((pieces + a.n_kv_heads - 1) / a.n_kv_heads);
     } else if (a.base_splits > 0) {
       a.n_splits = a.base_splits;
