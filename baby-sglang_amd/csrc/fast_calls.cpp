@@ -1,5 +1,5 @@
 // The scored attention, eviction and logit calls of _hip.py without their Python: a small call's host time is the time of the call (one
-// request's decode 8 us on the GPU, its wrapper 10), and most of it goes into asking a dozen tensors for type, shape, strides and
+// request's decode 6 us on the GPU, its wrapper 10, 4 this way), and most of it goes into asking a dozen tensors for type, shape, strides and
 // address one attribute at a time.  Every function here takes the wrapper's arguments, checks that they are the ordinary case -- tensors
 // on the current GPU, of the types and strides that the C entry point takes as they are -- and makes the call; it returns the entry point's
 // code, or None for anything else, without having called it: the wrapper then goes on as if it were not there, and raises or

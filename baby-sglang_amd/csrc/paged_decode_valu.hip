@@ -14,8 +14,8 @@
 //   softmax is the online (running max / running sum) form in base 2.
 //   Per-wave states are merged through LDS, per-split states through a second
 //   small kernel (merge_states_kernel).
-// SCORED: the scores of DecodeArgs::mods, as in paged_decode_mfma.hip; with mods.rows a row is an extend
-// token whose own position is not the request's last.
+// SCORED: the scores of DecodeArgs::mods, for what paged_decode_scored.hip does not take (and where a call asks for this
+// kernel); with mods.rows a row is an extend token whose own position is not the request's last.
 #include "bsgl_device.h"
 #include "bsgl_launch.h"
 #include "bsgl_score.h"
