@@ -190,7 +190,14 @@ struct ExpandArgs {
   int4* rows4;       // instead of row_req / row_len, for the scored form: {page-table row, request length, own position, 1}
   uint32_t* clear;   // words to be set to zero on the way (tickets), or NULL; not with row_req
   int32_t n_clear;
+  // scored form: the groups by the tokens they stream, most first (NULL: not made).  [n_order], n_order <= kMaxOrder; with more groups than
+  // that (extended_lens that contradict the number of q rows) they stay as they are
+  int32_t* order;
+  int32_t n_order;
+  int64_t table_cols;
+  const int32_t *from, *to;  // ScoreMods'
 };
+constexpr int kMaxOrder = 1024;
 
 // extend attention over blocks of 16 query positions (matrix-core kernel)
 struct PrefillArgs {
@@ -210,6 +217,8 @@ struct PrefillArgs {
   int32_t blk_rows;    // query positions per workgroup: 16 or 64
   int32_t grp_blocks;  // consecutive blocks of a request that form one group (share an XCD)
   int32_t max_groups;  // bound on cu_blk[batch]
+  const int32_t* order;  // scored form: launch order of the groups (ExpandArgs::order), or NULL
+  int32_t n_order;
   uint64_t* prof;      // tuning aid, normally NULL: 8 x uint64 of phase cycles per wave
   int32_t fold_group;  // two kv heads of 64 values streamed as one of 128 (see DecodeArgs::fold_group); 0 = no
   int32_t n_q_heads;

@@ -732,15 +732,29 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   // holds a workgroup for every block slot of every group, and the slots a request does not fill
   // retire at once -- but dispatching them is not free (batches of one-block requests in groups
   // of 8 spent 4/5 of the launch on it), so the group is no larger than the mean request needs.
+  bool sorted = false;
   {
     const int64_t per = (int64_t)pa.blk_rows * (batch > 0 ? batch : 1);
     const int64_t mean_blocks = ((int64_t)total_q_tokens + per - 1) / per;
-    int grp = 1;
-    // (scored form, launches that do not fill the machine: a group would put them on one of the eight XCDs)
-    // (two kv heads of 64 values run as one of 128 there, see below: 3 x 1500 over 1500, 14 / 2 heads: 164 us in groups, 106)
-    const int64_t kv_units = head_dim == 64 && n_kv_heads == 2 && dtype != BSGL_DTYPE_F32 ? 1 : n_kv_heads;
-    const bool spread = mods != nullptr && scored_workgroups(pa.blk_rows, total_q_tokens, batch, n_q_heads, kv_units) <= 512;
-    while (!spread && grp < 8 && grp < mean_blocks) grp *= 2;
+    int grp = 1, most = 8;
+    if (mods != nullptr) {
+      // Scored form: launches of up to ten rounds of the machine (two workgroups per CU) go block by block, and the longest streams
+      // first (prefill_order_kernel).  Against groups of 8 in the requests' order: 6 x 700 - 1501 tokens, 12 / 2 heads, with a bias 76 -> 52 us
+      // (f32 440 -> 299), documents 53 -> 43, 20 x 100 - 2000 of 14 / 2 heads of 64 211 -> 161, 200 x 10 - 300 over 500 252 -> 218, 1 x 4096
+      // of 28 / 4 heads 187 -> 174.  Larger ones stay in groups: 48 x 512 over 1536, 28 / 4 heads, 842, block by block -- its K/V
+      // then pass every L2 -- 880; sorted or not makes 1 - 2 % there (48 x 100 - 2000 875 - 910 -> 872 - 892).
+      // (two kv heads of 64 values run as one of 128 there, see below)
+      const int64_t kv_units = head_dim == 64 && n_kv_heads == 2 && dtype != BSGL_DTYPE_F32 ? 1 : n_kv_heads;
+      const int64_t n_wg = scored_workgroups(pa.blk_rows, total_q_tokens, batch, n_q_heads, kv_units);
+      most = n_wg <= 5120 ? 1 : 8;
+      sorted = n_wg > 256;  // (else every workgroup has a CU to itself)
+      // (more groups than the sort takes: many requests of one block or two, or very many rows)
+      if (((int64_t)total_q_tokens + pa.blk_rows - 1) / pa.blk_rows / most + batch + 1 > bsgl::kMaxOrder) {
+        most = n_wg <= 512 ? 1 : 8;
+        sorted = false;
+      }
+    }
+    while (grp < most && grp < mean_blocks) grp *= 2;
     const int forced = bsgl::knob(bsgl::kKnobPrefillGroup);  // tuning override
     pa.grp_blocks = forced > 0 ? forced : grp;
   }
@@ -750,6 +764,7 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   {
     const int64_t blocks = ((int64_t)total_q_tokens + pa.blk_rows - 1) / pa.blk_rows + batch;
     pa.max_groups = (int32_t)(pa.grp_blocks == 1 ? blocks : blocks / pa.grp_blocks + batch + 1);
+    if (pa.max_groups > bsgl::kMaxOrder) sorted = false;  // (also: mean_blocks below `most`)
   }
   pa.prof = g_prefill_prof;
   pa.n_q_heads = n_q_heads;
@@ -786,6 +801,16 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   const bool few = mods != nullptr && kind == BSGL_DECODE_AUTO && mfma_ok && streamed <= kFewTokens &&
                    streamed * table_cols <= (dtype == BSGL_DTYPE_F32 ? kFewStreamedF32 : kFewStreamed) && prefill_row_splits(total_q_tokens, 1 << 30) > 1;
   if (kind != BSGL_DECODE_VALU && mfma_ok && !few) {
+    if (sorted) {
+      // (in the row list's place: a group has a row at least)
+      ex.order = (int32_t*)ex.row_req;
+      ex.n_order = (int32_t)(2 * (int64_t)total_q_tokens < bsgl::kMaxOrder ? 2 * total_q_tokens : bsgl::kMaxOrder);
+      ex.table_cols = table_cols;
+      ex.from = mods->visible_from;
+      ex.to = mods->visible_to;
+      pa.order = ex.order;
+      pa.n_order = ex.n_order;
+    }
     ex.row_req = nullptr;  // only the running sums are needed
     if (mods != nullptr) {
       // Scored form: two workgroups fit a CU.  With room for more than twice the blocks there are at most, every

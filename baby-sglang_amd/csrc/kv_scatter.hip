@@ -34,7 +34,8 @@ __global__ __launch_bounds__(256) void kv_scatter_kernel(ScatterArgs a) {
 // exclusive running sums of extended_lens and of the block groups of each request,
 // ceil(ceil(extended_lens / blk_rows) / grp_blocks)  (negative lengths count as 0, lengths above
 // the number of q rows as that number)
-__device__ __forceinline__ void running_sums(const ExpandArgs& a) {
+// (`starts`: the groups' sums once more, in LDS, or NULL)
+__device__ __forceinline__ void running_sums(const ExpandArgs& a, int* starts = nullptr) {
   __shared__ int64_t s_ext[256], s_blk[256];
   const int tid = threadIdx.x;
   const int per = (a.batch + 255) / 256;
@@ -69,17 +70,84 @@ __device__ __forceinline__ void running_sums(const ExpandArgs& a) {
   if (tid == 255) {
     a.cu_ext[a.batch] = run + sum;
     if (a.cu_blk != nullptr) a.cu_blk[a.batch] = brun + blocks;
+    if (starts != nullptr) starts[a.batch] = (int)min(brun + blocks, (int64_t)0x7fffffff);
   }
   for (int i = lo; i < hi; ++i) {
     const int64_t e = min(max((int64_t)0, a.extended_lens[i]), (int64_t)a.total_q_tokens);  // (bounded: the sums cannot overflow)
     a.cu_ext[i] = run;
     if (a.cu_blk != nullptr) a.cu_blk[i] = brun;
+    if (starts != nullptr) starts[i] = (int)brun;
     run += e;
     brun += groups_of(e);
   }
 }
 
-__global__ void prefill_cu_kernel(ExpandArgs a) { running_sums(a); }
+__global__ __launch_bounds__(256) void prefill_cu_kernel(ExpandArgs a) { running_sums(a); }
+
+// The same and the order in which the scored extend kernel launches its groups: the longest streams first, so that the launch does not end
+// on a few of them (what a group streams is taken from its first row's beginning and its last row's end, exact for
+// causal, prefix, window and document masks).  A counting sort by 256 lengths; the order inside one is any.
+__global__ __launch_bounds__(256) void prefill_order_kernel(ExpandArgs a) {
+  __shared__ int s_start[kMaxOrder + 1];
+  __shared__ int s_bucket[256];
+  __shared__ int s_part[4], s_max[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  running_sums(a, s_start);
+  s_bucket[tid] = 0;
+  __threadfence_block();
+  __syncthreads();
+  const int n = s_start[a.batch];
+  if (n > a.n_order) {
+    for (int g = tid; g < a.n_order; g += 256) a.order[g] = g;
+    return;
+  }
+  constexpr int PER = kMaxOrder / 256;
+  const int64_t rows = (int64_t)max(a.grp_blocks, 1) * max(a.blk_rows, 1);
+  int key[PER], longest = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int g = tid + 256 * k;
+    key[k] = -1;
+    if (g >= n) continue;
+    int lo = 0, hi = a.batch;  // the last request that starts at g or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_start[mid] <= g) lo = mid; else hi = mid;
+    }
+    const int64_t ext = min(max((int64_t)0, a.extended_lens[lo]), (int64_t)a.total_q_tokens);
+    const int64_t seq = min(max((int64_t)0, a.seq_lens[lo]), a.table_cols);
+    const int64_t prefix = min(max((int64_t)0, a.prefix_lens[lo]), seq);
+    const int64_t r0 = (g - s_start[lo]) * rows, r1 = min(r0 + rows, ext) - 1;
+    const int64_t at = a.cu_ext[lo], last_row = (int64_t)a.total_q_tokens - 1;
+    int64_t end = min(seq, prefix + r1 + 1), begin = 0;
+    if (a.to != nullptr) end = min(seq, (int64_t)a.to[min(at + r1, last_row)]);
+    if (a.from != nullptr) begin = max((int64_t)0, (int64_t)a.from[min(at + r0, last_row)]);
+    key[k] = (int)max((int64_t)0, end - begin);
+    longest = max(longest, key[k]);
+  }
+  longest = __builtin_amdgcn_readlane(wave_inclusive_scan<ScanMax>(longest), 63);
+  if (lane == 0) s_max[wave] = longest;
+  __syncthreads();
+  longest = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+  const float f = 255.f / (float)max(longest, 1);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if (key[k] < 0) continue;
+    key[k] = 255 - min(255, (int)((float)key[k] * f));
+    atomicAdd(&s_bucket[key[k]], 1);
+  }
+  __syncthreads();
+  const int incl = wave_inclusive_scan<ScanAdd>(s_bucket[tid]);
+  if (lane == 63) s_part[wave] = incl;
+  __syncthreads();
+  int before = incl - s_bucket[tid];
+  for (int w = 0; w < wave; ++w) before += s_part[w];
+  s_bucket[tid] = before;  // (its own entry only)
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+    if (key[k] >= 0) a.order[atomicAdd(&s_bucket[key[k]], 1)] = tid + 256 * k;
+}
 
 // what the decode kernels have to know about extend token t
 __device__ __forceinline__ void expand_row(const ExpandArgs& a, int t) {
@@ -145,7 +213,9 @@ hipError_t launch_prefill_expand(const ExpandArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL(prefill_few_kernel, dim3(1), dim3(256), 0, stream, a);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(prefill_cu_kernel, dim3(1), dim3(256), 0, stream, a);
+  if (a.order != nullptr && (a.batch > kMaxOrder || a.n_order > kMaxOrder)) return hipErrorInvalidValue;
+  if (a.order != nullptr) hipLaunchKernelGGL(prefill_order_kernel, dim3(1), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL(prefill_cu_kernel, dim3(1), dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.total_q_tokens == 0 || (a.row_req == nullptr && a.rows4 == nullptr)) return e;
   hipLaunchKernelGGL(prefill_rows_kernel, dim3((a.total_q_tokens + 255) / 256), dim3(256), 0, stream, a);

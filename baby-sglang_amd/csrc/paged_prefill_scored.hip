@@ -1,7 +1,7 @@
 // Scored extend attention for gfx950: cap * tanh(s / cap), minus slope[head] * |i - j|, over an interval
 // [from, to) of positions per query row (ScoreMods); bf16 / f16, head_dim 128 or two kv heads of 64 folded.
 //
-// The frame is paged_prefill_mfma32.hip's: the same work list and launch order, four waves on 64 positions x 2
+// The frame is paged_prefill_mfma32.hip's: the same work list (launched longest stream first, see prefill_order_kernel), four waves on 64 positions x 2
 // q heads (or 16 x 8 for short extends), one K/V stream per workgroup through a four-stage ring, per 32-token
 // step 8 products for the scores of the NEXT step beside the exponentials of this one and 8 for P . V.  What is
 // new sits between the products:
@@ -177,7 +177,9 @@ void prefill_scored_kernel(PrefillArgs a) {
   if (g >= a.cu_blk[a.batch] * a.n_kv_heads) return;
   const int within = (int)(slot % (unsigned)per_group);
   const int kvh = (int)(g % a.n_kv_heads);
-  const int64_t pg = g / a.n_kv_heads;
+  int64_t pg = g / a.n_kv_heads;
+  // (longest streams first; whatever stands there, it is a group of this launch)
+  if (pg < a.n_order) pg = max((int64_t)0, min((int64_t)a.order[pg], a.cu_blk[a.batch] - 1));
   const int rt0 = (within % n_z) * HPW;
   const int n_rt = min(HPW, G - rt0);
   int i_req = 0;

@@ -387,7 +387,8 @@ int bsgl_paged_prefill(void* out /*device*/, int64_t out_row_stride,
 /*
  * bsgl_paged_prefill (arguments, work list, workspace as there) with scored attention: visible_from / visible_to
  * are per row of q, and a row's own position is prefix_lens[i] + r.  token_weights is not taken
- * (BSGL_ERR_UNSUPPORTED).
+ * (BSGL_ERR_UNSUPPORTED).  BSGL_PREFILL_LIST_READY: the list of an earlier SCORED call for this batch, with the same
+ * shapes and variant (the intervals, cap and slopes may differ); a plain call's list is another one.
  */
 int bsgl_paged_prefill_scored(void* out /*device*/, int64_t out_row_stride,
                               const void* q /*device*/, int64_t q_row_stride,

@@ -735,3 +735,71 @@ def test_decode_hints_that_are_wrong_change_nothing(gpu, hint):
     for batch in (2, 70):
         lens = [900, 300] + [5] * (batch - 2)
         decode_case(gpu, "1.5b", torch.bfloat16, lens, cap=8.0, seed=69, max_seq_len=hint)
+
+
+@pytest.mark.parametrize("heads,dtype,kind", [("7b", torch.bfloat16, "document"), ("0.5b", torch.float16, "wild"), ("1.5b", torch.float32, "prefix"), ("mha", torch.bfloat16, None)])
+def test_extend_many_groups_longest_first(gpu, heads, dtype, kind):
+    """Launches whose blocks are sorted by what they stream: ragged, with requests that bring nothing; several rows of one request."""
+    r = random.Random(5)
+    ext = [r.choice([0, 1, 63, 64, 65, r.randint(1, 400)]) for _ in range(40)]
+    prefix = [r.choice([0, 7, r.randint(0, 500)]) for _ in ext]
+    extend_case(gpu, heads, dtype, ext, prefix, cap=20.0, slopes=True, kind=kind, seed=50, extra_rows=2, only=80)
+
+
+@pytest.mark.parametrize("batch", [900, 1000, 1100])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_extend_about_as_many_groups_as_are_sorted(gpu, batch, dtype):
+    r = random.Random(batch)
+    ext = [r.randint(0, 3) for _ in range(batch - 2)] + [200, 90]
+    extend_case(gpu, "1.5b", dtype, ext, [r.randint(0, 20) for _ in ext], cap=20.0, kind="window", seed=51, only=120)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_extend_lengths_that_contradict_the_rows(gpu, dtype):
+    """100 requests that all claim the 100 rows: the first one has them, the others' lie behind the last row."""
+    from baby_sglang_amd import _hip
+
+    c = make(52, "7b", dtype, [150], q_rows=100)
+    d = to_gpu(c, gpu)
+    claim = lambda first, rest: torch.tensor([first] + [rest] * 99, device=gpu)  # noqa: E731
+    row = int(c["req"][0])
+    out = _hip.paged_prefill_scored(d["q"], d["k"], d["v"], d["table"], claim(row, row), claim(150, 150), claim(50, 0), claim(100, 100), logit_cap=9.0, variant=2)
+    alone = _hip.paged_prefill_scored(d["q"], d["k"], d["v"], d["table"], *(claim(x, 0)[:1] for x in (row, 150, 50, 100)), logit_cap=9.0, variant=2)
+    torch.cuda.synchronize()
+    want, mass, lse, _, top = orc.scored_exact(c["q"], c["k"], c["v"], c["table"][c["req"]], [150], [0] * 100, list(range(50, 150)), c["dim"] ** -0.5, 9.0, None, None, None)
+    u_p = {torch.bfloat16: 2.0**-8, torch.float32: 0.0}[dtype]
+    for got in (out, alone):
+        check_rows(got, want, mass, lse, top, 9.0, dtype, dtype, u_p, 150, c["v"].abs().max().item(), c["dim"])
+
+
+def test_extend_sorted_list_kept_and_replayed(gpu):
+    """A kept list under other masks and caps, and a captured pair of calls replayed with other lengths."""
+    from baby_sglang_amd import _hip
+
+    r = random.Random(8)
+    ext = [r.randint(60, 300) for _ in range(20)]
+    pre = [r.randint(0, 300) for _ in ext]
+    c = make(53, "7b", torch.bfloat16, [a + b for a, b in zip(ext, pre)], q_rows=sum(ext))
+    d = to_gpu(c, gpu)
+    pre_t, ext_t = torch.tensor(pre, device=gpu), torch.tensor(ext, device=gpu)
+    args = (d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], pre_t, ext_t)
+    ws = torch.empty(_hip.prefill_workspace_bytes(20, sum(ext), 28, 128), dtype=torch.uint8, device=gpu)
+    st, sp = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in intervals("both", c["lens"], ext, 3))
+    first = _hip.paged_prefill_scored(*args, logit_cap=10.0, workspace=ws)
+    kept = _hip.paged_prefill_scored(*args, logit_cap=30.0, visible_from=st, visible_to=sp, workspace=ws, list_ready=True)
+    assert torch.equal(first, _hip.paged_prefill_scored(*args, logit_cap=10.0))
+    assert torch.equal(kept, _hip.paged_prefill_scored(*args, logit_cap=30.0, visible_from=st, visible_to=sp))
+    out = torch.empty_like(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _hip.paged_prefill_scored(*args, logit_cap=10.0, workspace=ws, out=torch.empty_like(first))
+        _hip.paged_prefill_scored(*args, logit_cap=30.0, visible_from=st, visible_to=sp, workspace=ws, list_ready=True, out=out)
+    for turn in range(3):
+        e2 = ext[turn:] + ext[:turn]
+        ext_t.copy_(torch.tensor(e2))
+        pre_t.copy_(torch.tensor([n - e if n > e else 0 for n, e in zip(c["lens"], e2)]))
+        out.zero_()
+        eager = _hip.paged_prefill_scored(*args, logit_cap=30.0, visible_from=st, visible_to=sp)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
