@@ -122,7 +122,7 @@ __global__ __launch_bounds__(256) void prefill_order_kernel(ExpandArgs a) {
     int64_t end = min(seq, prefix + r1 + 1), begin = 0;
     if (a.to != nullptr) end = min(seq, (int64_t)a.to[min(at + r1, last_row)]);
     if (a.from != nullptr) begin = max((int64_t)0, (int64_t)a.from[min(at + r0, last_row)]);
-    key[k] = (int)max((int64_t)0, end - begin);
+    key[k] = (int)max((int64_t)0, min(end - begin, (int64_t)0x7fffffff));  // (never negative: every group has a place)
     longest = max(longest, key[k]);
   }
   longest = __builtin_amdgcn_readlane(wave_inclusive_scan<ScanMax>(longest), 63);
