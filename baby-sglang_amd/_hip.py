@@ -337,6 +337,16 @@ def _check_weights(t: torch.Tensor, table_shape, cols: int) -> int:
     return stride[0]
 
 
+def _check_evicted(t: torch.Tensor, batch: int) -> int:
+    """The row stride of a tensor for the evicted slots: its rows are written, so they must not share memory."""
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != batch:
+        raise ValueError(f"evicted must be int32 [{batch}, width], got {t.dtype} {tuple(t.shape)}")
+    width, (row, col) = t.shape[1], t.stride()
+    if (width > 1 and col != 1) or (batch > 1 and row < width):
+        raise ValueError(f"evicted must have dense rows that do not overlap, got strides {t.stride()} for rows of {width}")
+    return row if batch > 1 else width
+
+
 def _index_rows(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     """A dense int64 vector of ``n`` entries on the GPU."""
     if t.shape != (n,):
@@ -782,9 +792,7 @@ def evict_tokens(
     if evicted is None:
         longest = min(int(max_seq_len), cols) if max_seq_len > 0 else cols
         evicted = torch.empty((batch, max(0, longest - budget)), dtype=torch.int32, device=device)
-    elif evicted.dtype != torch.int32 or evicted.dim() != 2 or evicted.shape[0] != batch \
-            or (evicted.shape[1] > 1 and evicted.stride(1) != 1):
-        raise ValueError("evicted must be int32 [batch, width] with dense rows")
+    evicted_stride = _check_evicted(evicted, batch)
     width = evicted.shape[1]
     need = lib.bsgl_evict_workspace_bytes(batch, cols, budget)
     ws_ptr = ws_bytes = 0
@@ -798,7 +806,7 @@ def evict_tokens(
     rc = _launch(
         index, lib.bsgl_evict_tokens, out_table.data_ptr(), out_weights.data_ptr(), req_to_token.data_ptr(), stride,
         token_weights.data_ptr(), w_stride, n_rows, cols, req_pool_indices.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(),
-        evicted.data_ptr() if width else None, max(evicted.stride(0), width), width, batch, budget, recent, sinks, int(max_seq_len), ws_ptr, ws_bytes)
+        evicted.data_ptr() if width else None, evicted_stride, width, batch, budget, recent, sinks, int(max_seq_len), ws_ptr, ws_bytes)
     if rc:
         _check(rc, "bsgl_evict_tokens")
     return new_lens, evicted

@@ -215,3 +215,16 @@ def test_new_lengths_over_the_old_ones_are_refused(gpu):
     lens = torch.tensor([30, 3], device=gpu)
     with pytest.raises(ValueError, match="overlap"):
         _hip.evict_tokens(t, w, torch.tensor([0, 1], device=gpu), lens, 4, new_lens=lens)
+
+
+def test_evicted_rows_that_share_memory_are_refused(gpu):
+    """Through the fast way as well, which leaves such a tensor to the wrapper."""
+    from baby_sglang_amd import _hip
+
+    t, w = torch.zeros(4, 32, dtype=torch.int32, device=gpu), torch.zeros(4, 32, device=gpu)
+    req, lens = torch.tensor([0, 1, 2], device=gpu), torch.tensor([30, 3, 20], device=gpu)
+    one, new = torch.empty(7, dtype=torch.int32, device=gpu), torch.zeros(3, dtype=torch.int64, device=gpu)
+    for bad in (one.expand(3, 7), torch.as_strided(one, (3, 3), (2, 1))):
+        for kw in ({}, dict(new_lens=new)):
+            with pytest.raises(ValueError, match="evicted"):
+                _hip.evict_tokens(t, w, req, lens, 4, evicted=bad, **kw)

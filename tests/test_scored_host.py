@@ -118,3 +118,27 @@ def test_tensors_off_the_gpu_are_refused():
         _hip.evict_tokens(table, torch.zeros(1, 8), one, one, 2)
     with pytest.raises(RuntimeError):
         _hip.logit_controls(torch.zeros(1, 8))
+
+
+def test_evicted_rows_that_share_memory_are_refused(monkeypatch):
+    """The wrapper's own check of a given `evicted`, on CPU tensors with the launch caught: rows that overlap never reach the library, and
+    the stride that does is the tensor's own."""
+    calls = []
+    monkeypatch.setattr(_hip, "_need_gpu", lambda *t: None)
+    monkeypatch.setattr(_hip, "_same_gpu", lambda *t: None)
+    monkeypatch.setattr(_hip, "_launch", lambda index, fn, *args: calls.append(args) or 0)
+    table, w = torch.zeros(4, 32, dtype=torch.int32), torch.zeros(4, 32)
+    req, lens = torch.tensor([0, 1, 2]), torch.tensor([30, 3, 20])
+    one = torch.empty(7, dtype=torch.int32)
+    for bad in (one.expand(3, 7), torch.as_strided(one, (3, 3), (2, 1)), one[:1].expand(3, 1), torch.empty(7, 3, dtype=torch.int32).t(),
+                torch.empty(2, 7, dtype=torch.int32), torch.empty(3, 7)):
+        with pytest.raises(ValueError, match="evicted"):
+            _hip.evict_tokens(table, w, req, lens, 4, evicted=bad)
+    assert not calls
+    wide = torch.empty(3, 9, dtype=torch.int32)
+    for good, stride, width in ((wide, 9, 9), (wide[:, :5], 9, 5), (wide[:, 2:3], 9, 1), (wide[:, :0], 9, 0)):
+        _hip.evict_tokens(table, w, req, lens, 4, evicted=good)
+        # ... (out_table, out_weights, table, stride, weights, stride, rows, columns, requests, lengths, new lengths, evicted, stride, width, ..)
+        assert calls[-1][12:14] == (stride, width)
+    _hip.evict_tokens(table, w, req[:1], lens[:1], 4, evicted=one.expand(1, 7))
+    assert calls[-1][12:14] == (7, 7)
