@@ -302,6 +302,13 @@ class ServingLoop:
                             max_new_tokens=min(sampling.max_new_tokens, self.max_total_tokens), eos_id=sampling.eos_id)
             self.waiting.append(seq)
             order.append(seq)
+        if self.kv_budget is not None:
+            # (a step appends its token before it evicts; kv_budget + kv_slack fit a row)
+            width = self.req_to_token_pool.max_context_len
+            for i, seq in enumerate(order):
+                if len(seq.input_ids) + (seq.max_new_tokens > 1) > width:
+                    self.waiting = []
+                    raise ValueError(f"request {i}: a prompt of {len(seq.input_ids)} tokens and the next one do not fit a page-table row of {width}")
         while len(self.finished) < len(order):
             batch, mode = self._select()
             if mode == "error":
@@ -682,6 +689,10 @@ class ServingLoop:
         requests' last steps left in the per-row id buffer (overlap mode), not ``output_ids[-1]``;
         with ``gather_ids=False`` they are not gathered here (the forward worker does it on its own
         stream, behind the step that produces them) and ``input_ids`` is a placeholder."""
+        width = self.req_to_token_pool.max_context_len
+        if any(s.seq_len >= width for s in batch):
+            # (on the host: an index past the row ends the process on the GPU, or lands in the next request's)
+            raise RuntimeError(f"a request has filled its page-table row of {width} tokens")
         host_loc, new_slots = self._alloc_slots(len(batch))
         if host_loc is None:
             raise RuntimeError("Failed to allocate KV slots for decode")

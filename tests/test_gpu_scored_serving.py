@@ -278,3 +278,20 @@ def test_slopes_stay_in_32_bits_and_out_of_the_state(gpu):
     assert attn.distance_slopes.dtype == torch.float32 and attn.distance_slopes.device.type == "cuda"
     assert torch.equal(attn.distance_slopes.cpu(), torch.tensor([0.3, 0.1]))
     assert not any("slopes" in k for k in model.state_dict())
+
+
+def test_prompts_as_long_as_their_row(gpu):
+    """32 columns a row: a prompt of 31 leaves room for the next token and is then cut; one of 32 runs where nothing follows it."""
+    from baby_sglang_amd.serving_loop import SamplingParams, ServingLoop
+
+    loop = ServingLoop(tiny_model(gpu, torch.float32), max_total_tokens=64, max_requests=2, kv_budget=8, kv_slack=2)
+    lens = []
+    loop.on_batch = lambda mode, fb: lens.append(fb.seq_lens.tolist())
+    prompt = torch.randint(0, 64, (32,), generator=torch.Generator().manual_seed(3))
+    (out,) = loop.run_batch([prompt[:31]], SamplingParams(max_new_tokens=5))
+    assert len(out) == 5 and lens == [[31], [32], [9], [10], [9]]
+    (out,) = loop.run_batch([prompt], SamplingParams(max_new_tokens=1))
+    assert len(out) == 1
+    with pytest.raises(ValueError, match="row of 32"):
+        loop.run_batch([prompt], SamplingParams(max_new_tokens=2))
+    accounted(loop, 64)

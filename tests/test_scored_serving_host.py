@@ -61,3 +61,34 @@ def test_attention_shim_checks_its_slopes():
     biased = BabyRadixAttention(2, 64, 0.125, 2, 0, logit_cap=30.0, distance_slopes=[0.3, 0.1]).to(torch.bfloat16)
     assert biased.distance_slopes.dtype == torch.float32 and not biased.state_dict()
     assert torch.equal(biased.distance_slopes, torch.tensor([0.3, 0.1]))
+
+
+def _budget_loop(**kw):
+    """A loop on the CPU with a budget's settings put in by hand: what it refuses, it refuses before any model or kernel runs."""
+    from baby_sglang_amd.serving_loop import ServingLoop
+
+    loop = ServingLoop(_Model(), max_total_tokens=64, max_requests=2)
+    loop.kv_budget, loop.kv_recent, loop.kv_sinks, loop.kv_slack = 8, 2, 1, 2
+    for k, v in kw.items():
+        setattr(loop, k, v)
+    return loop
+
+
+def test_budget_refuses_prompts_that_fill_their_row():
+    """A row has 32 columns: the next token of a prompt of 32 would stand in column 32, in the row behind it."""
+    loop = _budget_loop()
+    for n, new in ((32, 2), (33, 1), (33, 5)):
+        with pytest.raises(ValueError, match="request 1"):
+            loop.run_batch([torch.tensor([1, 2]), torch.arange(n) % 8], smp.SamplingParams(max_new_tokens=new))
+        assert not loop.waiting and loop.req_to_token_pool.available_size() == 2
+
+
+def test_a_full_row_is_told_on_the_host():
+    from baby_sglang_amd.serving_loop import Sequence_, ServingLoop
+
+    loop = ServingLoop(_Model(), max_total_tokens=64, max_requests=2)
+    s = Sequence_(input_ids=[1] * 32, max_new_tokens=3, eos_id=-1)
+    s.row, s.seq_len, s.table, s.output_ids = 0, 32, list(range(1, 33)), [3]
+    with pytest.raises(RuntimeError, match="row of 32"):
+        loop._decode_batch([s])
+    assert s.seq_len == 32 and len(s.table) == 32 and loop.token_to_kv_pool.available_size() == 64
