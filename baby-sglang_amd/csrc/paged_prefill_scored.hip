@@ -61,12 +61,6 @@ template <> struct Mma32<f16_tag> {
   }
 };
 
-// Capped scores need no running maximum where the cap itself keeps their exponentials in range: |t| <= cap log2 e, so
-// with the reference fixed at 0 a probability lies in 2^+-87 for a cap of 60, a sum of 2^18 of them times values of up to
-// 2^20 below 2^127, and the smallest row sum is normal; bf16 has the same exponents.  (f16 has not, and a bias has no
-// bound.)  It saves the maxima and the checks of every step.
-constexpr float kFixedCap = 60.f;
-
 // row of the 32x32 accumulator that register r of a lane in half `hi` holds
 __device__ __forceinline__ constexpr int acc_row(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
 
@@ -123,9 +117,8 @@ __device__ __forceinline__ void rescue_row(const PrefillArgs& a, int64_t q_row, 
 // workgroup).  16: for batches of short extends a wave's columns are 2 q heads x 16 positions and
 // the workgroup covers 16 positions x 8 q heads, so a kv head's K/V is streamed by ONE workgroup
 // for up to 8 q heads instead of once per pair of heads.
-// CAP, BIAS: which of the two the call has (see the head of this file).  FIXED (a cap, no bias, bf16): the softmax's reference is 0
-// throughout -- see kFixedCap.
-template <typename Tag, int PW, bool CAP, bool BIAS, bool FIXED = false>
+// CAP, BIAS: which of the two the call has (see the head of this file).
+template <typename Tag, int PW, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void prefill_scored_kernel(PrefillArgs a) {
   using E = Elem<Tag>;
@@ -344,10 +337,20 @@ void prefill_scored_kernel(PrefillArgs a) {
     }
   }
 
-  // reference score of the lane's position, units of log2.  It is only moved when a score exceeds it by 2^6
-  // (the exact row maximum is never needed: probabilities stay below 64).
-  float m_run = kNegInf, m_sub = 0.f;  // m_sub: m_run, or 0 while nothing has been seen
-  constexpr float kSlack = 6.f;
+  // m_run: largest score of the lane's position when it was last looked for, units of log2; m_sub: what its scores are taken
+  // against.  The maximum of a step is looked for only until every row of the wave has seen a token, and where tokens are
+  // masked.  Otherwise the step's probabilities are made first and their sum, which is wanted anyway, tells: if a lane's 16 pass
+  // 2^kTop, the reference moves and they are made again, before a product has met a value.  A move is dear (every lane's 64
+  // sums), so the largest score stands at 2^kLift, well below that.  bf16 has f32's exponents and stands in the middle of them:
+  // 2^-10 to 2^10, 20 of the 2^+-126 that the products with the values have.
+  // (A cap bounds the scores, and a fixed reference of 0 needs no looking at all; but 2^(cap log2 e) times a value is not in range
+  // whatever the value is.)
+  constexpr bool HALF = std::is_same<Tag, f16_tag>::value;
+  constexpr float kLift = HALF ? 0.f : -10.f, kTop = HALF ? 6.f : 10.f;
+  constexpr float kMostSum = HALF ? 0x1p6f : 0x1p10f;
+  constexpr float kSlack = HALF ? 6.f : kTop - kLift - 4.f;  // (16 scores this far above m_run come to 2^kTop)
+  float m_run = kNegInf, m_sub = 0.f;           // (while nothing has been seen)
+  bool all_seen = false;                        // (wave-uniform)
   float l_run = 0.f;  // sum of this lane's probabilities (its 16 tokens of every step)
   f32x16 o_acc[4];
 #pragma unroll
@@ -429,7 +432,6 @@ void prefill_scored_kernel(PrefillArgs a) {
 
   const int n_groups = n_steps;  // (a step is the unit of requests, waits and barriers)
   f32x16 sc_a, sc_b;
-  float ext_nx = kHidden;
   if (n_groups > 0) {
     read_offsets(0);
     make_src();
@@ -440,8 +442,7 @@ void prefill_scored_kernel(PrefillArgs a) {
   if (n_groups > 3) read_offsets(3);
 
   // sc_a, sc_b: the u of the step about to be consumed, and the raw scores, then u, of the one after it: the
-  // two trade places from step to step.  ext_nx: the lane's extreme u of the step that comes next, found in
-  // the shadow of its predecessor's PV products (steps that need the mask look again, after masking)
+  // two trade places from step to step.  ext16: the extreme u of a lane
   auto ext16 = [&](const f32x16& v) {
     float m = ext3(v[0], v[1], v[2]);
 #pragma unroll
@@ -469,7 +470,6 @@ void prefill_scored_kernel(PrefillArgs a) {
       sc_a = scores(kf);
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc_a[r] = shape(sc_a[r], r);
-      ext_nx = ext16(sc_a);
     }
   }
 
@@ -536,28 +536,15 @@ void prefill_scored_kernel(PrefillArgs a) {
       const bool hides = step * STEP < full_from || step * STEP + STEP > full_to;  // wave-uniform
       const bool looks_ahead = BIAS && step * STEP < wave_pos;
       const float c_step = step_c(step);
-      float ext = ext_nx;
-      if (__builtin_expect(hides || looks_ahead, 0)) {  // (rare: the ends of the rows' intervals, and prefixes read both ways)
-        int t0m = step * STEP + 4 * hi;
-        asm volatile("" : "+v"(t0m));
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int t = t0m + acc_row(r, 0);
-          // (the bias above is slope * (j - i), which is what is wanted up to the row's own position)
-          if constexpr (BIAS) sc[r] = fmaf(-2.f * slope_u, (float)max(my_pos - t, 0), sc[r]);
-          sc[r] = (t >= my_lo && t < my_hi) ? sc[r] : kHidden;
-        }
-        if (!FIXED) ext = ext16(sc);
-      }
-      const float lmax = fmaf(ext, A, c_step);
-      if (!FIXED && __builtin_expect(__any(lmax > m_run + kSlack), 0)) {  // (rare after the first steps)
+      // moves the reference of every row to its largest score so far (`lmax`: the lane's)
+      auto move_reference = [&](float lmax) __attribute__((always_inline)) {
         float x = lmax, y = lmax;
         swap32(x, y);  // the partner lane holds the position's other 16 tokens
         const float m_new = max3(m_run, x, y);
         // a position with nothing visible yet keeps m = -inf: its factor is 1, not exp2(nan)
         const float alpha = m_new == kNegInf ? 1.f : fast_exp2(m_run - m_new);
         m_run = m_new;
-        m_sub = m_new == kNegInf ? 0.f : m_new;  // masked scores: exp2(-inf) = 0
+        m_sub = m_new == kNegInf ? 0.f : m_new - kLift;  // masked scores: exp2(-inf) = 0
         l_run *= alpha;
         // O has its positions in the registers: register r of this lane belongs to position
         // acc_row(r, hi), whose factor lives on lane acc_row(r, hi)
@@ -567,8 +554,22 @@ void prefill_scored_kernel(PrefillArgs a) {
 #pragma unroll
           for (int db = 0; db < 4; ++db) o_acc[db][r] *= ar;
         }
+      };
+      if (__builtin_expect(hides || looks_ahead || !all_seen, 0)) {  // (rare: the ends of the rows' intervals, and prefixes read both ways)
+        int t0m = step * STEP + 4 * hi;
+        asm volatile("" : "+v"(t0m));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int t = t0m + acc_row(r, 0);
+          // (the bias above is slope * (j - i), which is what is wanted up to the row's own position)
+          if constexpr (BIAS) sc[r] = fmaf(-2.f * slope_u, (float)max(my_pos - t, 0), sc[r]);
+          sc[r] = (t >= my_lo && t < my_hi) ? sc[r] : kHidden;
+        }
+        const float lmax = fmaf(ext16(sc), A, c_step);
+        if (__any(lmax > m_run + kSlack)) move_reference(lmax);
+        all_seen = !__any(live && m_run == kNegInf);
       }
-      const float c0 = FIXED ? c_step : c_step - m_sub;
+      float c0 = c_step - m_sub;
 
       // ---- from here to the end of the step: one basic block, issued in the order written ----
       // (a scheduling barrier after every product: the compiler's own order puts the vector
@@ -586,7 +587,7 @@ void prefill_scored_kernel(PrefillArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sn[r] = 0.f;
       float e[16], p[16];
-      float mx0 = kHidden, mx1 = kHidden;
+      float sum = 0.f;  // of the lane's probabilities of this step
       uint32_t pw[8];  // probabilities, two to a word: words 4 kk .. 4 kk + 3 = the A operand of tile kk
       uint4 vf[4];  // V fragments travel three products ahead of their use
       e[0] = fmaf(sc[0], A, c0);
@@ -603,8 +604,23 @@ void prefill_scored_kernel(PrefillArgs a) {
         }
         if (kb >= 4) pw[kb - 4] = E::pack2(p[2 * (kb - 4)], p[2 * (kb - 4) + 1]);
         if (kb >= 5) vf[kb - 5] = v_frag(kb - 5);
+        if (kb >= 1) sum = (sum + p[2 * kb - 2]) + p[2 * kb - 1];
         __builtin_amdgcn_sched_barrier(0);
       }
+      sum = (sum + p[14]) + p[15];
+      if (__builtin_expect(__any(sum > kMostSum), 0)) {
+        move_reference(fmaf(ext16(sc), A, c_step));
+        c0 = c_step - m_sub;
+        sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          p[r] = fast_exp2(fmaf(sc[r], A, c0));
+          sum += p[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pw[r] = E::pack2(p[2 * r], p[2 * r + 1]);
+      }
+      l_run += sum;
       // k-values of a lane in PV product i: registers 8 kk .. 8 kk + 7 of the score accumulator,
       // i.e. tokens {0-3, 8-11} + 4 hi of tile kk = i >> 2
 #pragma unroll
@@ -613,17 +629,13 @@ void prefill_scored_kernel(PrefillArgs a) {
         o_acc[i & 3] = Mma32<Tag>::mm(make_uint4(pw[4 * kk], pw[4 * kk + 1], pw[4 * kk + 2], pw[4 * kk + 3]), vf[i % 4], o_acc[i & 3]);
         if (i + 3 < 8) vf[(i + 3) % 4] = v_frag(i + 3);
         if (i < 4) pw[4 + i] = E::pack2(p[8 + 2 * i], p[8 + 2 * i + 1]);
-        l_run = (l_run + p[2 * i]) + p[2 * i + 1];
         // (the next step's scores are complete by now: three of them per gap)
         if (i >= 2) {
 #pragma unroll
           for (int r = 3 * (i - 2); r < (i == 7 ? 16 : 3 * (i - 1)); ++r) sn[r] = shape(sn[r], r);
-          if (!FIXED) mx0 = ext3(mx0, sn[3 * (i - 2)], sn[3 * (i - 2) + 1]);
-          if (!FIXED) mx1 = i == 7 ? ext3(mx1, sn[14], sn[15]) : ext3(mx1, sn[3 * (i - 2) + 2], sn[3 * (i - 2) + 2]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (!FIXED) ext_nx = ext3(mx0, mx1, mx1);
       __builtin_amdgcn_s_setprio(0);
     };
     static_assert(NSTAGE == 4, "the step loop below is unrolled over the ring");
@@ -702,8 +714,6 @@ template <typename Tag, int PW>
 void launch_shape(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
   const bool cap = a.mods.cap > 0.f, bias = a.mods.slopes != nullptr;
   if (cap && bias) hipLaunchKernelGGL((prefill_scored_kernel<Tag, PW, true, true>), grid, dim3(256), 0, stream, a);
-  else if (std::is_same<Tag, bf16_tag>::value && cap && a.mods.cap <= kFixedCap)
-    hipLaunchKernelGGL((prefill_scored_kernel<bf16_tag, PW, true, false, true>), grid, dim3(256), 0, stream, a);
   else if (cap) hipLaunchKernelGGL((prefill_scored_kernel<Tag, PW, true, false>), grid, dim3(256), 0, stream, a);
   else if (bias) hipLaunchKernelGGL((prefill_scored_kernel<Tag, PW, false, true>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((prefill_scored_kernel<Tag, PW, false, false>), grid, dim3(256), 0, stream, a);

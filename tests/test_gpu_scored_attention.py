@@ -803,3 +803,18 @@ def test_extend_sorted_list_kept_and_replayed(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("cap", [30.0, 60.0])
+@pytest.mark.parametrize("side,power", [(1.0, 60), (1.0, 100), (-1.0, -60)])
+def test_extend_values_of_the_whole_range(gpu, cap, side, power):
+    """Scores at one end of the cap's range and values far from 1: 2^power times a probability of 2^(cap log2 e) is no bf16, nor is what
+    2^-60 times 2^-(cap log2 e) leaves of it, and the result is as finite as the values are.  (Products of 2^10 with up to 103 values of 5.5 x
+    2^100 stay below 2^120.)"""
+    def poison(c, row_req, row_pos, st, sp):
+        c["k"][:] = c["k"].abs()
+        c["q"][::2] = (c["q"][::2].abs() * 40.0 * side).to(c["q"].dtype)
+        c["v"] *= 2.0**power
+
+    extend_case(gpu, "1.5b", torch.bfloat16, [90, 33], [0, 70], cap=cap, seed=70, poison=poison, variant=2)
+    extend_case(gpu, "1.5b", torch.bfloat16, [9, 3], [0, 70], cap=cap, seed=71, poison=poison, variant=2)
