@@ -51,6 +51,11 @@ template <typename Tag> __device__ __forceinline__ f32x4v score_product(u32x4v k
 }
 
 // waves per SIMD the registers of an instance allow
+// The largest score of a tile stands at 2^kLift: f16, whose probabilities enter the second product as they are, ends at 2^16, and what is
+// below 2^-25 is lost from the product but not from the sum -- 2^-40 from the largest score, nothing for rows of any length; with it
+// at 1, a tail of 60000 tokens of 2^-26 each loses 2^-10 of the row.
+template <typename Tag> constexpr float kLift = std::is_same<Tag, f16_tag>::value ? 15.f : 0.f;
+
 template <typename Tag, int D> constexpr int occupancy() { return std::is_same<Tag, f32_tag>::value && D == 128 ? 3 : 4; }
 
 // ROWS: extend tokens as rows (ScoreMods::rows), else requests
@@ -286,7 +291,7 @@ void decode_scored_kernel(DecodeArgs a) {
       const float m_new = fmaxf(m_run, t_max);
       const float alpha = m_new == kNegInf ? 1.f : fast_exp2(m_run - m_new);
       m_run = m_new;
-      m_sub = m_new == kNegInf ? 0.f : m_new;
+      m_sub = m_new == kNegInf ? 0.f : m_new - kLift<Tag>;
       l_run *= alpha;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -379,7 +384,7 @@ void decode_scored_kernel(DecodeArgs a) {
       for (int k = 0; k < 4; ++k) o[k] = fmaf(x[k], f, o[k]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const float lse = l == 0.f ? kNegInf : ((m == kNegInf ? 0.f : m) + __builtin_amdgcn_logf(l)) * kLn2;
+    const float lse = l == 0.f ? kNegInf : ((m == kNegInf ? 0.f : m - kLift<Tag>) + __builtin_amdgcn_logf(l)) * kLn2;
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[k] *= inv;
     if (direct) {

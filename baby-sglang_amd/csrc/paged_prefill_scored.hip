@@ -342,13 +342,14 @@ void prefill_scored_kernel(PrefillArgs a) {
   // masked.  Otherwise the step's probabilities are made first and their sum, which is wanted anyway, tells: if a lane's 16 pass
   // 2^kTop, the reference moves and they are made again, before a product has met a value.  A move is dear (every lane's 64
   // sums), so the largest score stands at 2^kLift, well below that.  bf16 has f32's exponents and stands in the middle of them:
-  // 2^-10 to 2^10, 20 of the 2^+-126 that the products with the values have.
+  // 2^-10 to 2^10, 20 of the 2^+-126 that the products with the values have.  f16 ends at 2^16, and what is below 2^-25 is lost from the
+  // product (not from the sum): from the largest score, at 2^6, that is 2^-31, 2^-14 in all for 131072 tokens.
   // (A cap bounds the scores, and a fixed reference of 0 needs no looking at all; but 2^(cap log2 e) times a value is not in range
   // whatever the value is.)
   constexpr bool HALF = std::is_same<Tag, f16_tag>::value;
-  constexpr float kLift = HALF ? 0.f : -10.f, kTop = HALF ? 6.f : 10.f;
-  constexpr float kMostSum = HALF ? 0x1p6f : 0x1p10f;
-  constexpr float kSlack = HALF ? 6.f : kTop - kLift - 4.f;  // (16 scores this far above m_run come to 2^kTop)
+  constexpr float kLift = HALF ? 6.f : -10.f, kTop = HALF ? 15.f : 10.f;
+  constexpr float kMostSum = HALF ? 0x1p15f : 0x1p10f;
+  constexpr float kSlack = kTop - kLift - 4.f;  // (16 scores this far above m_run come to 2^kTop)
   float m_run = kNegInf, m_sub = 0.f;           // (while nothing has been seen)
   bool all_seen = false;                        // (wave-uniform)
   float l_run = 0.f;  // sum of this lane's probabilities (its 16 tokens of every step)

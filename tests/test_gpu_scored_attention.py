@@ -818,3 +818,50 @@ def test_extend_values_of_the_whole_range(gpu, cap, side, power):
 
     extend_case(gpu, "1.5b", torch.bfloat16, [90, 33], [0, 70], cap=cap, seed=70, poison=poison, variant=2)
     extend_case(gpu, "1.5b", torch.bfloat16, [9, 3], [0, 70], cap=cap, seed=71, poison=poison, variant=2)
+
+
+@pytest.mark.parametrize("ext", [1, 40, 300])
+@pytest.mark.parametrize("cap", [0.0, 40.0])
+def test_f16_long_flat_tails(gpu, ext, cap):
+    """Tokens of score 18.5 among 60000 of score 0, which are 2^-26.7 of one of them each: a probability that f16 cannot hold beside 1, all
+    together a part of the row that it can.  The values of the few are 0, so that the tail is all there is of the result.  Extend: one such
+    token, ahead of the new ones (the stream goes from the last one back); decode: four in every 512, in f32, so that every piece has some.
+
+    A probability is rounded to 2^-11 of itself, or to a step of 2^-25 where it is below 2^-14: the kernels hold the largest at 2^6 or more, so a
+    token of 2^-26.7 stands at 2^-20.7 and is off by 2^-4.3 of itself at most, all of them alike; the rest of the bound is as above (score
+    error: products of 128 terms, all but one of them 0, a top of 20)."""
+    from baby_sglang_amd import _hip
+
+    n, hq, hkv, dim = 60000, 2, 1, 128
+    s = cap * math.tanh(18.5 / cap) if cap else 18.5
+    ds = score_error(torch.tensor(20.0), cap, torch.tensor(s), dim).item()
+    rel = 2.0**-4.3 + 2 * ds + 2.0**-21 + n * 2.0**-23
+    table = torch.arange(n + ext, dtype=torch.int32, device=gpu)[None].contiguous()
+    q = torch.zeros((ext, hq, dim), dtype=torch.float16, device=gpu)
+    q[:, :, 0] = 1.0
+    req, seq = torch.zeros(1, dtype=torch.int64, device=gpu), torch.tensor([n + ext], device=gpu)
+    for decode in (False, True):
+        kv = torch.zeros((n + ext, 2, hkv, dim), dtype=torch.float16, device=gpu)
+        kv[:, 1] = 1.0
+        few = torch.tensor([i + 5 + 16 * w for i in range(0, n - 64, 512) for w in range(4)] if decode else [n - 1], device=gpu)
+        kv[few, 0, 0, 0], kv[few, 1] = 18.5, 0.0
+        if decode:
+            out = _hip.paged_decode_scored(q[:1], kv[:, 0], kv[:, 1], table, req, seq, scale=1.0, logit_cap=cap, out_dtype=torch.float32)
+        else:
+            out = _hip.paged_prefill_scored(q, kv[:, 0], kv[:, 1], table, req, seq, seq - ext, torch.tensor([ext], device=gpu), scale=1.0, logit_cap=cap,
+                                            variant=2 if ext > 1 else 0)
+        rows = [n + ext] if decode else [n + i + 1 for i in range(ext)]
+        want = torch.tensor([(m - len(few)) / (m - len(few) + len(few) * math.exp(s)) for m in rows], dtype=torch.float64)[:, None]
+        step = 0.0 if decode else 2.0**-11 * want + 2.0**-25
+        assert bool(((out.double().cpu() - want).abs() <= step + rel * want).all()), (decode, (out.double().cpu() / want).aminmax())
+
+
+@pytest.mark.parametrize("power", [-14, 15])
+def test_f16_values_at_the_ends_of_the_type(gpu, power):
+    """Probabilities that stand high in f16 do not make large values infinite, nor small ones less exact than f16 is."""
+    def poison(c, row_req, row_pos, st, sp):
+        c["v"][:] = (c["v"].clamp(-1.9, 1.9) * 2.0**power).to(c["v"].dtype)
+
+    for heads, ext, pre in (("1.5b", [90, 33], [0, 70]), ("0.5b", [9, 3], [0, 700]), ("7b", [1, 2], [300, 20])):
+        extend_case(gpu, heads, torch.float16, ext, pre, cap=20.0, seed=72, poison=poison)
+        extend_case(gpu, heads, torch.float16, ext, pre, slopes=True, seed=73, poison=poison)
