@@ -24,6 +24,10 @@ typedef __attribute__((ext_vector_type(4))) float f32x4;
 constexpr int kTokens = 256;  // tokens per workgroup: four per lane of a wave
 constexpr int kWaves = 4;     // that share the heads
 
+// a head's log-sum-exp as what its scores are taken against.  A head whose visible scores are all -inf (an infinity in K) has one of
+// -inf and gives its tokens nothing: -inf - -inf would be NaN, which a weight never loses again.  (A NaN among the scores passes.)
+__device__ __forceinline__ float against(float lse) { return lse == kNegInf ? -kNegInf : lse * kLog2e; }
+
 __global__ __launch_bounds__(64 * kWaves) void token_weights_kernel(WeightsArgs a) {
   __shared__ f32x4 s_sum[kWaves][64];
   __shared__ int s_same[kWaves];
@@ -58,7 +62,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_weights_kernel(WeightsArgs 
 #pragma unroll 4
       for (int h = wave; h < a.n_q_heads; h += kWaves) {
         const f32x4 s = *(const f32x4*)(src + h * a.mods.score_stride + t);
-        const float l = lse[h] * kLog2e;
+        const float l = against(lse[h]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) w[k] += fast_exp2(s[k] - l);
       }
@@ -103,7 +107,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_weights_kernel(WeightsArgs 
       if (t < 0 || t >= r.y) continue;
       any = true;
       const float* si = a.mods.scores + (int64_t)i * a.n_q_heads * a.mods.score_stride;
-      for (int h = 0; h < a.n_q_heads; ++h) sum += fast_exp2(si[h * a.mods.score_stride + t] - a.lse[(int64_t)i * a.n_q_heads + h] * kLog2e);
+      for (int h = 0; h < a.n_q_heads; ++h) sum += fast_exp2(si[h * a.mods.score_stride + t] - against(a.lse[(int64_t)i * a.n_q_heads + h]));
     }
     const int64_t at = req * a.row_stride + c;
     if (any) a.out[at] = a.old[at] + sum;

@@ -865,3 +865,42 @@ def test_f16_values_at_the_ends_of_the_type(gpu, power):
     for heads, ext, pre in (("1.5b", [90, 33], [0, 70]), ("0.5b", [9, 3], [0, 700]), ("7b", [1, 2], [300, 20])):
         extend_case(gpu, heads, torch.float16, ext, pre, cap=20.0, seed=72, poison=poison)
         extend_case(gpu, heads, torch.float16, ext, pre, slopes=True, seed=73, poison=poison)
+
+
+@pytest.mark.parametrize("variant", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("same_row", [False, True])
+def test_weights_of_scores_that_are_all_minus_infinity(gpu, dtype, variant, same_row):
+    """-inf in every visible key of kv head 0: its q heads get zeros and give no weight; those of the other kv head give theirs.  A request of
+    one row and two requests of the same row (which are added up another way)."""
+    from baby_sglang_amd import _hip
+
+    c = make(74, "1.5b", dtype, [90, 300], q_rows=3)
+    c["q"] = c["q"].abs() + 0.5
+    c["k"][c["table"][c["req"][0], :90].long(), 0, 5] = float("-inf")
+    d = to_gpu(c, gpu)
+    pick = torch.tensor([0, 1, 0] if same_row else [0, 1], device=gpu)
+    n = len(pick)
+    old = torch.rand(d["table"].shape, device=gpu)
+    w = old.clone()
+    out = _hip.paged_decode_scored(d["q"][:n], d["k"], d["v"], d["table"], d["req"][pick], d["seq"][pick], token_weights=w, variant=variant).view(n, 12, 128)
+    finite = {k: v.clone() for k, v in c.items() if torch.is_tensor(v)}
+    finite["k"][~finite["k"].isfinite()] = 0.0
+    rows = c["table"][c["req"]][pick.cpu()]
+    want, mass, lse, received, top = orc.scored_exact(finite["q"][:n], finite["k"], finite["v"], rows, [c["lens"][i] for i in pick.tolist()], range(n),
+                                                      [c["lens"][i] - 1 for i in pick.tolist()], 128**-0.5)
+    ds = score_error(top, 0.0, lse, 128).max().item()
+    expect = old.double().cpu()
+    slack = torch.zeros_like(expect)
+    for i, at in enumerate(pick.tolist()):
+        m, r = c["lens"][at], int(c["req"][at])
+        if at == 0:
+            assert not bool(out[i, :6].any())
+            q, k = finite["q"][i, 6:].double(), finite["k"][rows[i, :m].long()][:, 1].double()
+            got = torch.softmax(q @ k.t().contiguous() * 128**-0.5, -1).sum(0)
+        else:
+            got = received[i]
+        expect[r, :m] += got
+        slack[r, :m] += got * (4 * ds + 2.0**-20 + m * 2.0**-23)
+    assert bool(out.isfinite().all())
+    assert bool(((w.double().cpu() - expect).abs() <= slack + 2.0**-22 * expect).all())
