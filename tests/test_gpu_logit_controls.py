@@ -238,3 +238,30 @@ def test_a_history_without_columns(gpu):
     got = _hip.logit_controls(x, history=torch.zeros((2, 0), dtype=torch.int32, device=gpu), history_lens=torch.zeros(2, dtype=torch.int64, device=gpu),
                               repetition=1.5, presence=1.0)
     assert torch.equal(got, x)
+
+
+def test_the_repetition_penalty_is_the_quotient(gpu):
+    """x / repetition in 32 bits, rounded once, is one number: that of the torch division, for ordinary penalties and for those whose
+    reciprocal is no normal number or none at all; in 16 bits it is rounded a second time, as the torch one is."""
+    from baby_sglang_amd import _hip
+
+    vocab = 5000
+    for rep in (1.3, 1.1, 0.7, 3.0, 1e-38, 2e-39, 1e-44, 1e38, 3e38):
+        r = torch.tensor(rep, dtype=torch.float32)
+        for dtype in (torch.float32, torch.bfloat16, torch.float16):
+            x = (3 * torch.randn(4, vocab, generator=torch.Generator().manual_seed(5))).to(dtype)
+            x[0, :4] = torch.tensor([0.0, -0.0, 65504.0, 6e-8]).to(dtype)
+            hist = torch.arange(vocab, dtype=torch.int32).repeat(4, 1)
+            lens = [vocab, 3000, 1, 0]
+            want = x.clone()
+            for i, n in enumerate(lens):
+                f = x[i, :n].float()
+                want[i, :n] = torch.where(f > 0, f / r, f * r).to(dtype)
+            got = _hip.logit_controls(x.to(gpu), history=hist.to(gpu), history_lens=torch.tensor(lens, device=gpu), repetition=torch.full((4,), r.item(), device=gpu))
+            ok = (got.cpu() == want) | (f_tiny(want) & f_tiny(got.cpu()))
+            assert bool(ok.all()), (rep, dtype, got.cpu()[~ok][:4], want[~ok][:4])
+
+
+def f_tiny(t):
+    """(subnormal results may be flushed)"""
+    return t.float().abs() < 2.0**-126
