@@ -5,6 +5,8 @@
 #include "bsgl_device.h"
 #include "bsgl_launch.h"
 
+#include <type_traits>
+
 namespace bsgl {
 
 // {first visible position, number of visible positions} of a row, inside [0, seq): `to_default` is the end
@@ -53,5 +55,43 @@ struct ScoreShape {
     return fmaf(-slope, dist, s);
   }
 };
+
+// a 16-byte piece of a row holds an infinity or a NaN
+template <typename Tag> __device__ __forceinline__ bool not_finite(const uint4& x) {
+  constexpr uint32_t e = std::is_same<Tag, f32_tag>::value ? 0x7f800000u : std::is_same<Tag, bf16_tag>::value ? 0x7f80u : 0x7c00u;
+  bool bad = false;
+  for (uint32_t w : {x.x, x.y, x.z, x.w}) {
+    bad |= (w & e) == e;
+    if constexpr (!std::is_same<Tag, f32_tag>::value) bad |= (w >> 16 & e) == e;
+  }
+  return bad;
+}
+
+// Extend kernels: whether this lane's row has met the values of a token that it does not see -- P . V multiplies them by an exact zero -- and
+// one of them is no number.  That can only be in a step of 32 places that some row of the wave does not see whole; places are counted from the last
+// token back, those past `kv_len` repeat it, the row sees [lo, hi) of them and every live row sees [full_from, full_to).  `v`: byte 0 of the kv head's
+// part of slot 0.  (Run only where a row came out NaN: the tokens are read once, 16 bytes a lane.)
+template <typename Tag, int ROW>
+__device__ __forceinline__ bool met_unseen(const char* v, int64_t slab_row_bytes, const int32_t* table_row, uint32_t max_slot, int kv_len, int wave_len,
+                                           int full_from, int full_to, int lo, int hi) {
+  constexpr int LPT = ROW / 16, TPL = 64 / LPT;  // lanes per token, tokens per load
+  const int lane = threadIdx.x & 63;
+  bool met = false;
+  for (int t0 = 0; t0 < min(kv_len, wave_len); t0 += 32) {
+    if (t0 >= full_from && t0 + 32 <= full_to) continue;
+    uint32_t odd = 0;  // the step's tokens with such a value
+#pragma unroll 4
+    for (int q = 0; q < 32; q += TPL) {
+      uint32_t slot = (uint32_t)table_row[max(kv_len - 1 - (t0 + q + lane / LPT), 0)];
+      slot = slot > max_slot ? max_slot : slot;
+      const unsigned long long b = __ballot(not_finite<Tag>(*(const uint4*)(v + slot * slab_row_bytes + 16 * (lane % LPT))));
+#pragma unroll
+      for (int k = 0; k < TPL; ++k) odd |= (b >> (k * LPT) & ((1ull << LPT) - 1)) != 0 ? 1u << (q + k) : 0u;
+    }
+    auto below = [&](int t) { return t <= t0 ? 0u : t >= t0 + 32 ? ~0u : (1u << (t - t0)) - 1; };
+    met |= (odd & ~(below(hi) & ~below(lo))) != 0;
+  }
+  return met;
+}
 
 }  // namespace bsgl

@@ -35,8 +35,9 @@ __device__ __forceinline__ constexpr int acc_row(int r, int hi) { return (r & 3)
 // where token t's 16-byte piece p stands in its row: p ^ deal(t)
 __device__ __forceinline__ constexpr int deal(int t) { return t ^ (((t >> 2) & 1) << 3); }
 
-// One query row of one head by itself, from the tokens [lo, hi) it sees.  Slow, and only ever run for rows that came out NaN: a
-// product multiplies the values of a token that the row must not see by an exact zero, and 0 * NaN is NaN.
+// One query row of one head by itself, from the tokens [lo, hi) it sees, 8 of them on their way at a time.  Slow, and only ever run for
+// rows that met_unseen names: a product multiplies the values of a token that the row must not see by an exact zero, and
+// 0 * NaN is NaN.
 template <int D>
 __device__ __forceinline__ void rescue_row(const PrefillArgs& a, int64_t q_row, int head, int kvh, int64_t req, int pos, int lo, int hi, int split) {
   constexpr int N = D / 64;
@@ -51,21 +52,45 @@ __device__ __forceinline__ void rescue_row(const PrefillArgs& a, int64_t q_row, 
   }
   const int32_t* table_row = a.kv.table + req * a.kv.table_row_stride;
   const uint32_t max_slot = (uint32_t)(a.kv.n_slots - 1);
-  for (int j = lo; j < hi; ++j) {
-    uint32_t slot = (uint32_t)table_row[j];
-    slot = slot > max_slot ? max_slot : slot;
-    const int64_t at = (int64_t)slot * a.kv.slab_row_stride + (int64_t)kvh * D + N * lane;
-    const float *k = (const float*)a.kv.k_slab + at, *v = (const float*)a.kv.v_slab + at;
-    float dot = 0.f;
+  constexpr int B = 8;
+  for (int j0 = lo; j0 < hi; j0 += B) {
+    float k[B][N], v[B][N], s[B], mn = m;
 #pragma unroll
-    for (int i = 0; i < N; ++i) dot = fmaf(q[i], k[i], dot);
-    const float s = shape.precise(group_sum<64>(dot), (float)abs(pos - j));
-    const float mn = s > m ? s : m;
-    const float alpha = mn == kNegInf ? 1.f : fast_exp2(m - mn), p = s == kNegInf ? 0.f : fast_exp2(s - mn);
+    for (int i = 0; i < B; ++i) {
+      uint32_t slot = (uint32_t)table_row[min(j0 + i, hi - 1)];
+      slot = slot > max_slot ? max_slot : slot;
+      const int64_t at = (int64_t)slot * a.kv.slab_row_stride + (int64_t)kvh * D + N * lane;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        k[i][n] = ((const float*)a.kv.k_slab)[at + n];
+        v[i][n] = ((const float*)a.kv.v_slab)[at + n];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      float dot = 0.f;
+#pragma unroll
+      for (int n = 0; n < N; ++n) dot = fmaf(q[n], k[i][n], dot);
+      s[i] = shape.precise(group_sum<64>(dot), (float)abs(pos - (j0 + i)));
+      if (j0 + i >= hi) {
+        s[i] = kNegInf;
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[i][n] = 0.f;
+      }
+      mn = s[i] > mn ? s[i] : mn;
+    }
+    const float alpha = mn == kNegInf ? 1.f : fast_exp2(m - mn);
     m = mn;
-    l = l * alpha + p;
+    l *= alpha;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * alpha + p * v[i];
+    for (int n = 0; n < N; ++n) o[n] *= alpha;
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const float p = s[i] == kNegInf ? 0.f : fast_exp2(s[i] - mn);
+      l += p;
+#pragma unroll
+      for (int n = 0; n < N; ++n) o[n] += p * v[i][n];
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float* dst = (float*)a.out + q_row * a.out_row_stride + (int64_t)head * D + N * lane;
@@ -333,7 +358,18 @@ void prefill_scored_f32_kernel(PrefillArgs a) {
     if (b & 0xffffffffull) bad |= 1u << acc_row(r, 0);
     if (b >> 32) bad |= 1u << acc_row(r, 1);
   }
-  // rows that came out NaN: again, by themselves
+  // rows that came out NaN and have met a value that they do not see (not those with a NaN among the scores they do see): again, by themselves
+  bad &= ~(uint32_t)__ballot(l_all != l_all);
+  if (bad != 0) {
+    int g0 = live ? my_lo : 0, g1 = live ? my_hi : 0x7fffffff;  // what every row of the wave sees
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      g0 = max(g0, __shfl_xor(g0, d));
+      g1 = min(g1, __shfl_xor(g1, d));
+    }
+    bad &= (uint32_t)__ballot(met_unseen<f32_tag, ROW>((const char*)a.kv.v_slab + (int64_t)kvh * ROW, a.kv.slab_row_stride * 4, table_row, max_slot, kv_len,
+                                                       wave_hi, __builtin_amdgcn_readfirstlane(g0), __builtin_amdgcn_readfirstlane(g1), my_lo, my_hi));
+  }
   if (bad != 0) __builtin_amdgcn_s_waitcnt(0x0F70);  // (behind the stores above, which went to the same rows)
   while (bad != 0) {
     const int r = __ffs((int)bad) - 1;

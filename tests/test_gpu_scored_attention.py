@@ -904,3 +904,41 @@ def test_weights_of_scores_that_are_all_minus_infinity(gpu, dtype, variant, same
         slack[r, :m] += got * (4 * ds + 2.0**-20 + m * 2.0**-23)
     assert bool(out.isfinite().all())
     assert bool(((w.double().cpu() - expect).abs() <= slack + 2.0**-22 * expect).all())
+
+
+@pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("0.5b", torch.float16), ("1.5b", torch.float32)])
+@pytest.mark.parametrize("what", ["k", "v", "one value"])
+def test_extend_that_sees_a_nan_takes_no_longer(gpu, heads, dtype, what):
+    """A NaN in the prefix, in front of every row: the rows are NaN (in its column, where it is one value) and the launch takes what it
+    takes without.  20 times that and a millisecond is far from noise, and from rows computed again one by one."""
+    from baby_sglang_amd import _hip
+
+    c = make(75, heads, dtype, [4300], q_rows=300)
+    d = to_gpu(c, gpu)
+    args = (d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.tensor([4000], device=gpu), torch.tensor([300], device=gpu))
+
+    def timed():
+        best = float("inf")
+        for _ in range(4):
+            t0, t1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            t0.record()
+            out = _hip.paged_prefill_scored(*args, logit_cap=10.0, variant=2)
+            t1.record()
+            torch.cuda.synchronize()
+            best = min(best, t0.elapsed_time(t1))
+        return out.view(300, c["hq"], c["dim"]), best
+
+    clean, before = timed()
+    slot = c["table"][c["req"][0], 5].long().item()
+    if what == "one value":
+        d["v"][slot, :, 3] = float("nan")
+    else:
+        d[what][slot] = float("nan")
+    got, after = timed()
+    if what == "one value":
+        assert bool(got[:, :, 3].isnan().all())
+        rest = [i for i in range(c["dim"]) if i != 3]
+        assert torch.equal(got[:, :, rest], clean[:, :, rest])
+    else:
+        assert bool(got.isnan().all())
+    assert after <= 20 * before + 1.0, (before, after)
