@@ -434,6 +434,7 @@ void decode_scored_kernel(DecodeArgs a) {
         const int p = min(p0 + j, n_parts - 1);
         x[j] = __builtin_bit_cast(f32x4v, __builtin_amdgcn_raw_buffer_load_b128(all_rsrc, p * part_stride + (h * D + 4 * c4) * 4, 0, 16));
         w[j] = p0 + j < n_parts ? s_w[h][p] : 0.f;
+        if (p0 + j >= n_parts) x[j] = f32x4v{0.f, 0.f, 0.f, 0.f};  // (0 times an infinity is none)
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256) void merge_states_kernel(MergeArgs a) {
   const int64_t part_stride = n_rh * D;
   for (int p0 = 0; p0 < a.n_parts; p0 += 8) {
     // 8 parts per round so their loads are in flight together; parts past the end
-    // re-read the last one with weight 0
+    // re-read the last one and count as zeros (a weight of 0 alone does not do it: 0 times infinity)
     float w[8];
     float2 v[8];
 #pragma unroll
@@ -292,6 +292,7 @@ __global__ __launch_bounds__(256) void merge_states_kernel(MergeArgs a) {
       w[j] = p0 + j < a.n_parts ? __shfl(my_w, p) : 0.f;
       if constexpr (EPL == 2) v[j] = *(const float2*)(po + p * part_stride);
       else v[j] = make_float2(po[p * part_stride], 0.f);
+      if (p0 + j >= a.n_parts) v[j] = make_float2(0.f, 0.f);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

@@ -261,7 +261,8 @@ int bsgl_paged_decode_static(void* out /*device*/, int64_t out_row_stride,
  * [0, seq_len).  Default: from 0 to the row's own position, that one included.  Given, visible_to may lie behind the
  * row's own position (prefixes read in both directions); document and window masks are a visible_from.
  * A row whose interval is empty gets zeros (and a log-sum-exp of -inf), and so does a head whose visible scores are all -inf;
- * either gives no token a weight.  Tokens that no row of a call
+ * either gives no token a weight.  A value that is not finite makes its column infinite or NaN in the rows that see it, and in no
+ * others.  Tokens that no row of a call
  * may see are not read, whatever they hold.  (Sums of products with the values are held in f32, up to 2^10 times what they are
  * normalised to: values beyond 2^100 or so may overflow them.)
  * The reference passes neither a scale nor a mask of its own to its attention (attn_backend.py:94-101,

@@ -942,3 +942,52 @@ def test_extend_that_sees_a_nan_takes_no_longer(gpu, heads, dtype, what):
     else:
         assert bool(got.isnan().all())
     assert after <= 20 * before + 1.0, (before, after)
+
+
+@pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("0.5b", torch.float16), ("7b", torch.float32), ("one", torch.bfloat16)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [0, 31, 32, 100, 149, 205, 299])
+def test_extend_rows_around_a_value_that_is_no_number(gpu, heads, dtype, bad, at):
+    """One such value: causal rows before it, and the rows of windows that have left it behind, are right to the bit of their own sums; who sees it
+    has it in that column and nowhere else."""
+    from baby_sglang_amd import _hip
+
+    n = 300
+    c = make(76, heads, dtype, [n], q_rows=n)
+    start, stop = [max(0, i - 120) for i in range(n)], [i + 1 for i in range(n)]
+    st, sp = (torch.tensor(x, dtype=torch.int32) for x in (start, stop))
+    slot = c["table"][c["req"][0], at].long()
+    finite = {k: (v.clone() if torch.is_tensor(v) else v) for k, v in c.items()}
+    c["v"][slot, :, 7] = bad
+    d = to_gpu(c, gpu)
+    out = _hip.paged_prefill_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.zeros(1, dtype=torch.int64, device=gpu), d["seq"], logit_cap=9.0,
+                                    visible_from=st.to(gpu), visible_to=sp.to(gpu), variant=2).view(n, c["hq"], c["dim"]).cpu()
+    sees = torch.tensor([a <= at < b for a, b in zip(start, stop)])
+    assert bool((out[sees][:, :, 7].isnan() if bad != bad else out[sees][:, :, 7].isinf()).all())
+    want, mass, lse, _, top = orc.scored_exact(finite["q"], finite["k"], finite["v"], finite["table"][finite["req"]], [n], [0] * n, range(n), c["dim"] ** -0.5, 9.0,
+                                               None, st, sp)
+    u_p = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 0.0}[dtype]
+    keep = torch.ones(c["dim"], dtype=torch.bool)
+    keep[7] = False
+    check_rows(out[:, :, keep], want[:, :, keep], mass[:, :, keep], lse, top, 9.0, dtype, dtype, u_p, n, 6.0, c["dim"])
+    check_rows(out[~sees], want[~sees], mass[~sees], lse[~sees], top[~sees], 9.0, dtype, dtype, u_p, n, 6.0, c["dim"])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n_splits,variant", [(3, 0), (7, 0x200), (3, 1), (64, 0)])
+def test_decode_infinite_values_in_every_piece(gpu, dtype, n_splits, variant):
+    """An infinite value shows in its column and nowhere else, whichever piece of the request it is in: the pieces that a merge reads twice to
+    fill a round among them.  Where every probability meets the values once, as a positive number, the column is infinite; as the
+    sum of two (bf16), or by the generic kernel, it may be NaN."""
+    from baby_sglang_amd import _hip
+
+    lens = [900, 40, 2000]
+    for at in (0, 450, 899):
+        c = make(77, "1.5b", dtype, lens)
+        c["v"][c["table"][c["req"][0], at].long(), :, 7] = float("inf")
+        d = to_gpu(c, gpu)
+        out = _hip.paged_decode_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], logit_cap=5.0, n_splits=n_splits, variant=variant).view(3, 12, 128)
+        once = dtype != torch.bfloat16 and variant != 1
+        assert bool((out[0, :, 7] == float("inf")).all() if once else (~out[0, :, 7].isfinite()).all())
+        out[0, :, 7] = 0.0
+        assert bool(out.isfinite().all())
