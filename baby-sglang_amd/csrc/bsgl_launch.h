@@ -182,7 +182,9 @@ struct ExpandArgs {
   int32_t batch;
   int32_t total_q_tokens;
   int64_t* cu_ext;   // [batch + 1] running sum of extended_lens
-  int64_t* cu_blk;   // [batch + 1] running sum of block GROUPS: ceil(ceil(extended_lens / blk_rows) / grp_blocks); may be NULL
+  // [batch + 2] running sum of block GROUPS: ceil(ceil(extended_lens / blk_rows) / grp_blocks), and behind it whether `order` was made with
+  // them (a later launch that takes the list over has to know: the row list stands in its place otherwise); may be NULL
+  int64_t* cu_blk;
   int32_t blk_rows;  // 16 or 64 (0 counts as 16)
   int32_t grp_blocks;  // blocks per group (0 counts as 1)
   int64_t* row_req;  // [total_q_tokens]; may be NULL (then only the running sums are made)

@@ -640,9 +640,9 @@ static int32_t prefill_row_splits(int32_t total_q_tokens, int32_t max_context_le
 
 size_t bsgl_prefill_workspace_bytes(int32_t batch, int32_t total_q_tokens, int32_t n_q_heads, int32_t head_dim) {
   if (batch <= 0 || total_q_tokens <= 0) return 0;
-  // cu_ext[batch + 1], row_req[T], row_len[T], then split partials sized for the
+  // cu_ext[batch + 1], cu_blk[batch + 2], row_req[T], row_len[T], then split partials sized for the
   // worst case over context lengths (64 splits only when T is tiny)
-  size_t bytes = 2 * align_up((size_t)(batch + 1) * 8, 256) + 2 * align_up((size_t)total_q_tokens * 8, 256);
+  size_t bytes = align_up((size_t)(batch + 1) * 8, 256) + align_up((size_t)(batch + 2) * 8, 256) + 2 * align_up((size_t)total_q_tokens * 8, 256);
   const int32_t splits = prefill_row_splits(total_q_tokens, 1 << 30);
   bytes += bsgl_decode_workspace_bytes(total_q_tokens, n_q_heads, head_dim, splits, 0);
   return bytes;
@@ -692,7 +692,7 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   ex.cu_ext = (int64_t*)ws;
   ws += align_up((size_t)(batch + 1) * 8, 256);
   ex.cu_blk = (int64_t*)ws;
-  ws += align_up((size_t)(batch + 1) * 8, 256);
+  ws += align_up((size_t)(batch + 2) * 8, 256);
   ex.row_req = (int64_t*)ws;
   ws += align_up((size_t)total_q_tokens * 8, 256);
   ex.row_len = (int64_t*)ws;

@@ -69,7 +69,10 @@ __device__ __forceinline__ void running_sums(const ExpandArgs& a, int* starts = 
   }
   if (tid == 255) {
     a.cu_ext[a.batch] = run + sum;
-    if (a.cu_blk != nullptr) a.cu_blk[a.batch] = brun + blocks;
+    if (a.cu_blk != nullptr) {
+      a.cu_blk[a.batch] = brun + blocks;
+      a.cu_blk[a.batch + 1] = a.order != nullptr;
+    }
     if (starts != nullptr) starts[a.batch] = (int)min(brun + blocks, (int64_t)0x7fffffff);
   }
   for (int i = lo; i < hi; ++i) {

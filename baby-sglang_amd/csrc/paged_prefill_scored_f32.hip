@@ -136,8 +136,8 @@ void prefill_scored_f32_kernel(PrefillArgs a) {
   const int within = (int)(slot % (unsigned)per_group);
   const int kvh = (int)(g % a.n_kv_heads);
   int64_t pg = g / a.n_kv_heads;
-  // (longest streams first; whatever stands there, it is a group of this launch)
-  if (pg < a.n_order) pg = max((int64_t)0, min((int64_t)a.order[pg], a.cu_blk[a.batch] - 1));
+  // (longest streams first, if the launch that made the list sorted it; whatever stands there, it is a group of this launch)
+  if (pg < a.n_order && a.cu_blk[a.batch + 1] != 0) pg = max((int64_t)0, min((int64_t)a.order[pg], a.cu_blk[a.batch] - 1));
   const int rt0 = (within % n_z) * HPW;
   const int n_rt = min(HPW, G - rt0);
   int i_req = 0;

@@ -991,3 +991,25 @@ def test_decode_infinite_values_in_every_piece(gpu, dtype, n_splits, variant):
         assert bool((out[0, :, 7] == float("inf")).all() if once else (~out[0, :, 7].isfinite()).all())
         out[0, :, 7] = 0.0
         assert bool(out.isfinite().all())
+
+
+@pytest.mark.parametrize("heads,dtype", [("7b", torch.bfloat16), ("7b", torch.float32)])
+def test_extend_list_taken_over_from_a_call_of_another_path(gpu, heads, dtype):
+    """Layers of one batch that differ in their cap, with a scale that only the generic kernel takes without one (16 bits): the list that the first
+    call left is right for the second, sorted or not, either way round."""
+    from baby_sglang_amd import _hip
+
+    r = random.Random(9)
+    ext = [r.randint(60, 300) for _ in range(31)]  # (with the end of the sums on a border of the workspace's parts: 31 + 1 entries of 8 bytes)
+    pre = [r.randint(0, 300) for _ in ext]
+    c = make(78, heads, dtype, [a + b for a, b in zip(ext, pre)], q_rows=sum(ext))
+    d = to_gpu(c, gpu)
+    args = (d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"], torch.tensor(pre, device=gpu), torch.tensor(ext, device=gpu))
+    ws = torch.empty(_hip.prefill_workspace_bytes(len(ext), sum(ext), c["hq"], c["dim"]), dtype=torch.uint8, device=gpu)
+    generic = dict(scale=-0.09) if dtype != torch.float32 else dict(scale=0.09)
+    forms = [dict(generic, logit_cap=0.0), dict(generic, logit_cap=10.0), dict(generic, logit_cap=30.0)]
+    want = [_hip.paged_prefill_scored(*args, **kw) for kw in forms]
+    for first, *later in ((0, 1, 2, 0, 1), (1, 0, 1, 2), (2, 2, 1)):
+        assert torch.equal(_hip.paged_prefill_scored(*args, workspace=ws, **forms[first]), want[first])
+        for i in later:
+            assert torch.equal(_hip.paged_prefill_scored(*args, workspace=ws, list_ready=True, **forms[i]), want[i]), (first, i)
