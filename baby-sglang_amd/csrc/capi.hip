@@ -105,6 +105,24 @@ int check_paged(const void* out, int64_t out_row_stride, const void* q, int64_t 
   return BSGL_OK;
 }
 
+// Rows of `bytes` bytes, `rows` of them, strides in bytes, of a result and an input that are not the same rows: do they share
+// memory?  (A kernel may compute in place, every row from itself; a result that is shifted against its input would be read
+// as input by whoever comes late.)
+bool partly_the_same(const void* out, int64_t out_stride, const void* in, int64_t in_stride, int64_t rows, int64_t bytes) {
+  if (rows <= 0 || bytes <= 0 || out == nullptr || in == nullptr) return false;
+  if (out == in && (rows == 1 || out_stride == in_stride)) return false;
+  const __int128 o = (uintptr_t)out, i = (uintptr_t)in;
+  if (o + (__int128)(rows - 1) * out_stride + bytes <= i || i + (__int128)(rows - 1) * in_stride + bytes <= o) return false;
+  for (int64_t r = 0; r < rows; ++r) {
+    // the first input row that ends behind this one's beginning
+    const __int128 at = o + (__int128)r * out_stride, past = at - bytes - i;
+    const __int128 j = past < 0 ? 0 : rows == 1 ? (past >= 0) : past / in_stride + 1;
+    if (j < rows && i + j * in_stride < at + bytes) return true;
+    if (out_stride == in_stride && r > 0 && r < rows - 1) r = rows - 2;  // (the same picture for all but the first and the last)
+  }
+  return false;
+}
+
 // fixed-size ticket area at the head of every decode workspace, so that its place
 // does not move when one workspace serves calls of different batch sizes
 constexpr size_t kCounterBytes = 65536;
@@ -588,6 +606,8 @@ int bsgl_paged_decode_scored(const bsgl_decode_call* c, const bsgl_score_mods* m
     return fail(BSGL_ERR_BAD_ARG, "token_weights and token_weights_out go together");
   if (mods->token_weights != nullptr && mods->weights_row_stride < c->table_cols)
     return fail(BSGL_ERR_BAD_ARG, "token weight row stride shorter than the page table's column count");
+  if (partly_the_same(mods->token_weights_out, mods->weights_row_stride * 4, mods->token_weights, mods->weights_row_stride * 4, c->table_rows, c->table_cols * 4))
+    return fail(BSGL_ERR_BAD_ARG, "token_weights_out must be token_weights or share no memory with it");
   return decode_entry(c->out, c->out_row_stride, c->lse, c->q, c->q_row_stride, c->k_new, c->v_new, c->k_new_row_stride,
                       c->v_new_row_stride, c->out_cache_loc, c->k_slab, c->v_slab, c->slab_row_stride, c->n_slots,
                       c->req_to_token, c->table_row_stride, c->table_rows, c->table_cols, c->req_pool_indices, c->seq_lens,
@@ -957,9 +977,15 @@ int bsgl_evict_tokens(int32_t* out_table, float* out_weights, const int32_t* req
     // (workgroups of a request read its length after others have written the new one)
     const uintptr_t s0 = (uintptr_t)seq_lens, n0 = (uintptr_t)new_lens, bytes = (uintptr_t)batch * 8;
     if (s0 < n0 + bytes && n0 < s0 + bytes) return fail(BSGL_ERR_BAD_ARG, "new_lens must not overlap seq_lens");
+    // (and the rows that earlier requests name)
+    const uintptr_t r0 = (uintptr_t)req_pool_indices;
+    if (r0 < n0 + bytes && n0 < r0 + bytes) return fail(BSGL_ERR_BAD_ARG, "new_lens must not overlap req_pool_indices");
   }
   if (table_row_stride < table_cols || weights_row_stride < table_cols)
     return fail(BSGL_ERR_BAD_ARG, "a row stride is shorter than the page table's column count");
+  if (partly_the_same(out_table, table_row_stride * 4, req_to_token, table_row_stride * 4, table_rows, table_cols * 4) ||
+      partly_the_same(out_weights, weights_row_stride * 4, token_weights, weights_row_stride * 4, table_rows, table_cols * 4))
+    return fail(BSGL_ERR_BAD_ARG, "out_table / out_weights must be their input or share no memory with it");
   if (evicted_cols < 0 || (evicted != nullptr && evicted_row_stride < evicted_cols))
     return fail(BSGL_ERR_BAD_ARG, "evicted row stride shorter than its column count");
   if (batch > 65535) return fail(BSGL_ERR_UNSUPPORTED, "batch %d above 65535", batch);
@@ -1004,6 +1030,11 @@ int bsgl_logit_controls(const bsgl_logit_call* c) {
   if (c->out_row_stride < c->vocab || c->logits_row_stride < c->vocab) return fail(BSGL_ERR_BAD_ARG, "logit row stride shorter than the vocabulary");
   if (c->out == c->logits && c->batch > 1 && c->out_row_stride != c->logits_row_stride)
     return fail(BSGL_ERR_BAD_ARG, "logits controlled in place must keep their row stride");
+  {
+    const int64_t eb = bsgl::dtype_bytes(c->dtype);
+    if (partly_the_same(c->out, c->out_row_stride * eb, c->logits, c->logits_row_stride * eb, c->batch, c->vocab * eb))
+      return fail(BSGL_ERR_BAD_ARG, "out must be logits or share no memory with them");
+  }
   if (c->history != nullptr) {
     if (!c->history_lens) return fail(BSGL_ERR_BAD_ARG, "history without history_lens");
     if (c->history_n_rows <= 0 || c->history_cols < 0 || c->history_row_stride < c->history_cols)

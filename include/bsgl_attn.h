@@ -276,7 +276,7 @@ typedef struct bsgl_score_mods {
   /* decode only, both or neither: the attention weight every visible token received in this call, summed
    * over the q heads, is added to a table parallel to the page table --
    *   token_weights_out[req_pool_indices[i], j] = token_weights[req_pool_indices[i], j] + sum_h softmax(s)[h, j]
-   * (fp32, [table_rows, table_cols] with row stride weights_row_stride; out may be the same table).  Entries of
+   * (fp32, [table_rows, table_cols] with row stride weights_row_stride; out may be the same table, and not overlap it otherwise).  Entries of
    * tokens that are not visible are left as they were.  Requests that name the same row are added up, in
    * batch order: the result never depends on the launch. */
   const float* token_weights;
@@ -306,7 +306,8 @@ int bsgl_paged_decode_scored(const bsgl_decode_call* call, const bsgl_score_mods
  * its input), new_lens[i] = min(seq_lens[i], budget) receives their number, and evicted (optional, [batch, evicted_cols])
  * the slots of the others in their order, as many as fit, then -1.  Entries behind new_lens[i], and rows that no request
  * names, are left as they are.  A row named by several requests is compacted for the first of them; the others get an
- * empty evicted list.  new_lens must not overlap seq_lens.  max_seq_len (0 = unknown) shapes the launch only.  workspace: bsgl_evict_workspace_bytes, may be
+ * empty evicted list.  new_lens must not overlap seq_lens
+ * or req_pool_indices, nor an out_ table its input other than by being it.  max_seq_len (0 = unknown) shapes the launch only.  workspace: bsgl_evict_workspace_bytes, may be
  * NULL when that is 0.
  */
 size_t bsgl_evict_workspace_bytes(int32_t batch, int64_t table_cols, int32_t budget);
@@ -330,7 +331,7 @@ int bsgl_evict_tokens(int32_t* out_table /*device*/, float* out_weights /*device
  * of row history_rows[i] (NULL: row i), the first prompt_lens[i] (NULL: 0) of them its prompt.  Ids outside the vocabulary are ignored,
  * in biases too (padding); up to 4096 biases and a history of up to
  * 262143 tokens per request (BSGL_ERR_UNSUPPORTED beyond).  mask_rows[i] (NULL: i) outside [0, mask_n_rows) = no mask.  A mask without any bit
- * leaves a row of -inf.  Everything but logits and out may be NULL; out may be logits.  repetition, presence, frequency: fp32
+ * leaves a row of -inf.  Everything but logits and out may be NULL; out may be logits, and not overlap them otherwise.  repetition, presence, frequency: fp32
  * [batch], repetition > 0.
  */
 typedef struct bsgl_logit_call {

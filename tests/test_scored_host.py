@@ -142,3 +142,48 @@ def test_evicted_rows_that_share_memory_are_refused(monkeypatch):
         assert calls[-1][12:14] == (stride, width)
     _hip.evict_tokens(table, w, req[:1], lens[:1], 4, evicted=one.expand(1, 7))
     assert calls[-1][12:14] == (7, 7)
+
+
+def test_evict_new_lengths_over_the_requests_rows():
+    """Later requests look at the rows that earlier ones name."""
+    def f(req, new, batch=4, cols=64):
+        return lib.bsgl_evict_tokens(P, P, P, cols, P, cols, 2, cols, ctypes.c_void_p(req), ctypes.c_void_p(1 << 20), ctypes.c_void_p(new), None, 0, 0, batch, 4, 0, 0,
+                                     0, None, 0, None)
+
+    for new in (4096, 4096 - 24, 4096 + 24):
+        assert f(4096, new) == _hip.BSGL_ERR_BAD_ARG and b"req_pool_indices" in lib.bsgl_last_error()
+
+
+def test_results_that_are_their_inputs_in_part():
+    """Shifted by an element, by a row, by a part of a row's gap: refused; in place, beside each other, columns apart: not this refusal's business (what
+    answers those calls here is a workspace that is missing, or a type that is none, behind the check)."""
+    at = 1 << 20
+
+    def evict(out_t, out_w, rows=5, cols=20000, stride=40000):  # (rows this long need a workspace)
+        v = ctypes.c_void_p
+        return lib.bsgl_evict_tokens(v(out_t), v(out_w), v(at), stride, v(at), stride, rows, cols, v(64), v(1 << 10), v(1 << 12), None, 0, 0, 2, 4, 0, 0, 0, None, 0, None)
+
+    row = 40000 * 4
+    far = at + 100 * row
+    for out in (at + 4, at - 4, at + row, at - row, at + 4 * row, at - 4 * row, at + 3 * row + 19999 * 4, at + row - 4, at + 20000 * 4 - 4):
+        assert evict(out, far) == _hip.BSGL_ERR_BAD_ARG and b"share no memory" in lib.bsgl_last_error(), out
+        assert evict(far, out) == _hip.BSGL_ERR_BAD_ARG and b"share no memory" in lib.bsgl_last_error(), out
+    for out in (at, at + 20000 * 4, at - 20000 * 4, at + 5 * row, at + row + 20000 * 4, far):
+        assert evict(out, out) == _hip.BSGL_ERR_WORKSPACE, out
+
+    def logits(out, out_stride, in_stride=100, batch=3, vocab=100):
+        c = _hip.LogitCall()
+        for k, v in dict(out=out, logits=at, out_row_stride=out_stride, logits_row_stride=in_stride, batch=batch, vocab=vocab, dtype=2, repetition=256).items():
+            setattr(c, k, v)
+        return lib.bsgl_logit_controls(ctypes.byref(c))  # (penalties without a history: refused next)
+
+    for out, stride in ((at + 4, 100), (at + 400, 100), (at - 400, 100), (at + 400, 300), (at - 4, 1000)):
+        assert logits(out, stride) == _hip.BSGL_ERR_BAD_ARG and b"share no memory" in lib.bsgl_last_error(), (out, stride)
+    for out, stride, kw in ((at, 100, {}), (at + 1200, 100, {}), (at - 1200, 100, {}), (at + 400, 200, dict(in_stride=200)), (at, 500, dict(batch=1)), (at + 800, 100, dict(in_stride=2000, batch=1))):
+        assert logits(out, stride, **kw) == _hip.BSGL_ERR_BAD_ARG and b"history" in lib.bsgl_last_error(), (out, stride)
+    w = dict(weights_row_stride=64)
+    for out in (at + 4, at + 256, at - 252):
+        assert lib.bsgl_paged_decode_scored(decode_call(), mods(token_weights=at, token_weights_out=out, **w)) == _hip.BSGL_ERR_BAD_ARG
+        assert b"share no memory" in lib.bsgl_last_error()
+    assert lib.bsgl_paged_decode_scored(decode_call(), mods(token_weights=at, token_weights_out=at, **w)) == _hip.BSGL_ERR_WORKSPACE
+    assert lib.bsgl_paged_decode_scored(decode_call(), mods(token_weights=at, token_weights_out=at + 512, **w)) == _hip.BSGL_ERR_WORKSPACE
