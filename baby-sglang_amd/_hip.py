@@ -192,12 +192,20 @@ lib = _load()
 
 try:  # the ordinary case of the small calls without their Python (csrc/fast_calls.cpp); the wrappers work without it
     from . import _fast_calls as _fast
-
-    _fast.bind(*(ctypes.cast(getattr(lib, name), _vp).value for name in (
-        "bsgl_paged_decode_scored", "bsgl_decode_scored_workspace_bytes", "bsgl_evict_tokens", "bsgl_evict_workspace_bytes", "bsgl_logit_controls",
-        "bsgl_paged_prefill_scored", "bsgl_prefill_workspace_bytes")))
 except ImportError:
     _fast = None
+
+
+def bind_fast_calls(stand_ins=None) -> None:
+    """Hand the extension the library's entry points (a test may give others in their places)."""
+    at = stand_ins or {}
+    _fast.bind(*(ctypes.cast(at.get(name, getattr(lib, name)), _vp).value for name in (
+        "bsgl_paged_decode_scored", "bsgl_decode_scored_workspace_bytes", "bsgl_evict_tokens", "bsgl_evict_workspace_bytes", "bsgl_logit_controls",
+        "bsgl_paged_prefill_scored", "bsgl_prefill_workspace_bytes")))
+
+
+if _fast is not None:
+    bind_fast_calls()
 
 
 def _check(rc: int, what: str) -> None:

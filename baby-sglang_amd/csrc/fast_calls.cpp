@@ -23,6 +23,21 @@ decltype(&bsgl_evict_tokens) g_evict;
 decltype(&bsgl_evict_workspace_bytes) g_evict_bytes;
 decltype(&bsgl_logit_controls) g_logits;
 
+// The call itself, without the interpreter's lock: a launch waits where the stream's queue is full, and other threads (the overlap mode's
+// worker among them) go on meanwhile, as they do through ctypes.  The arguments are held by the caller.
+template <typename F> PyObject* unlocked(F call) {
+  struct Unlocked {  // (taken back whichever way the call is left)
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+  };
+  int rc;
+  {
+    Unlocked u;
+    rc = call();
+  }
+  return PyLong_FromLong(rc);
+}
+
 // One call's look at its arguments: `ok` falls when anything is not the ordinary case.
 struct Look {
   int index;
@@ -177,7 +192,7 @@ PyObject* decode_scored(PyObject*, PyObject* const* a, Py_ssize_t n) {
     m.token_weights_out = (float*)wo->data_ptr();
     m.weights_row_stride = w_stride;
   }
-  return PyLong_FromLong(g_decode(&c, &m));
+  return unlocked([&] { return g_decode(&c, &m); });
 }
 
 // index, stream, q, k_slab, v_slab, req_to_token, req_pool_indices, seq_lens, prefix_lens, extended_lens, scale, logit_cap, slopes,
@@ -207,10 +222,12 @@ PyObject* prefill_scored(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!k.ok || table->size(0) < 1 || table->size(1) < 1 || !(cap >= 0.0) || !std::isfinite(cap)) Py_RETURN_NONE;
   m.logit_cap = (float)cap;
   if (!ws->is_contiguous() || ws->nbytes() < g_prefill_bytes((int32_t)batch, (int32_t)tokens, (int32_t)hq, (int32_t)dim)) Py_RETURN_NONE;
-  return PyLong_FromLong(g_prefill(out->data_ptr(), tokens > 1 ? out->stride(0) : hq * dim, q->data_ptr(), tokens > 1 ? q->stride(0) : hq * dim, ks->data_ptr(),
-                                   vs->data_ptr(), ks->stride(0), ks->size(0), (const int32_t*)table->data_ptr(), table_stride, table->size(0), table->size(1),
-                                   (const int64_t*)req, (const int64_t*)lens, (const int64_t*)prefix, (const int64_t*)ext, (int32_t)batch, (int32_t)tokens,
-                                   (int32_t)hq, (int32_t)hkv, (int32_t)dim, scale, code, variant, ws->data_ptr(), ws->nbytes(), &m, k.stream));
+  return unlocked([&] {
+    return g_prefill(out->data_ptr(), tokens > 1 ? out->stride(0) : hq * dim, q->data_ptr(), tokens > 1 ? q->stride(0) : hq * dim, ks->data_ptr(),
+                     vs->data_ptr(), ks->stride(0), ks->size(0), (const int32_t*)table->data_ptr(), table_stride, table->size(0), table->size(1),
+                     (const int64_t*)req, (const int64_t*)lens, (const int64_t*)prefix, (const int64_t*)ext, (int32_t)batch, (int32_t)tokens,
+                     (int32_t)hq, (int32_t)hkv, (int32_t)dim, scale, code, variant, ws->data_ptr(), ws->nbytes(), &m, k.stream);
+  });
 }
 
 // index, stream, req_to_token, token_weights, req_pool_indices, seq_lens, budget, recent, sinks, out_table, out_weights, evicted,
@@ -237,9 +254,11 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
       ow->sizes() != t->sizes() || ots != ts || ows != ws || ev->size(0) != batch || ev->size(1) > INT32_MAX)
     Py_RETURN_NONE;
   if (g_evict_bytes((int32_t)batch, t->size(1), budget) != 0) Py_RETURN_NONE;  // (long rows: the wrapper sees to the workspace)
-  return PyLong_FromLong(g_evict((int32_t*)ot->data_ptr(), (float*)ow->data_ptr(), (const int32_t*)t->data_ptr(), ts, (const float*)w->data_ptr(), ws, t->size(0),
-                                 t->size(1), (const int64_t*)req, (const int64_t*)lens, (int64_t*)nl, ev->size(1) > 0 ? (int32_t*)ev->data_ptr() : nullptr, es,
-                                 (int32_t)ev->size(1), (int32_t)batch, budget, recent, sinks, longest, nullptr, 0, k.stream));
+  return unlocked([&] {
+    return g_evict((int32_t*)ot->data_ptr(), (float*)ow->data_ptr(), (const int32_t*)t->data_ptr(), ts, (const float*)w->data_ptr(), ws, t->size(0),
+                   t->size(1), (const int64_t*)req, (const int64_t*)lens, (int64_t*)nl, ev->size(1) > 0 ? (int32_t*)ev->data_ptr() : nullptr, es,
+                   (int32_t)ev->size(1), (int32_t)batch, budget, recent, sinks, longest, nullptr, 0, k.stream);
+  });
 }
 
 // index, stream, logits, history, history_rows, history_lens, prompt_lens, repetition, presence, frequency, bias_ids, bias_values,
@@ -295,7 +314,7 @@ PyObject* logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
   c.vocab = (int32_t)vocab;
   c.dtype = code;
   c.stream = k.stream;
-  return PyLong_FromLong(g_logits(&c));
+  return unlocked([&] { return g_logits(&c); });
 }
 
 // no C++ exception leaves a function that Python calls: whatever it was, the wrapper looks again

@@ -118,3 +118,50 @@ def test_on_a_stream_of_its_own_and_captured(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+SLOW = """
+#include <unistd.h>
+int slow(void) { usleep(400000); return 0; }
+"""
+
+
+def test_other_threads_run_while_a_call_waits(gpu, monkeypatch, tmp_path):
+    """A launch that has to wait (here: a function of 0.4 s in an entry point's place) does not stop the process's other threads."""
+    import ctypes
+    import subprocess
+    import threading
+    import time
+
+    from baby_sglang_amd import _hip
+
+    src, so = tmp_path / "slow.c", tmp_path / "slow.so"
+    src.write_text(SLOW)
+    subprocess.check_call(["gcc", "-shared", "-fPIC", "-o", str(so), str(src)])
+    slow = ctypes.CDLL(str(so))
+    d = sa.to_gpu(sa.make(9, "1.5b", torch.bfloat16, [30, 500]), gpu)
+    args = (d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"])
+    ws = _hip.new_decode_workspace(_hip.decode_scored_workspace_bytes(2, 12, 128, 4, d["table"].shape[1], True), gpu)
+    ext = torch.tensor([1, 1], device=gpu)
+    pws = torch.empty(_hip.prefill_workspace_bytes(2, 2, 12, 128), dtype=torch.uint8, device=gpu)
+    x, mask = torch.zeros(2, 64, device=gpu), torch.zeros(2, 2, dtype=torch.int32, device=gpu)
+    table, weights = torch.zeros(3, 64, dtype=torch.int32, device=gpu), torch.zeros(3, 64, device=gpu)
+    new, gone = torch.zeros(2, dtype=torch.int64, device=gpu), torch.zeros((2, 9), dtype=torch.int32, device=gpu)
+    calls = (lambda: _hip.paged_decode_scored(*args, n_splits=4, workspace=ws), lambda: _hip.paged_prefill_scored(*args, d["seq"] - ext, ext, workspace=pws),
+             lambda: _hip.evict_tokens(table, weights, ext, ext, 8, evicted=gone, new_lens=new), lambda: _hip.logit_controls(x, token_mask=mask))
+    for call in calls:
+        call()
+    try:
+        _hip.bind_fast_calls({name: slow.slow for name in ("bsgl_paged_decode_scored", "bsgl_evict_tokens", "bsgl_logit_controls", "bsgl_paged_prefill_scored")})
+        for call in calls:
+            worker = threading.Thread(target=call)
+            t0, gap = time.perf_counter(), 0.0
+            worker.start()
+            while worker.is_alive():
+                t1 = time.perf_counter()
+                time.sleep(0.002)
+                gap = max(gap, time.perf_counter() - t1)
+            assert time.perf_counter() - t0 > 0.3  # (the stand-in was called)
+            assert gap < 0.2, gap
+    finally:
+        _hip.bind_fast_calls()
