@@ -187,3 +187,16 @@ def test_results_that_are_their_inputs_in_part():
         assert b"share no memory" in lib.bsgl_last_error()
     assert lib.bsgl_paged_decode_scored(decode_call(), mods(token_weights=at, token_weights_out=at, **w)) == _hip.BSGL_ERR_WORKSPACE
     assert lib.bsgl_paged_decode_scored(decode_call(), mods(token_weights=at, token_weights_out=at + 512, **w)) == _hip.BSGL_ERR_WORKSPACE
+
+
+def test_the_library_alone_needs_no_python_to_build():
+    """`make` is the C library with hipcc; what needs PyTorch and its headers is a target of its own."""
+    import os
+    import subprocess
+
+    csrc = os.path.join(os.path.dirname(_hip.LIB_PATH), "csrc")
+    plan = lambda *goals: subprocess.run(["make", "-n", "-B", "-C", csrc, *goals], capture_output=True, text=True, check=True).stdout  # noqa: E731
+    alone = plan()
+    assert "libbsgl_attn.so" in alone and "fast_calls" not in alone and "python" not in alone.replace("/python", "")
+    both = plan("python")
+    assert "libbsgl_attn.so" in both and "fast_calls" in both
