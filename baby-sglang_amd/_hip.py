@@ -199,13 +199,19 @@ except ImportError:
 def bind_fast_calls(stand_ins=None) -> None:
     """Hand the extension the library's entry points (a test may give others in their places)."""
     at = stand_ins or {}
-    _fast.bind(*(ctypes.cast(at.get(name, getattr(lib, name)), _vp).value for name in (
+    _fast.bind(lib.bsgl_abi_version(), *(ctypes.sizeof(t) for t in (DecodeCall, ScoreMods, LogitCall)), *(ctypes.cast(at.get(name, getattr(lib, name)), _vp).value for name in (
         "bsgl_paged_decode_scored", "bsgl_decode_scored_workspace_bytes", "bsgl_evict_tokens", "bsgl_evict_workspace_bytes", "bsgl_logit_controls",
         "bsgl_paged_prefill_scored", "bsgl_prefill_workspace_bytes")))
 
 
 if _fast is not None:
-    bind_fast_calls()
+    try:
+        bind_fast_calls()
+    except (ImportError, TypeError) as e:  # one that was built for another version: the wrappers do its work
+        import warnings
+
+        warnings.warn(f"{_fast.__file__}: {e}; build it again (make -C csrc python)")
+        _fast = None
 
 
 def _check(rc: int, what: str) -> None:

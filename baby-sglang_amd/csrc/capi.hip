@@ -295,7 +295,7 @@ int run_scored(bsgl::DecodeArgs& a, int32_t variant, uint32_t* counters, hipStre
 
 extern "C" {
 
-int bsgl_abi_version(void) { return 2; }
+int bsgl_abi_version(void) { return BSGL_ABI_VERSION; }
 
 void bsgl_debug_decode_trace(void* device_buf) { bsgl::set_decode_trace((uint64_t*)device_buf); }
 

@@ -330,12 +330,16 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// the addresses of the seven entry points
+// the library's ABI version, the sizes of its descriptors as the wrappers have them, and the addresses of the seven entry points
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "seven addresses");
+  const long want[4] = {BSGL_ABI_VERSION, (long)sizeof(bsgl_decode_call), (long)sizeof(bsgl_score_mods), (long)sizeof(bsgl_logit_call)};
+  bool same = n == 11;
+  for (int i = 0; same && i < 4; ++i) same = PyLong_AsLong(a[i]) == want[i];
+  if (!same) {
+    if (PyErr_Occurred() == nullptr) PyErr_SetString(PyExc_ImportError, "_fast_calls was built for another version of the library");
     return nullptr;
   }
+  a += 4;
   g_decode = (decltype(g_decode))PyLong_AsVoidPtr(a[0]);
   g_decode_bytes = (decltype(g_decode_bytes))PyLong_AsVoidPtr(a[1]);
   g_evict = (decltype(g_evict))PyLong_AsVoidPtr(a[2]);

@@ -69,7 +69,8 @@ extern "C" {
  * Ignored where the generic path runs (it rebuilds its row list every time). */
 #define BSGL_PREFILL_LIST_READY 0x400
 
-/* ABI version of this header (bumped on any signature change). */
+/* ABI version of this header (bumped on any signature change): what bsgl_abi_version() of a library built from it returns. */
+#define BSGL_ABI_VERSION 2
 int bsgl_abi_version(void);
 
 /* Tuning aid with no counterpart in the reference: when device_buf is not NULL,

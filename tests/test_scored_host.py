@@ -200,3 +200,22 @@ def test_the_library_alone_needs_no_python_to_build():
     assert "libbsgl_attn.so" in alone and "fast_calls" not in alone and "python" not in alone.replace("/python", "")
     both = plan("python")
     assert "libbsgl_attn.so" in both and "fast_calls" in both
+
+
+def test_the_fast_calls_of_another_version_are_not_taken():
+    """Another ABI version, or a descriptor of another size, than the extension was built with."""
+    import ctypes as ct
+
+    fast = _hip._fast
+    assert fast is not None, "build baby-sglang_amd/_fast_calls.so (make -C baby-sglang_amd/csrc python)"
+    right = [_hip.ABI_VERSION] + [ct.sizeof(t) for t in (_hip.DecodeCall, _hip.ScoreMods, _hip.LogitCall)]
+    try:
+        for i in range(4):
+            with pytest.raises(ImportError, match="another version"):
+                fast.bind(*(x + (j == i) for j, x in enumerate(right)), *[0] * 7)
+        with pytest.raises(ImportError):
+            fast.bind(*[0] * 7)
+        with pytest.raises(TypeError):
+            fast.bind("2", *right[1:], *[0] * 7)
+    finally:
+        _hip.bind_fast_calls()
