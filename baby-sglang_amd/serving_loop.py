@@ -54,7 +54,8 @@ Bounded cache (not in the reference): with ``kv_budget = N`` a request never hol
 grown to N + ``kv_slack`` tokens, the ones with the least weight are evicted down to N (``ReqToTokenPool.evict_tokens``; the
 first ``kv_sinks`` and the last ``kv_recent`` always stay).  Kept keys keep the positions they were rotated to,
 and new tokens go on counting from where the request really is; a distance bias counts cached tokens.  Evicted slots
-that the prefix tree holds stay with the tree, and a request that has lost tokens is not put into it at its end.
+that the prefix tree holds stay with the tree, so a prompt longer than N is not put into it while its request runs (a running request
+holds N tokens of the tree's and N + ``kv_slack`` of its own at most), and a request that has lost tokens is not put into it at its end.
 Off, nothing of this runs.
 
 Controlled logits (not in the reference): presence / frequency penalties, biases and allowed tokens of
@@ -791,6 +792,10 @@ class ServingLoop:
         and point its page-table row at the tree's own slots for it."""
         tokens = list(s.input_ids)
         if not tokens:
+            return
+        if self.kv_budget is not None and len(tokens) > self.kv_budget:
+            # (to be cut at its next eviction: in the tree, locked while the request runs, none of its slots would come back.  What
+            # the tree already had of it stays there)
             return
         tree = self.tree_cache
         slots = torch.tensor(s.table[: len(tokens)], dtype=torch.int32)

@@ -295,3 +295,30 @@ def test_prompts_as_long_as_their_row(gpu):
     with pytest.raises(ValueError, match="row of 32"):
         loop.run_batch([prompt], SamplingParams(max_new_tokens=2))
     accounted(loop, 64)
+
+
+@pytest.mark.parametrize("chunk", [None, 9])
+def test_budget_gives_the_slots_of_long_prompts_back(gpu, chunk):
+    """Prompts of four times the budget: once they have been cut, the pool holds what the requests hold, N + slack each, and the tree
+    nothing of them; a prompt within the budget is in the tree as ever, and a long one may begin with it."""
+    from baby_sglang_amd.serving_loop import SamplingParams, ServingLoop
+
+    model = tiny_model(gpu, torch.float32)
+    g = torch.Generator().manual_seed(4)
+    short = torch.randint(0, 64, (10,), generator=g)
+    prompts = [torch.randint(0, 64, (50,), generator=g), torch.cat((short, torch.randint(0, 64, (40,), generator=g)))]
+    loop = ServingLoop(model, max_total_tokens=192, max_requests=3, chunked_prefill_size=chunk, kv_budget=12, kv_slack=4)
+    loop.run_batch([short], SamplingParams(max_new_tokens=3))
+    in_tree = int(loop.tree_cache.evictable_size())
+    assert in_tree >= 10
+    held = []
+    loop.on_batch = lambda mode, fb: held.append((mode, 192 - loop.token_to_kv_pool.available_size(), fb.seq_lens.tolist()))
+    outs = loop.run_batch(prompts, SamplingParams(max_new_tokens=30))
+    assert [len(o) for o in outs] == [30, 30]
+    for mode, used, lens in held[-20:]:
+        assert mode == "decode" and max(lens) <= 16
+        assert used <= in_tree + 2 * 16, (used, lens)
+    accounted(loop, 192)
+    assert int(loop.tree_cache.evictable_size()) == in_tree
+    loop.run_batch([short], SamplingParams(max_new_tokens=3))  # (what the tree had is still right)
+    accounted(loop, 192)
