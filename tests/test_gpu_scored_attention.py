@@ -1013,3 +1013,13 @@ def test_extend_list_taken_over_from_a_call_of_another_path(gpu, heads, dtype):
         assert torch.equal(_hip.paged_prefill_scored(*args, workspace=ws, **forms[first]), want[first])
         for i in later:
             assert torch.equal(_hip.paged_prefill_scored(*args, workspace=ws, list_ready=True, **forms[i]), want[i]), (first, i)
+
+
+def test_f32_of_16_heads_per_kv_head_everywhere(gpu):
+    """The sizes that the tests above leave out for it: f32 takes up to 16 q heads per kv head in every form."""
+    decode_case(gpu, "one", torch.float32, [1, 2, 15, 16, 17, 300, 33, 64], cap=8.0, slopes=True)
+    for ext, prefix in (([3, 1, 0, 17, 40], [0, 5, 9, 33, 600]), ([130, 64, 1, 200], [0, 31, 70, 513])):
+        extend_case(gpu, "one", torch.float32, ext, prefix, cap=8.0, slopes=True, only=60)
+    for ext, prefix, kind in (([1], [0], None), ([1], [2500], None), ([3, 0, 2], [700, 9, 0], "both"), ([7, 11], [1300, 40], "document"),
+                              ([5, 9, 20], [0, 600, 33], "wild"), ([8], [4000], "prefix")):
+        extend_case(gpu, "one", torch.float32, ext, prefix, cap=20.0, slopes=True, kind=kind, seed=36, extra_rows=3)
