@@ -1023,3 +1023,29 @@ def test_f32_of_16_heads_per_kv_head_everywhere(gpu):
     for ext, prefix, kind in (([1], [0], None), ([1], [2500], None), ([3, 0, 2], [700, 9, 0], "both"), ([7, 11], [1300, 40], "document"),
                               ([5, 9, 20], [0, 600, 33], "wild"), ([8], [4000], "prefix")):
         extend_case(gpu, "one", torch.float32, ext, prefix, cap=20.0, slopes=True, kind=kind, seed=36, extra_rows=3)
+
+
+@pytest.mark.parametrize("heads", ["1.5b", "0.5b", "7b"])
+def test_decode_f32_is_as_exact_as_f32_is(gpu, heads):
+    """The results' distance from the definition, beside that of elementary operations in 32 bits (products, exp, sums by torch on the same
+    tensors): both round some 130 times on the way to a score, so neither should be far ahead; 1.35 times is allowed."""
+    from baby_sglang_amd import _hip
+
+    lens = [300, 900, 555, 731, 402, 618, 850, 333]
+    c = make(79, heads, torch.float32, lens, q_scale=3.0)
+    d = to_gpu(c, gpu)
+    hq, hkv, dim = c["hq"], c["hkv"], c["dim"]
+    got = _hip.paged_decode_scored(d["q"], d["k"], d["v"], d["table"], d["req"], d["seq"]).view(len(lens), hq, dim).double()
+    kernel = plain = 0.0
+    for i, n in enumerate(lens):
+        slots = d["table"][d["req"][i], :n].long()
+        k, v = d["k"][slots].transpose(0, 1).contiguous(), d["v"][slots].transpose(0, 1).contiguous()  # [Hkv, n, D]
+        q = d["q"][i].view(hkv, hq // hkv, dim)
+        outs = []
+        for t in (torch.float64, torch.float32):
+            s = torch.matmul(q.to(t), k.to(t).transpose(1, 2).contiguous()) * dim**-0.5
+            p = torch.exp(s - s.amax(-1, keepdim=True))
+            outs.append((torch.matmul(p, v.to(t)) / p.sum(-1, keepdim=True)).reshape(hq, dim).double())
+        kernel += (got[i] - outs[0]).square().sum().item()
+        plain += (outs[1] - outs[0]).square().sum().item()
+    assert kernel <= 1.35**2 * plain, (kernel / plain) ** 0.5
