@@ -759,10 +759,11 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
     int grp = 1, most = 8;
     if (mods != nullptr) {
       // Scored form: launches of up to ten rounds of the machine (two workgroups per CU) go block by block, and the longest streams
-      // first (prefill_order_kernel).  Against groups of 8 in the requests' order: 6 x 700 - 1501 tokens, 12 / 2 heads, with a bias 76 -> 52 us
-      // (f32 440 -> 299), documents 53 -> 43, 20 x 100 - 2000 of 14 / 2 heads of 64 211 -> 161, 200 x 10 - 300 over 500 252 -> 218, 1 x 4096
-      // of 28 / 4 heads 187 -> 174.  Larger ones stay in groups: 48 x 512 over 1536, 28 / 4 heads, 842, block by block -- its K/V
-      // then pass every L2 -- 880; sorted or not makes 1 - 2 % there (48 x 100 - 2000 875 - 910 -> 872 - 892).
+      // first (prefill_order_kernel).  Against groups of 8, sorted as well (profiles/scored_operators_shapes.csv): 6 x 700 - 1501 tokens, 12 / 2 heads, with a bias 49.8 / 56.6 us
+      // (f32 309 / 328), 20 x 100 - 2000 of 14 / 2 heads of 64 160 / 181, 200 x 10 - 300 over 500 220 / 253, 300 x 10 - 300 204 / 224, 1 x 4096
+      // of 28 / 4 heads 174 / 188, documents no difference.  In the requests' order those groups took 76 (f32 440) with the bias and 211 of 14 / 2
+      // heads.  Larger ones stay in groups: 48 x 512 over 1536, 28 / 4 heads, took 842 in them and 880 block by block -- its K/V
+      // then pass every L2 --; sorted or not makes 1 - 2 % there.
       // (two kv heads of 64 values run as one of 128 there, see below)
       const int64_t kv_units = head_dim == 64 && n_kv_heads == 2 && dtype != BSGL_DTYPE_F32 ? 1 : n_kv_heads;
       const int64_t n_wg = scored_workgroups(pa.blk_rows, total_q_tokens, batch, n_q_heads, kv_units);
@@ -813,9 +814,11 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
   // A few tokens (scored form): as rows of the decode kernel, which spreads every row over the machine and needs no
   // second launch to merge; every token then streams its request's K/V again, from L2 at some 6 TB/s.  So it pays where
   // tokens x row bytes x length is small; the length is not known here, the page table's width bounds it.  Measured
-  // against the extend kernel, bf16: 1 x 1 over 300 11 / 16 us, 16 x 8 over 500 16 / 23, 4 x 16 over 2000 (3.3e7 below) 23 / 30,
-  // 2 x 128 over 500 (4.2e7) 24 / 26, 1 x 100 over 2000 (5.4e7) 32 / 28, 16 x 4 over 8192 (1.3e8) 57 / 40; f32: 1 x 1 over 300
-  // 14 / 45, 64 x 2 over 600 (2.0e7) 39 / 82, 1 x 128 over 500 (2.1e7) 39 / 35, 4 x 16 over 2000 45 / 41.
+  // against the extend kernel (profiles/scored_operators_shapes.csv), 12 / 2 heads, bf16: 1 x 1 over 300 11.1 / 18.1 us, 16 x 8 over 500
+  // 18.3 / 23.4, 4 x 16 over 2000 (3.3e7 below) 22.2 / 31.3, 2 x 128 over 500 (4.2e7) 22.6 / 28.5, and beyond the border 1 x 100 over 2000 (5.4e7)
+  // 32 / 30.5, 16 x 4 over 8192 (1.3e8) 57 / 43; f32: 1 x 1 over 300 14.5 / 29.8, 64 x 2 over 600 (2.0e7) 39 / 82, 1 x 128 over 500 (2.1e7) 38.5 / 34,
+  // beyond it 4 x 16 over 2000 45 / 40.  (A wide page table of short requests leaves it for its width alone: five turns of 3 - 41 over
+  // 333, 14 / 2 heads of 64, 11.6 us on a table of 338 columns, 19.8 on one of 4096.)
   const int64_t streamed = (int64_t)total_q_tokens * n_kv_heads * head_dim;
   // (only where a row may be cut does the workspace have a ticket area)
   const bool few = mods != nullptr && kind == BSGL_DECODE_AUTO && mfma_ok && streamed <= kFewTokens &&
@@ -836,7 +839,7 @@ static int prefill_entry(void* out, int64_t out_row_stride, const void* q, int64
       // Scored form: two workgroups fit a CU.  With room for more than twice the blocks there are at most, every
       // block's stream is cut, into as many pieces as the workspace holds partial rows for (1024 rows or so) and none
       // shorter than 512 tokens of the widest request the page table allows.  512 tokens over 8192, 12 / 2 heads: 190 us in one piece,
-      // 116 in two; 64 over 8192 195 and 31 (8 pieces); where there is nothing to stream the merge costs 2 - 4 us (200 over 200: 21).
+      // 119 in two; 64 over 8192 195 and 31.5 (8 pieces); where there is nothing to stream the merge costs 2 - 4 us (200 over 200: 18).
       // (f32: 64 tokens, a step of 32 takes 3.4 us there: 1 token over 300 41 us in two pieces, 30 in four)
       int64_t s = 512 / scored_workgroups(pa.blk_rows, total_q_tokens, batch, pa.n_q_heads, pa.n_kv_heads);
       const int64_t room = prefill_row_splits(total_q_tokens, 1 << 30), by_len = table_cols / (dtype == BSGL_DTYPE_F32 ? 64 : 512);

@@ -477,9 +477,9 @@ static void launch_scored_tag(const DecodeArgs& a, hipStream_t stream) {
   else a.head_dim == 128 ? go(decode_scored_kernel<Tag, 128, false>) : go(decode_scored_kernel<Tag, 64, false>);
 }
 
-// Per call, with a cap, K/V from memory: 64 requests of 2048 tokens, 12 / 2 heads of 128: bf16 30.5 us (135 MB; the plain decode 29), f32
-// 59.5 (270 MB; the plain generic kernel 66); 128 of 2048 - 4096, 28 / 4 heads, 161 (the copy rate); 96 documents of 1 - 3363 tokens, 28 / 4
-// heads, f16, 40 (143 MB); one request of 4000 tokens 11 (the plain decode 13.4).
+// Per call, with a cap, K/V from memory: 64 requests of 2048 tokens, 12 / 2 heads of 128: bf16 29.8 us (135 MB; the plain decode 28.6), f32
+// 60.5 (270 MB; the generic kernel 98); 128 of 2048 - 4096, 28 / 4 heads, 161 (the copy rate; the plain decode 157); 96 documents of 1 - 3363
+// tokens, 28 / 4 heads, f16, 39 (143 MB); one request of 4000 tokens 10.6 (the plain decode 12.8).
 hipError_t launch_decode_scored(const DecodeArgs& a_in, hipStream_t stream) {
   if (a_in.rows == 0) return hipSuccess;
   DecodeArgs a = a_in;

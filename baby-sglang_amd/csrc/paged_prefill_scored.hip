@@ -16,6 +16,9 @@
 //     slope x row in registers the bias cost 200 us of a 780 us launch, sixteen registers too many).  A cap costs 24 issue
 //     cycles a score -- multiply, exp2, add, reciprocal -- beside the 20 of the plain softmax: this kernel is bound by
 //     vector issue where the plain one is bound by both pipes.
+//   * probabilities are rounded once, to bf16 (2^-8 of each) or f16 (2^-11), on their way into the second product; sums and
+//     statistics are f32.  bf16 results are 1.35 times as far from 64 bits as their own rounding puts them; the decode kernel's two
+//     halves would double the products of P V and add 24 vector instructions to a step that is bound by their issue.
 //   * the tokens are streamed from the last one back (the page-table entries are staged in that order, nothing else
 //     changes): a bias makes the nearest tokens the largest, so going forward a steep slope raises the running maximum in
 //     every step, and every step then rescales the output (48 x 512 over 1536, 28 / 4 heads: 983 us forward, 768 back; without a

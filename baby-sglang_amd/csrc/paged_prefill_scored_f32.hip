@@ -397,9 +397,9 @@ bool prefill_scored_f32_supported(const PrefillArgs& a, const char** why) {
   return true;
 }
 
-// Against the tokens as rows of the generic kernel, with a cap (12 / 2 heads of 128): 1 token over 300 29.6 us / 40, 64 over
-// 300 33 / 46, 4 x 200 over 300 66 / 251, 8 x 512 over 1536 598 / 4071 (75 TFLOP/s; 384 workgroups for 512 places, the one
-// with two to a CU sets the time); 28 / 4 heads, 4 x 300 over 800: 330 / 1579.  Two accumulators for the scores instead
+// Against the tokens as rows of the generic kernel, with a cap (12 / 2 heads of 128): 1 token over 300 29.8 us / 40, 64 over
+// 300 33 / 46, 4 x 200 over 300 66 / 247, 8 x 512 over 1536 551 / 4081 (82 TFLOP/s; 384 workgroups for 512 places, the one
+// with two to a CU sets the time); 28 / 4 heads, 4 x 300 over 800: 298 / 1575.  Two accumulators for the scores instead
 // of one chain of products: no difference.
 hipError_t launch_prefill_scored_f32(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
   const dim3 block(64 * kWaves);
