@@ -1049,3 +1049,19 @@ def test_decode_f32_is_as_exact_as_f32_is(gpu, heads):
         kernel += (got[i] - outs[0]).square().sum().item()
         plain += (outs[1] - outs[0]).square().sum().item()
     assert kernel <= 1.35**2 * plain, (kernel / plain) ** 0.5
+
+
+@pytest.mark.parametrize("heads,dtype", [("1.5b", torch.bfloat16), ("0.5b", torch.float16), ("one", torch.float16), ("1.5b", torch.float32)])
+@pytest.mark.parametrize("ext", [[150, 70], [9, 20]])
+@pytest.mark.parametrize("cap,slopes", [(0.0, False), (0.0, True), (900.0, False), (900.0, True)])
+def test_extend_scores_that_rise_away_from_the_row(gpu, heads, dtype, ext, cap, slopes):
+    """Keys that grow by leaps with the distance: scores exceed all before them by 2^3 to 2^1000 of probability inside steps that every row sees
+    whole, where nobody looks for a maximum beforehand; and fall back again."""
+    def poison(c, row_req, row_pos, st, sp):
+        for r, n in zip(c["req"].tolist(), c["lens"]):
+            for lo, hi, by in ((600, 700, 1.5), (400, 520, 4.0), (330, 331, 12.0), (200, 280, 25.0), (100, 101, 60.0), (10, 40, 0.1)):
+                slots = c["table"][r, lo : min(hi, n)].long()
+                c["k"][slots] = (c["k"][slots].float() * by).to(dtype)
+
+    extend_case(gpu, heads, dtype, ext, [700, 640], cap=cap, slopes=slopes, seed=80, poison=poison, variant=2, only=60)
+    extend_case(gpu, heads, dtype, ext, [700, 640], cap=cap, slopes=slopes, kind="document", seed=81, poison=poison, variant=2, only=60)
